@@ -10,7 +10,7 @@ NVCC ?= nvcc
 ARCH_FLAGS = -gencode arch=compute_100a,code=sm_100a
 NVCC_FLAGS = -O3 -std=c++17 -lineinfo -Xcompiler -fPIC
 CSRC = megakernel_b200/csrc
-UNITS = $(CSRC)/megakernel.cu $(CSRC)/tp.cu
+UNITS = $(CSRC)/megakernel.cu $(CSRC)/tp.cu $(CSRC)/paged.cu $(CSRC)/kv8_attend.cu
 DEPS = $(wildcard $(CSRC)/*.cu $(CSRC)/*.cuh) include/megakernel.h
 BUILD ?= _build
 LIB_OUT ?= megakernel.so
@@ -25,7 +25,7 @@ $(BUILD)/%.o: $(CSRC)/%.cu $(DEPS)
 	@mkdir -p $(BUILD)
 	$(NVCC) $(ARCH_FLAGS) $(NVCC_FLAGS) -c $< -o $@
 
-$(LIB_OUT) megakernel_b200/libmegakernel.so: $(BUILD)/megakernel.o $(BUILD)/tp.o
+$(LIB_OUT) megakernel_b200/libmegakernel.so: $(UNITS:$(CSRC)/%.cu=$(BUILD)/%.o)
 	$(NVCC) $(ARCH_FLAGS) -shared $^ -o $@
 
 clean:

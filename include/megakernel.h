@@ -256,6 +256,106 @@ int megakernel_tp_info(void* handle, int* rank, int* size);
  * [tp_size][hidden] fp32 on the engine's device.  Synchronous. */
 int megakernel_tp_exchange_slots(void* handle, float* d_out);
 
+/* ---- paged 8-bit serving operators (no reference counterpart) --------------
+ * The parts of a serving step with drafted tokens, each one launch on
+ * `stream` (cudaStream_t, NULL = the default stream) of the current device,
+ * asynchronous, without allocation; all may be captured into a CUDA graph.
+ *
+ * Rows are packed over sequences: sequence b owns rows
+ * [d_starts[b], d_starts[b + 1]), and its first row stands at position
+ * d_first[b]; rows at negative positions are padding (append and read skip
+ * them, attention returns 0 for them).  Position p of sequence b lives in page
+ * d_page_table[b][p / page_size], slot p % page_size.
+ *
+ * Host arguments are checked before the launch.  What lies on the device
+ * (d_starts, d_first, page ids, positions) is checked by the kernels: a work
+ * item whose metadata is out of range is left out, and the first such error
+ * (MK_ERR_INVALID_ARG or MK_ERR_CAPACITY) is kept in *d_status, a device int
+ * that the caller sets to 0 (NULL: not reported). */
+
+enum { MK_TYPE_F32 = 0, MK_TYPE_BF16 = 1, MK_TYPE_F16 = 2 };
+enum { MK_KV8_E4M3 = 0, MK_KV8_INT8 = 1 };
+
+/* q and k head rows [rows][heads][head_dim] (strides in elements, head_dim
+ * contiguous, 16-byte aligned rows), normalised to unit mean square with eps,
+ * times the gain, then rotated: halves (x1, x2) become
+ * (x1 c - x2 s, x2 c + x1 s), c and s = row d_positions[row] of the fp32
+ * tables [table_rows][head_dim / 2] (megakernel_rope_table).  head_dim 64 or
+ * 128; q, k, gains and outputs share `type`; an output may be its input.
+ * A row whose position is outside the tables is not written
+ * (MK_ERR_CAPACITY). */
+typedef struct mk_qk_norm_rope {
+  const void *d_q, *d_k, *d_q_gain, *d_k_gain;
+  void *d_q_out, *d_k_out;
+  const float *d_cos, *d_sin;
+  const int* d_positions;
+  long long q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
+  int table_rows, rows, q_heads, kv_heads, head_dim, type;
+  float eps;
+} mk_qk_norm_rope;
+int megakernel_qk_norm_rope(const mk_qk_norm_rope* args, int* d_status, void* stream);
+
+/* A cache of 8-bit codes in pages, with one fp32 scale per (page, K or V,
+ * head): value = code x scale.  d_codes [num_pages][2][kv_heads][page_size]
+ * [head_dim], page_stride bytes from page to page (a multiple of 16, 16-byte
+ * aligned base); d_scales [num_pages][2][kv_heads], scale_stride floats from
+ * page to page; d_page_table [seqs][table_width], table_stride ints from row
+ * to row.  page_size 16, 32 or 64; head_dim 64 or 128. */
+typedef struct mk_kv8 {
+  void* d_codes;
+  float* d_scales;
+  const int *d_page_table, *d_starts, *d_first;
+  long long page_stride, scale_stride, table_stride;
+  int num_pages, table_width, kv_heads, page_size, head_dim, format, seqs, rows;
+} mk_kv8;
+
+/* Write the rows of d_k and d_v ([rows][kv_heads][head_dim], strides in
+ * elements) at their positions.  The scale of a page is the smallest power of
+ * two 2^e (e >= -126) with max |x| <= 2^e x 448 (e4m3) or 127 (int8) over the
+ * finite values written; a page that holds earlier positions of its sequence
+ * (in front of the first row) keeps the larger of its scale and the new one,
+ * its earlier codes rounded again when it grows.  Codes are x / scale to
+ * nearest even; infinities saturate; NaN stays NaN in e4m3 and becomes 0 in
+ * int8.  No two sequences of a call may write to one page. */
+int megakernel_kv8_append(const mk_kv8* cache, const void* d_k, long long k_row, long long k_head, const void* d_v,
+                          long long v_row, long long v_head, int type, int* d_status, void* stream);
+
+/* The values of the rows' positions back, contiguous [rows][kv_heads]
+ * [head_dim] of `type`.  Rows of padding are not written. */
+int megakernel_kv8_read(const mk_kv8* cache, void* d_k, void* d_v, int type, int* d_status, void* stream);
+
+/* Attention of q rows [rows][q_heads][head_dim] (strides in elements; type
+ * bf16 or f16; q_heads a multiple of kv_heads, query head h reads kv head
+ * h / (q_heads / kv_heads)) over the cache: a row at position p of sequence b
+ * sees the positions j < len_b, with causal also j <= p, with window > 0 also
+ * j > p - window; len_b = d_kv_lens[b], or the position after the sequence's
+ * last row where d_kv_lens is NULL.  d_out [rows][q_heads][head_dim]
+ * contiguous; d_lse (may be NULL) [rows][q_heads] = ln sum exp of the scaled
+ * scores.  A row that sees nothing gives 0 and -inf. */
+int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long long q_row, long long q_head, int q_heads,
+                          int type, float sm_scale, int causal, int window, const int* d_kv_lens, void* d_out,
+                          float* d_lse, int* d_status, void* stream);
+
+/* Keep or refuse drafted tokens.  Row i of sequence b was fed token
+ * d_tokens[starts[b] + i]: row 0 the last confirmed one, the others drafts.
+ * d_target [rows][vocab] fp32: the target's probabilities after each row;
+ * d_draft (may be NULL: each draft was certain) [rows][vocab]: what the next
+ * row's draft was picked from (a sequence's last row is not read);
+ * d_uniforms [rows]: row i decides on draft i + 1; d_sample_u [seqs]; both in
+ * [0, 1).  Draft x after row i is kept iff u q(x) < p(x) and all before it
+ * were.  At the first refusal the token is drawn from max(p - q, 0)
+ * (normalised), after the last row from p, at sample_u of the running sum over
+ * token ids.  d_out [rows]: the kept drafts, the drawn token, then -1;
+ * d_accepted [seqs]: how many drafts were kept.  Probabilities count in units
+ * of 2^-36 and random numbers in units of 2^-24, so the result is exact;
+ * values outside [0, 1] are clamped, NaN is 0; a row may sum to less than 8.
+ * Where max(p - q, 0) is all zero p itself is drawn from; where p is all zero
+ * too the drawn token is -1.  A draft outside the vocabulary is refused. */
+int megakernel_verify_drafts(const int* d_tokens, const float* d_target, long long target_row, const float* d_draft,
+                             long long draft_row, const float* d_uniforms, const float* d_sample_u,
+                             const int* d_starts, int seqs, int rows, int vocab, int* d_out, int* d_accepted,
+                             int* d_status, void* stream);
+
 /* ---- host-only helpers (no GPU needed) ----------------------------------- */
 
 /* Shape id matching a flat-binary offsets array, or MK_ERR_SHAPE. */

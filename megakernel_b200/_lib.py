@@ -17,9 +17,9 @@ LIB_PATH = os.path.join(PKG_DIR, "libmegakernel.so")
 HEADER = os.path.join(ROOT, "include", "megakernel.h")
 SOURCES = [os.path.join(CSRC, f) for f in ("megakernel.cu", "noalloc.cu", "decode_kernel.cuh", "ptx.cuh",
                                                   "shapes.cuh", "batch.cu", "tc_gemm.cuh", "tc_ptx.cuh",
-                                                  "tp.cu")]
+                                                  "tp.cu", "paged.cuh", "paged.cu", "kv8_attend.cu")]
 # Translation units, compiled in parallel and linked into one library.
-UNITS = ["megakernel.cu", "tp.cu"]
+UNITS = ["megakernel.cu", "tp.cu", "paged.cu", "kv8_attend.cu"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
@@ -71,6 +71,22 @@ class MkOptions(ctypes.Structure):
     _fields_ = [("device", ctypes.c_int), ("shape_id", ctypes.c_int), ("max_seq", ctypes.c_int),
                 ("num_ctas", ctypes.c_int), ("timeout_ns", ctypes.c_longlong),
                 ("debug_skip_cta", ctypes.c_int)]
+
+
+class MkQkNormRope(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "q_gain", "k_gain", "q_out", "k_out", "cos", "sin",
+                                               "positions")] + \
+               [(n, ctypes.c_longlong) for n in ("q_row", "q_head", "k_row", "k_head", "qo_row", "qo_head",
+                                                 "ko_row", "ko_head")] + \
+               [(n, ctypes.c_int) for n in ("table_rows", "rows", "q_heads", "kv_heads", "head_dim", "type")] + \
+               [("eps", ctypes.c_float)]
+
+
+class MkKv8(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scales", "page_table", "starts", "first")] + \
+               [(n, ctypes.c_longlong) for n in ("page_stride", "scale_stride", "table_stride")] + \
+               [(n, ctypes.c_int) for n in ("num_pages", "table_width", "kv_heads", "page_size", "head_dim",
+                                            "format", "seqs", "rows")]
 
 
 def signatures() -> dict:
@@ -129,6 +145,13 @@ def signatures() -> dict:
         "megakernel_tp_connect": ([vp, vp], c_int),
         "megakernel_tp_info": ([vp, ip, ip], c_int),
         "megakernel_tp_exchange_slots": ([vp, vp], c_int),
+        "megakernel_qk_norm_rope": ([ctypes.POINTER(MkQkNormRope), vp, vp], c_int),
+        "megakernel_kv8_append": ([ctypes.POINTER(MkKv8), vp, c_ll, c_ll, vp, c_ll, c_ll, c_int, vp, vp], c_int),
+        "megakernel_kv8_read": ([ctypes.POINTER(MkKv8), vp, vp, c_int, vp, vp], c_int),
+        "megakernel_kv8_attend": ([ctypes.POINTER(MkKv8), vp, c_ll, c_ll, c_int, c_int, ctypes.c_float, c_int,
+                                   c_int, vp, vp, vp, vp, vp], c_int),
+        "megakernel_verify_drafts": ([vp, vp, c_ll, vp, c_ll, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp, vp],
+                                     c_int),
         "megakernel_infer_shape": ([llp, c_int], c_int),
         "megakernel_rope_table": ([c_int, ctypes.c_double, c_int, fp, fp], c_int),
         "megakernel_plan_bytes": ([c_int, c_int, c_int, llp], c_int),

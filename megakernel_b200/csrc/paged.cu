@@ -1,0 +1,485 @@
+// Paged 8-bit serving operators: norm + rotation of queries and keys, the
+// write of keys and values into the 8-bit cache, its read-back, and the
+// verification of drafted tokens (C ABI in include/megakernel.h).  Attention
+// over the cache is in kv8_attend.cu.  The reference has no counterpart.
+#include "paged.cuh"
+
+namespace mkp {
+
+// ---- norm of each head and rotation -------------------------------------------
+//
+//   y = x g / sqrt(mean(x^2) + eps),  o1 = y1 cos - y2 sin,  o2 = y2 cos + y1 sin
+//
+// for the two halves (1, 2) of a head row of D.  A group of D/16 lanes holds a
+// row: lane l its elements [8l, 8l+8) of both halves, so that the rotation
+// stays in the lane and the sum of squares is the only exchange.  fp32
+// throughout, one rounding at the store.
+struct NormRope {
+  const void *q, *k, *q_gain, *k_gain;
+  void *q_out, *k_out;
+  const float *cos, *sin;
+  const int* positions;
+  long long q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
+  int table_rows, rows, q_heads, kv_heads;
+  float eps;
+  int* status;
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(128) norm_rope_kernel(const NormRope a) {
+  constexpr int kLanes = D / 16, kHalf = D / 2;
+  const int heads = a.q_heads + a.kv_heads;
+  const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
+  const int l = threadIdx.x % kLanes;
+  if (item >= (long long)a.rows * heads) return;   // whole groups leave together
+  const int row = (int)(item / heads), h = (int)(item % heads);
+  const bool is_q = h < a.q_heads;
+  const T* x = is_q ? (const T*)a.q + row * a.q_row + h * a.q_head
+                    : (const T*)a.k + row * a.k_row + (h - a.q_heads) * a.k_head;
+  T* o = is_q ? (T*)a.q_out + row * a.qo_row + h * a.qo_head
+              : (T*)a.k_out + row * a.ko_row + (h - a.q_heads) * a.ko_head;
+  const T* g = (const T*)(is_q ? a.q_gain : a.k_gain);
+  Vec8<T> x1, x2, g1, g2;
+  x1.load(x + 8 * l);
+  x2.load(x + kHalf + 8 * l);
+  g1.load(g + 8 * l);
+  g2.load(g + kHalf + 8 * l);
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss += x1.f(i) * x1.f(i) + x2.f(i) * x2.f(i);
+  const unsigned group = ((1u << kLanes) - 1u) << ((threadIdx.x & 31) / kLanes * kLanes);
+#pragma unroll
+  for (int s = kLanes / 2; s > 0; s >>= 1) ss += __shfl_xor_sync(group, ss, s);
+  const float r = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+  const int pos = __ldg(a.positions + row);
+  if (pos < 0 || pos >= a.table_rows) {
+    if (l == 0) report(a.status, MK_ERR_CAPACITY);
+    return;
+  }
+  const float* c = a.cos + (long long)pos * kHalf + 8 * l;
+  const float* s = a.sin + (long long)pos * kHalf + 8 * l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y1 = x1.f(i) * r * g1.f(i), y2 = x2.f(i) * r * g2.f(i);
+    x1.set(i, y1 * c[i] - y2 * s[i]);
+    x2.set(i, y2 * c[i] + y1 * s[i]);
+  }
+  x1.store(o + 8 * l);
+  x2.store(o + kHalf + 8 * l);
+}
+
+// ---- cache write ------------------------------------------------------------------
+//
+// One block of threads per (page that new rows fall into, K or V, head).  The
+// page's scale is the smallest power of two that fits its largest magnitude;
+// if the page already holds earlier positions the scale only grows, and then
+// the earlier codes are rounded again to the larger one.  A power of two makes
+// x / scale exact, so the codes do not depend on how the division is done, and
+// growing the scale of e4m3 codes loses nothing but what falls below the
+// smallest subnormal.
+template <class T, class F, int P, int D>
+__global__ void __launch_bounds__(128) append_kernel(const Cache c, const T* k, const T* v, long long k_row,
+                                                     long long k_head, long long v_row, long long v_head,
+                                                     int* status) {
+  constexpr int kLanes = D / 16, kRows = 128 / kLanes;   // 16 elements per thread, kRows rows per pass
+  constexpr int kPasses = (P + kRows - 1) / kRows;
+  Block blk;
+  if (!block_of<P>(c, (int)blockIdx.x, &blk, status)) return;
+  const Span s = blk.s;
+  const int pg = blk.blk, p0 = blk.p0, p1 = blk.p1;
+  const int id = page_id(c, blk.b, pg, status);
+  if (id < 0) return;
+  const int h = blockIdx.y >> 1, kv = blockIdx.y & 1;
+  const T* src = kv ? v + h * v_head : k + h * k_head;
+  const long long src_row = kv ? v_row : k_row;
+  const int lane = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
+  const int keep = p0 - pg * P, end = p1 - pg * P;   // slots [0, keep) held, [keep, end) new
+  uint8_t* dst = c.codes + id * c.page_stride + (long long)(kv * c.kv_heads + h) * P * D;
+  float* scale = c.scales + id * c.scale_stride + kv * c.kv_heads + h;
+
+  Vec8<T> x[kPasses][2];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int slot = i * kRows + sub;
+    if (slot < keep || slot >= end) continue;
+    const T* p = src + (s.row + (pg * P + slot - s.pos)) * src_row + 16 * lane;
+    x[i][0].load(p);
+    x[i][1].load(p + 8);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float m = fabsf(x[i][j >> 3].f(j & 7));
+      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);   // finite values only
+    }
+  }
+  amax = mk::warp_max(amax);
+  __shared__ float part[4];
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  float sc = scale_for<F>(amax);
+  if (keep > 0) {
+    const float old = *scale;
+    sc = fmaxf(sc, old);
+    if (sc != old) {
+      const float ratio = old / sc;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int slot = i * kRows + sub;
+        if (slot >= keep) continue;
+        uint4* p = reinterpret_cast<uint4*>(dst + slot * D + 16 * lane);
+        uint4 w = *p;
+        uint8_t* e = reinterpret_cast<uint8_t*>(&w);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) e[j] = F::encode(F::decode(e[j]) * ratio);
+        *p = w;
+      }
+    }
+  }
+  const float inv = 1.f / sc;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int slot = i * kRows + sub;
+    if (slot < keep || slot >= end) continue;
+    uint4 w;
+    uint8_t* e = reinterpret_cast<uint8_t*>(&w);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) e[j] = F::encode(x[i][j >> 3].f(j & 7) * inv);
+    *reinterpret_cast<uint4*>(dst + slot * D + 16 * lane) = w;
+  }
+  __syncthreads();   // every thread has read the old scale
+  if (threadIdx.x == 0) *scale = sc;
+}
+
+// ---- cache read -------------------------------------------------------------------
+template <class T, class F, int P, int D>
+__global__ void __launch_bounds__(256) read_kernel(const Cache c, T* k, T* v, int* status) {
+  Block blk;
+  if (!block_of<P>(c, (int)blockIdx.x, &blk, status)) return;
+  const Span s = blk.s;
+  const int pg = blk.blk, p0 = blk.p0, p1 = blk.p1;
+  const int id = page_id(c, blk.b, pg, status);
+  if (id < 0) return;
+  const uint8_t* src = c.codes + id * c.page_stride;
+  const float* scale = c.scales + id * c.scale_stride;
+  constexpr int kVecs = D / 16;
+  const int total = 2 * c.kv_heads * P * kVecs;
+  for (int i = threadIdx.x; i < total; i += blockDim.x) {
+    const int vec = i % kVecs, slot = i / kVecs % P, kh = i / (kVecs * P);
+    const int pos = pg * P + slot;
+    if (pos < p0 || pos >= p1) continue;
+    const uint4 w = *reinterpret_cast<const uint4*>(src + (long long)i * 16);
+    const uint8_t* e = reinterpret_cast<const uint8_t*>(&w);
+    const float sc = __ldg(scale + kh);
+    const int kv = kh >= c.kv_heads, h = kh - kv * c.kv_heads;
+    T* o = (kv ? v : k) + ((long long)(s.row + pos - s.pos) * c.kv_heads + h) * D + 16 * vec;
+    Vec8<T> y;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y.set(j, F::decode(e[8 * g + j]) * sc);
+      y.store(o + 8 * g);
+    }
+  }
+}
+
+// ---- verification of drafted tokens --------------------------------------------------
+//
+// Probabilities are taken in units of 2^-36 and random numbers in units of
+// 2^-24 (P, Q, U below, whole numbers), so that every comparison and sum is
+// exact and the tokens do not depend on the order of summation:
+//   draft x of row r is kept iff U_r Q_r(x) < P_r(x) 2^24;
+//   the first row that keeps none (or the last row) is sampled from
+//   R = max(P - Q, 0) (or P, for the last row, or if R is all zero) at the
+//   first token whose running sum exceeds floor(U' sum(R) / 2^24).
+// Products stay below 2^63 while a row's probabilities sum to less than 8.
+constexpr int kFix = 36, kFixU = 24;
+
+__device__ __forceinline__ long long fix_p(float p) {
+  return p > 0.f ? __float2ll_rn(fminf(p, 1.f) * 68719476736.f) : 0;   // NaN: 0
+}
+__device__ __forceinline__ long long fix_u(float u) {
+  return u > 0.f ? (long long)(fminf(u, 1.f) * 16777216.f) : 0;
+}
+
+struct Verify {
+  const int* tokens;
+  const float *target, *draft, *uniforms, *sample_u;
+  long long target_row, draft_row;
+  const int* starts;
+  int seqs, rows, vocab;
+  int *out, *accepted, *status;
+};
+
+constexpr int kVerifyThreads = 1024;
+
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const Verify a) {
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int r0 = __ldg(a.starts + b), r1 = __ldg(a.starts + b + 1);
+  if (r0 < 0 || r1 < r0 || r1 > a.rows) {
+    if (tid == 0) {
+      report(a.status, MK_ERR_INVALID_ARG);
+      a.accepted[b] = 0;
+    }
+    return;
+  }
+  const int n = r1 - r0;
+  if (n == 0) {
+    if (tid == 0) a.accepted[b] = 0;
+    return;
+  }
+  // rows in order: the first draft that is refused
+  __shared__ int s_acc;
+  __shared__ long long s_part[kVerifyThreads / 32], s_base;
+  __shared__ int s_token;
+  if (tid == 0) s_acc = n - 1;
+  __syncthreads();
+  for (int i = tid; i < n - 1; i += kVerifyThreads) {
+    const int x = a.tokens[r0 + i + 1];
+    bool keep = false;
+    if (x >= 0 && x < a.vocab) {
+      const long long p = fix_p(a.target[(r0 + i) * a.target_row + x]);
+      const long long q = a.draft ? fix_p(a.draft[(r0 + i) * a.draft_row + x]) : 1LL << kFix;
+      keep = fix_u(a.uniforms[r0 + i]) * q < (p << kFixU);
+    }
+    if (!keep) atomicMin(&s_acc, i);
+  }
+  __syncthreads();
+  const int acc = s_acc;
+  const bool refused = acc < n - 1;
+  const float* p = a.target + (r0 + acc) * a.target_row;
+  const float* q = refused && a.draft ? a.draft + (r0 + acc) * a.draft_row : nullptr;
+  const int banned = refused && !a.draft ? a.tokens[r0 + acc + 1] : -1;
+  int token = -1;
+  for (int fallback = 0; fallback < 2; ++fallback) {
+    auto weight = [&](int t) {
+      long long w = fix_p(p[t]);
+      if (!fallback) {
+        if (q) w = max(w - fix_p(q[t]), 0LL);
+        if (t == banned) w = 0;
+      }
+      return w;
+    };
+    // each thread owns a contiguous run of tokens
+    const int run = (a.vocab + kVerifyThreads - 1) / kVerifyThreads;
+    const int t0 = min(tid * run, a.vocab), t1 = min(t0 + run, a.vocab);
+    long long mine = 0;
+    for (int t = t0; t < t1; ++t) mine += weight(t);
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, upto, o);
+      if ((tid & 31) >= o) upto += other;
+    }
+    if ((tid & 31) == 31) s_part[tid >> 5] = upto;
+    if (tid == 0) s_token = -1;
+    __syncthreads();
+    if (tid < 32) {
+      long long w = s_part[tid];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, w, o);
+        if (tid >= o) w += other;
+      }
+      s_part[tid] = w;
+      if (tid == 31) s_base = w;
+    }
+    __syncthreads();
+    const long long total = s_base;
+    if (tid >= 32) upto += s_part[(tid >> 5) - 1];
+    if (total > 0) {
+      const long long bar = (fix_u(a.sample_u[b]) * total) >> kFixU;
+      if (upto - mine <= bar && bar < upto) {
+        long long sum = upto - mine;
+        for (int t = t0; t < t1; ++t) {
+          sum += weight(t);
+          if (sum > bar) {
+            s_token = t;
+            break;
+          }
+        }
+      }
+      __syncthreads();
+      token = s_token;
+      break;
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += kVerifyThreads)
+    a.out[r0 + i] = i < acc ? a.tokens[r0 + i + 1] : i == acc ? token : -1;
+  if (tid == 0) a.accepted[b] = acc;
+}
+
+// ---- host side -----------------------------------------------------------------------
+
+static int launched() { return cudaGetLastError() == cudaSuccess ? MK_OK : MK_ERR_CUDA; }
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows and heads that a kernel reads in 16-byte vectors.
+static bool strides_ok(long long row, long long head, int size) {
+  return row >= 0 && head >= 0 && row * size % 16 == 0 && head * size % 16 == 0;
+}
+
+static int type_size(int type) { return type == MK_TYPE_F32 ? 4 : 2; }
+static bool type_ok(int type) { return type == MK_TYPE_F32 || type == MK_TYPE_BF16 || type == MK_TYPE_F16; }
+
+// The arguments every cache operator shares.  Returns MK_OK and fills *c.
+int cache_of(const mk_kv8* m, Cache* c) {
+  if (!m) return MK_ERR_INVALID_ARG;
+  if (m->seqs < 0 || m->rows < 0 || m->num_pages < 0 || m->table_width < 0 || m->kv_heads < 1 || m->kv_heads > 1024)
+    return MK_ERR_INVALID_ARG;
+  if (m->head_dim != 64 && m->head_dim != 128) return MK_ERR_INVALID_ARG;
+  if (m->page_size != 16 && m->page_size != 32 && m->page_size != 64) return MK_ERR_INVALID_ARG;
+  if (m->format != MK_KV8_E4M3 && m->format != MK_KV8_INT8) return MK_ERR_INVALID_ARG;
+  const long long page = 2LL * m->kv_heads * m->page_size * m->head_dim;
+  if (m->page_stride < page || m->page_stride % 16 || m->scale_stride < 2LL * m->kv_heads ||
+      m->table_stride < m->table_width)
+    return MK_ERR_INVALID_ARG;
+  if (m->seqs > 0 && m->rows > 0 &&
+      (!m->d_codes || !m->d_scales || !m->d_page_table || !m->d_starts || !m->d_first || !aligned16(m->d_codes)))
+    return MK_ERR_INVALID_ARG;
+  // item numbers (rows / 16 + 2 seqs at most) and row numbers are 32-bit
+  if (m->seqs > (1 << 24) || m->rows > (1 << 29) || m->table_width > (1 << 24)) return MK_ERR_INVALID_ARG;
+  c->codes = (uint8_t*)m->d_codes;
+  c->scales = m->d_scales;
+  c->table = m->d_page_table;
+  c->starts = m->d_starts;
+  c->first = m->d_first;
+  c->page_stride = m->page_stride;
+  c->scale_stride = m->scale_stride;
+  c->table_stride = m->table_stride;
+  c->num_pages = m->num_pages;
+  c->table_width = m->table_width;
+  c->kv_heads = m->kv_heads;
+  c->seqs = m->seqs;
+  c->rows = m->rows;
+  return MK_OK;
+}
+
+// Calls f with the compile-time page size and head size of m (checked before).
+template <class Fn>
+static int by_page(const mk_kv8* m, Fn f) {
+  auto with_d = [&](auto page) {
+    return m->head_dim == 64 ? f(page, std::integral_constant<int, 64>{})
+                             : f(page, std::integral_constant<int, 128>{});
+  };
+  if (m->page_size == 16) return with_d(std::integral_constant<int, 16>{});
+  if (m->page_size == 32) return with_d(std::integral_constant<int, 32>{});
+  return with_d(std::integral_constant<int, 64>{});
+}
+template <class Fn>
+static int by_type(int type, Fn f) {
+  if (type == MK_TYPE_F32) return f(float{});
+  if (type == MK_TYPE_BF16) return f(__nv_bfloat16{});
+  return f(__half{});
+}
+template <class Fn>
+static int by_format(int format, Fn f) {
+  return format == MK_KV8_E4M3 ? f(E4M3{}) : f(I8{});
+}
+
+}  // namespace mkp
+
+using namespace mkp;
+
+extern "C" {
+
+int megakernel_qk_norm_rope(const mk_qk_norm_rope* m, int* d_status, void* stream) {
+  if (!m || m->rows < 0 || m->q_heads < 0 || m->kv_heads < 0 || m->table_rows < 0 || !type_ok(m->type))
+    return MK_ERR_INVALID_ARG;
+  if (m->head_dim != 64 && m->head_dim != 128) return MK_ERR_INVALID_ARG;
+  if (!(m->eps >= 0.f)) return MK_ERR_INVALID_ARG;
+  const long long heads = (long long)m->q_heads + m->kv_heads;
+  if (m->rows == 0 || heads == 0) return MK_OK;
+  const int size = type_size(m->type);
+  const void* must[] = {m->d_cos, m->d_sin, m->d_positions};
+  for (const void* p : must)
+    if (!p) return MK_ERR_INVALID_ARG;
+  if (m->q_heads > 0 && (!m->d_q || !m->d_q_out || !m->d_q_gain || !aligned16(m->d_q) || !aligned16(m->d_q_out) ||
+                         !aligned16(m->d_q_gain) || !strides_ok(m->q_row, m->q_head, size) ||
+                         !strides_ok(m->qo_row, m->qo_head, size)))
+    return MK_ERR_INVALID_ARG;
+  if (m->kv_heads > 0 && (!m->d_k || !m->d_k_out || !m->d_k_gain || !aligned16(m->d_k) || !aligned16(m->d_k_out) ||
+                          !aligned16(m->d_k_gain) || !strides_ok(m->k_row, m->k_head, size) ||
+                          !strides_ok(m->ko_row, m->ko_head, size)))
+    return MK_ERR_INVALID_ARG;
+  const int lanes = m->head_dim / 16;
+  const long long blocks = ((long long)m->rows * heads * lanes + 127) / 128;
+  if (blocks > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
+  NormRope a{m->d_q, m->d_k, m->d_q_gain, m->d_k_gain, m->d_q_out, m->d_k_out, m->d_cos, m->d_sin, m->d_positions,
+             m->q_row, m->q_head, m->k_row, m->k_head, m->qo_row, m->qo_head, m->ko_row, m->ko_head,
+             m->table_rows, m->rows, m->q_heads, m->kv_heads, m->eps, d_status};
+  return by_type(m->type, [&](auto t) {
+    using T = decltype(t);
+    if (m->head_dim == 64)
+      norm_rope_kernel<T, 64><<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a);
+    else
+      norm_rope_kernel<T, 128><<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a);
+    return launched();
+  });
+}
+
+int megakernel_kv8_append(const mk_kv8* cache, const void* d_k, long long k_row, long long k_head, const void* d_v,
+                          long long v_row, long long v_head, int type, int* d_status, void* stream) {
+  Cache c;
+  const int rc = cache_of(cache, &c);
+  if (rc != MK_OK) return rc;
+  if (!type_ok(type)) return MK_ERR_INVALID_ARG;
+  if (c.seqs == 0 || c.rows == 0) return MK_OK;
+  const int size = type_size(type);
+  if (!d_k || !d_v || !aligned16(d_k) || !aligned16(d_v) || !strides_ok(k_row, k_head, size) ||
+      !strides_ok(v_row, v_head, size))
+    return MK_ERR_INVALID_ARG;
+  const dim3 grid((unsigned)item_count(c.rows, c.seqs, cache->page_size), 2 * c.kv_heads);
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    return by_format(cache->format, [&](auto f) {
+      using F = decltype(f);
+      return by_page(cache, [&](auto p, auto d) {
+        append_kernel<T, F, decltype(p)::value, decltype(d)::value><<<grid, 128, 0, (cudaStream_t)stream>>>(
+            c, (const T*)d_k, (const T*)d_v, k_row, k_head, v_row, v_head, d_status);
+        return launched();
+      });
+    });
+  });
+}
+
+int megakernel_kv8_read(const mk_kv8* cache, void* d_k, void* d_v, int type, int* d_status, void* stream) {
+  Cache c;
+  const int rc = cache_of(cache, &c);
+  if (rc != MK_OK) return rc;
+  if (!type_ok(type)) return MK_ERR_INVALID_ARG;
+  if (c.seqs == 0 || c.rows == 0) return MK_OK;
+  if (!d_k || !d_v || !aligned16(d_k) || !aligned16(d_v)) return MK_ERR_INVALID_ARG;
+  const unsigned grid = (unsigned)item_count(c.rows, c.seqs, cache->page_size);
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    return by_format(cache->format, [&](auto f) {
+      using F = decltype(f);
+      return by_page(cache, [&](auto p, auto d) {
+        read_kernel<T, F, decltype(p)::value, decltype(d)::value><<<grid, 256, 0, (cudaStream_t)stream>>>(
+            c, (T*)d_k, (T*)d_v, d_status);
+        return launched();
+      });
+    });
+  });
+}
+
+int megakernel_verify_drafts(const int* d_tokens, const float* d_target, long long target_row, const float* d_draft,
+                             long long draft_row, const float* d_uniforms, const float* d_sample_u,
+                             const int* d_starts, int seqs, int rows, int vocab, int* d_out, int* d_accepted,
+                             int* d_status, void* stream) {
+  if (seqs < 0 || rows < 0 || vocab < 1 || rows > (1 << 30)) return MK_ERR_INVALID_ARG;
+  if (seqs == 0) return MK_OK;
+  if (!d_starts || !d_accepted) return MK_ERR_INVALID_ARG;
+  if (rows > 0 && (!d_tokens || !d_target || !d_uniforms || !d_sample_u || !d_out || target_row < vocab ||
+                   (d_draft && draft_row < vocab)))
+    return MK_ERR_INVALID_ARG;
+  const Verify a{d_tokens, d_target, d_draft, d_uniforms, d_sample_u, target_row, draft_row,
+                 d_starts, seqs, rows, vocab, d_out, d_accepted, d_status};
+  verify_kernel<<<(unsigned)seqs, kVerifyThreads, 0, (cudaStream_t)stream>>>(a);
+  return launched();
+}
+
+}  // extern "C"

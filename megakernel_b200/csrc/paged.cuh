@@ -1,0 +1,193 @@
+// Shared pieces of the paged 8-bit serving operators (qk_norm_rope,
+// kv8_append, kv8_read, kv8_attend, verify_drafts): element types, the map
+// from packed rows to sequences, and the two code formats.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+
+#include "../../include/megakernel.h"
+#include "ptx.cuh"
+
+namespace mkp {
+
+// ---- status word -------------------------------------------------------------
+// Device-side metadata (row starts, positions, page ids) cannot be checked on
+// the host without a synchronisation.  The kernels check it, leave the work
+// item out and keep the first error here.
+__device__ __forceinline__ void report(int* status, int code) {
+  if (status) atomicCAS(status, MK_OK, code);
+}
+
+// ---- element types -------------------------------------------------------------
+template <class T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float to_f32(float v) { return v; }
+  static __device__ __forceinline__ float from_f32(float v) { return v; }
+};
+template <> struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Elem<__half> {
+  static __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+};
+
+// Eight consecutive elements as they lie in memory: one 16-byte vector for the
+// 16-bit types, two for fp32.
+template <class T>
+struct alignas(16) Vec8 {
+  T v[8];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+    } else {
+      reinterpret_cast<uint4*>(v)[0] = reinterpret_cast<const uint4*>(p)[0];
+      reinterpret_cast<uint4*>(v)[1] = reinterpret_cast<const uint4*>(p)[1];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+    } else {
+      reinterpret_cast<uint4*>(p)[0] = reinterpret_cast<const uint4*>(v)[0];
+      reinterpret_cast<uint4*>(p)[1] = reinterpret_cast<const uint4*>(v)[1];
+    }
+  }
+  __device__ __forceinline__ float f(int i) const { return Elem<T>::to_f32(v[i]); }
+  __device__ __forceinline__ void set(int i, float x) { v[i] = Elem<T>::from_f32(x); }
+};
+
+// ---- the cache -------------------------------------------------------------------
+// codes [num_pages][2][kv_heads][page_size][head_dim], scales [num_pages][2][kv_heads];
+// the page strides are the caller's (bytes of codes, floats of scales).
+struct Cache {
+  uint8_t* codes;
+  float* scales;
+  const int* table;    // [seqs][table_width] page ids
+  const int* starts;   // [seqs + 1] first packed row of each sequence
+  const int* first;    // [seqs] position of that row
+  long long page_stride, scale_stride, table_stride;
+  int num_pages, table_width, kv_heads, seqs, rows;
+};
+
+// Largest b in [0, n) with key(b) <= x, for a non-decreasing key with
+// key(0) <= x: a 32-way search by the whole warp (two dependent loads for
+// 1,024 sequences).
+template <class F>
+__device__ __forceinline__ int warp_search(int n, int x, F key) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5;
+    const int at = lane * step;
+    const bool below = at < n && key(lo + at) <= x;
+    const int k = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return lo;
+}
+
+// The rows of sequence b as the kernels may use them: packed rows
+// [row, row + count) at positions [pos, pos + count).  Rows at negative
+// positions are left out (they stand for padding).
+struct Span {
+  int row, pos, count;
+};
+__device__ __forceinline__ bool span_of(const Cache& c, int b, Span* s, int* status) {
+  const int r0 = __ldg(c.starts + b), r1 = __ldg(c.starts + b + 1);
+  int p = __ldg(c.first + b);
+  s->row = s->pos = s->count = 0;
+  if (r0 < 0 || r1 < r0 || r1 > c.rows || p > (1 << 30)) {
+    report(status, MK_ERR_INVALID_ARG);
+    return false;
+  }
+  const int skip = p < 0 ? (int)min((long long)(r1 - r0), -(long long)p) : 0;
+  s->row = r0 + skip;
+  s->count = r1 - r0 - skip;
+  s->pos = p + skip;   // still negative only if no row is left
+  return s->count > 0;
+}
+
+// Work items that each hold the rows of one sequence inside one block of `u`
+// positions: sequence b owns the item numbers from starts[b] / u + 2 b on, which
+// leaves room for its at most count / u + 2 blocks, so no prefix sum over the
+// sequences is needed.  item_count bounds the numbers.
+__host__ __device__ inline long long item_count(long long rows, long long seqs, int u) {
+  return rows / u + 2 * seqs;
+}
+
+// The part of a sequence's rows that work item `item` stands for: block `blk`
+// of u positions, positions [p0, p1) of it.  False if the item is spare.
+struct Block {
+  int b, blk, p0, p1;
+  Span s;
+};
+template <int U>
+__device__ __forceinline__ bool block_of(const Cache& c, int item, Block* k, int* status) {
+  const int b = warp_search(c.seqs, item, [&](int i) { return __ldg(c.starts + i) / U + 2 * i; });
+  k->b = b;
+  if (!span_of(c, b, &k->s, status)) return false;
+  const int j = item - (__ldg(c.starts + b) / U + 2 * b);
+  k->blk = k->s.pos / U + j;
+  if (j < 0 || k->blk > (k->s.pos + k->s.count - 1) / U) return false;
+  k->p0 = max(k->s.pos, k->blk * U);
+  k->p1 = min(k->s.pos + k->s.count, k->blk * U + U);
+  return true;
+}
+
+// Page id of page `pg` of sequence b, or -1 (reported) if the table ends
+// before it or the id is no page of the pool.
+__device__ __forceinline__ int page_id(const Cache& c, int b, int pg, int* status) {
+  if (pg >= c.table_width) {
+    report(status, MK_ERR_CAPACITY);
+    return -1;
+  }
+  const int id = __ldg(c.table + (long long)b * c.table_stride + pg);
+  if (id < 0 || id >= c.num_pages) {
+    report(status, MK_ERR_INVALID_ARG);
+    return -1;
+  }
+  return id;
+}
+
+// ---- code formats ----------------------------------------------------------------
+struct E4M3 {
+  static constexpr float kMax = 448.f;       // 1.75 x 2^8
+  static constexpr uint32_t kTopMant = 0x600000u;   // mantissa bits of 1.75
+  static constexpr int kTopExp = 8;
+  // Nearest code, ties to even; out of range saturates; NaN stays NaN.
+  static __device__ __forceinline__ uint8_t encode(float x) {
+    return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  }
+  static __device__ __forceinline__ float decode(uint8_t c) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3);
+    return __half2float(__half(h));
+  }
+};
+struct I8 {
+  static constexpr float kMax = 127.f;       // 1.984375 x 2^6
+  static constexpr uint32_t kTopMant = 0x7e0000u;
+  static constexpr int kTopExp = 6;
+  // Nearest code, ties to even; out of range saturates; NaN has no code and
+  // becomes 0 (fmaxf returns the other operand).
+  static __device__ __forceinline__ uint8_t encode(float x) {
+    x = x != x ? 0.f : fminf(fmaxf(x, -127.f), 127.f);
+    return (uint8_t)(int8_t)__float2int_rn(x);
+  }
+  static __device__ __forceinline__ float decode(uint8_t c) { return (float)(int8_t)c; }
+};
+
+// Smallest power of two 2^e, e >= -126, with amax <= kMax 2^e.
+template <class F>
+__device__ __forceinline__ float scale_for(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = (int)(b >> 23) - 127 - F::kTopExp + ((b & 0x7fffffu) > F::kTopMant ? 1 : 0);
+  return __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
+}
+
+}  // namespace mkp
