@@ -11,83 +11,556 @@ struct Attend {
   long long q_row, q_head;
   int q_heads, causal, window;
   float scale;   // log2(e) x the softmax scale
+  int bf16;      // q and out: bf16, else f16
   int* status;
 };
 
-// One block of four warps per (row, query head); each warp walks every fourth
-// position with a running maximum and sum, and the four are joined at the end.
-template <class T, class F, int P, int D>
-__global__ void __launch_bounds__(128) attend_simple_kernel(const Cache c, const Attend a) {
-  constexpr int kPer = D / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x, hq = blockIdx.y, group = a.q_heads / c.kv_heads, h = hq / group;
-  const int b = warp_search(c.seqs, row, [&](int i) { return __ldg(c.starts + i); });
+// ---- warp-level pieces ---------------------------------------------------------------
+
+// D[16x8] += A[16x16] B[16x8], f16 in, fp32 accumulate.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two codes (the low or the high half of w) -> f16x2, exactly: e4m3 and the
+// whole numbers to 127 are f16 values.
+template <class F> __device__ __forceinline__ void expand(uint32_t w, uint32_t& lo, uint32_t& hi);
+template <> __device__ __forceinline__ void expand<E4M3>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// 0x6400 + b is the f16 value 1024 + b for a byte b; codes are biased by 128.
+template <> __device__ __forceinline__ void expand<I8>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 bias = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+  uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 a = __hsub2(*reinterpret_cast<__half2*>(&x), bias);
+  const __half2 b = __hsub2(*reinterpret_cast<__half2*>(&y), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Bits 7 of the bytes of w that are e4m3 NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+__device__ __forceinline__ float load_q(const void* q, long long i, bool bf16) {
+  return bf16 ? __bfloat162float(((const __nv_bfloat16*)q)[i]) : __half2float(((const __half*)q)[i]);
+}
+__device__ __forceinline__ void store_out(void* o, long long i, float v, bool bf16) {
+  if (bf16) ((__nv_bfloat16*)o)[i] = __float2bfloat16_rn(v);
+  else ((__half*)o)[i] = __float2half_rn(v);
+}
+
+// Every thread of every block of the cluster arrives and waits.
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The word at p's place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ float remote_f32(const float* p, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mk::smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+
+constexpr int kStages = 4;
+constexpr int kWarps = 4;
+constexpr int kStageBytes = 4096;      // K and V of one step
+constexpr uint32_t kWaitLimit = 1u << 22;
+
+// Bounded wait; each probe may itself suspend for a while.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i)
+    if (mk::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
+template <int D, int MW>
+constexpr int rows_smem() {
+  constexpr int ring = (kWarps / MW) * kStages * kStageBytes, parts = kWarps * 16 * D * 4;
+  return ring > parts ? ring : parts;
+}
+
+// ---- attention of few rows per sequence -------------------------------------------------
+//
+// Work item: (16 MW rows of one sequence and kv head, counting a row once per
+// query head of the group; the positions split over the S blocks of a cluster
+// and their warps).  MW warps that hold 16 rows each share a stream of steps
+// of TS positions; the 4 / MW such groups of a block, and the blocks of the
+// cluster, take every (4 / MW) S-th step.
+//
+// The codes of a step, contiguous in a page, arrive by bulk copies in a ring
+// of four stages per group (K 2 KB and V 2 KB each): nothing of the stream
+// passes through registers before it is used.  Scores and output are
+// m16n8k16 f16 products with fp32 accumulation.  The order of the head
+// dimension in the first product and of the output columns in the second is
+// free, so a lane reads 16 consecutive bytes of K (its part of four k-steps)
+// and 8 or 16 consecutive bytes of V from each of four positions; the code
+// bytes become f16 in registers, exactly.  q is brought to 2^14 by a power of
+// two per row (bf16 values fit f16 then, 2^-39 of the row's largest lost at
+// most).
+//
+// Softmax per row with running maximum m and sum l of p = 2^(s - m), fp32.
+// The scale of a K page multiplies the scores, that of a V page the weights:
+// w = 2^15 p scale / vref, vref the largest V scale so far, goes into the second
+// product in f16: 11 bits down to 2^-29 of the row's largest, an absolute 2^-40
+// below that (at 1 instead of 2^15 it was 2^-25, which rows with one dominant
+// position showed).  The sum l takes the unrounded p.
+template <class F, int P, int D, int MW>
+__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kernel(const Cache c, const Attend a) {
+  constexpr int TS = 2048 / D, NB = TS / 8, kSub = TS > P ? TS / P : 1, kGroups = kWarps / MW;
+  constexpr int kSubRows = TS / kSub;               // positions of a step in one page
+  constexpr int kBatch = 32 / kSub;                 // steps whose pages the lanes hold
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t s_full[kGroups * kStages], s_empty[kGroups * kStages];
+  __shared__ float s_m[kWarps][16], s_l[kWarps][16], s_v[kWarps], s_top[MW * 16], s_sum[MW * 16];
+  __shared__ int s_nan;
+
+  uint32_t rank, split;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int mw = warp % MW, grp = warp / MW;
+  const int group = a.q_heads / c.kv_heads;
+  const int cta = blockIdx.x / split, h = cta % c.kv_heads, item = cta / c.kv_heads;
+
+  // sequence b owns the items from starts[b] group / (16 MW) + b on
+  auto key = [&](int i) { return (int)((long long)__ldg(c.starts + i) * group / (16 * MW)) + i; };
+  const int b = warp_search(c.seqs, item, key);
   const int r0 = __ldg(c.starts + b), r1 = __ldg(c.starts + b + 1), first = __ldg(c.first + b);
-  int lo = 0, hi = 0;
   if (r0 < 0 || r1 < r0 || r1 > c.rows || first > (1 << 30)) {
     report(a.status, MK_ERR_INVALID_ARG);
-  } else if (row >= r0 && row < r1) {
-    const int pos = first + row - r0;
-    int len = a.kv_lens ? __ldg(a.kv_lens + b) : first + r1 - r0;
-    if (len > c.table_width * P) {
-      report(a.status, MK_ERR_CAPACITY);
-      len = c.table_width * P;
-    }
-    if (pos >= 0) {
-      hi = a.causal ? min(len, pos + 1) : len;
+    return;   // the whole cluster: every block of it has this item
+  }
+  const int n = r1 - r0, m0 = (item - key(b)) * 16 * MW;
+  if (m0 < 0 || m0 >= n * group) return;
+  const int valid = min(n * group - m0, 16 * MW);
+  int len = a.kv_lens ? __ldg(a.kv_lens + b) : first + n;
+  if (len > c.table_width * P) {
+    report(a.status, MK_ERR_CAPACITY);
+    len = c.table_width * P;
+  }
+  // what the row of index m sees: [lo, hi)
+  auto sees = [&](int m, int& lo, int& hi) {
+    const int pos = first + m / group;
+    lo = hi = 0;
+    if (m < n * group && pos >= 0) {
+      hi = max(a.causal ? min(len, pos + 1) : len, 0);
       lo = a.window ? max(pos - a.window + 1, 0) : 0;
     }
-  }
-  float q[kPer], acc[kPer] = {};
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    q[i] = Elem<T>::to_f32(((const T*)a.q)[row * a.q_row + hq * a.q_head + lane * kPer + i]) * a.scale;
-  float m = -INFINITY, l = 0.f;
-  for (int j = lo + warp; j < hi; j += 4) {
-    const int id = page_id(c, b, j / P, a.status);
-    if (id < 0) continue;
-    const uint8_t* kp = c.codes + id * c.page_stride + (long long)h * P * D + (j % P) * D + lane * kPer;
-    const uint8_t* vp = kp + (long long)c.kv_heads * P * D;
-    const float* sc = c.scales + id * c.scale_stride + h;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s += q[i] * F::decode(kp[i]);
-    s = mk::warp_sum(s) * sc[0];
-    const float top = fmaxf(m, s), w = exp2f(s - top), keep = exp2f(m - top);
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * keep + w * sc[c.kv_heads] * F::decode(vp[i]);
-    m = top;
-  }
-  __shared__ float s_m[4], s_l[4], s_acc[4][D];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) s_acc[warp][lane * kPer + i] = acc[i];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
+  };
+  int lo_all, hi_all, lo_max, hi_min;
+  sees(m0 + valid - 1, lo_max, hi_all);
+  sees(m0, lo_all, hi_min);
+  const int begin = lo_all / TS * TS;
+  const int all_steps = hi_all > begin ? (hi_all - begin + TS - 1) / TS : 0;
+  const int lanes_of_steps = (int)split * kGroups, my = (int)rank * kGroups + grp;
+  const int steps = all_steps > my ? (all_steps - my - 1) / lanes_of_steps + 1 : 0;
+
+  if (threadIdx.x == 0) {
+    s_nan = 0;
+    for (int i = 0; i < kGroups * kStages; ++i) {
+      mk::mbar_init(&s_full[i], 1);
+      mk::mbar_init(&s_empty[i], MW);
+    }
+    mk::fence_mbar_init();
   }
   __syncthreads();
-  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float w[4], sum = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    w[i] = s_l[i] > 0.f ? exp2f(s_m[i] - top) : 0.f;
-    sum += w[i] * s_l[i];
+
+  // pages of kBatch steps, one per lane: id (-1: not wanted, or reported), scales
+  struct Page { int id; float ks, vs; };
+  auto pages_from = [&](int step) {
+    Page p{-1, 1.f, 0.f};   // a V scale of 0 leaves vref alone
+    const int st = step + lane / kSub;
+    const int pos = begin + (st * lanes_of_steps + my) * TS + (lane % kSub) * kSubRows;
+    if (st < steps && pos < hi_all && pos + kSubRows > lo_all) {
+      p.id = page_id(c, b, pos / P, a.status);
+      if (p.id >= 0) {
+        const float* sc = c.scales + p.id * c.scale_stride + h;
+        p.ks = __ldg(sc);
+        p.vs = __ldg(sc + c.kv_heads);
+      }
+    }
+    return p;
+  };
+  Page cur = pages_from(0), nxt = pages_from(kBatch);
+  int base = 0;
+  uint8_t* ring = smem + grp * kStages * kStageBytes;
+  // Codes that no other item reads do not stay in the L2 cache.
+  const uint64_t policy = n * group <= 16 * MW ? mk::policy_evict_first() : policy_evict_normal();
+  auto fetch = [&](int st) {   // by the whole first warp of a group
+    if (st >= steps) return;
+    const int pos = begin + (st * lanes_of_steps + my) * TS;
+    int ids[kSub];
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) {
+      const int src = (st - base) * kSub + i;
+      ids[i] = src < 32 ? __shfl_sync(0xffffffffu, cur.id, src) : __shfl_sync(0xffffffffu, nxt.id, src - 32);
+      bytes += ids[i] >= 0 ? 2 * kSubRows * D : 0;
+    }
+    if (lane == 0) {
+      uint64_t* bar = &s_full[grp * kStages + st % kStages];
+      uint8_t* dst = ring + st % kStages * kStageBytes;
+      mk::mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        if (ids[i] < 0) continue;
+        const uint8_t* k = c.codes + ids[i] * c.page_stride + ((long long)h * P + (pos + i * kSubRows) % P) * D;
+        mk::bulk_g2s(dst + i * kSubRows * D, k, kSubRows * D, bar, policy);
+        mk::bulk_g2s(dst + TS * D + i * kSubRows * D, k + (long long)c.kv_heads * P * D, kSubRows * D, bar, policy);
+      }
+    }
+  };
+  if (mw == 0)
+    for (int i = 0; i < kStages; ++i) fetch(i);
+
+  // q fragments of rows g and g + 8 of this warp's tile: k-step j holds
+  // dimensions 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1 | 2, 3}
+  uint32_t q[D / 16][4];
+  float rq[2];
+  int lo[2], hi[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int m = m0 + mw * 16 + g + 8 * e;
+    sees(m, lo[e], hi[e]);
+    const bool real = m < n * group;
+    const long long at = real ? (long long)(r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head : 0;
+    float v[D / 4];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) {
+      v[i] = real ? load_q(a.q, at + i / 16 * 64 + 16 * t + i % 16, a.bf16) : 0.f;
+      top = fmaxf(top, fabsf(v[i]));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // power of two that brings the largest to [2^14, 2^15)
+    const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);
+    const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
+    rq[e] = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      q[j][e] = pack_f16(v[4 * j] * up, v[4 * j + 1] * up);
+      q[j][2 + e] = pack_f16(v[4 * j + 2] * up, v[4 * j + 3] * up);
+    }
   }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float o = 0.f;
-    for (int i = 0; i < 4; ++i) o += w[i] * s_acc[i][d];
-    ((T*)a.out)[((long long)row * a.q_heads + hq) * D + d] = Elem<T>::from_f32(sum > 0.f ? o / sum : 0.f);
+
+  float o[D / 8][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
+  bool alive = true;
+  int nan_seen = 0, failed = 0;
+  for (int st = 0; st < steps; ++st) {
+    if (st - base == kBatch) {
+      base += kBatch;
+      cur = nxt;
+      nxt = pages_from(base + kBatch);
+    }
+    float ks[kSub], vs[kSub];
+    bool have[kSub], whole = true;
+    float vmax = vref;
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) {
+      const int src = (st - base) * kSub + i;
+      ks[i] = __shfl_sync(0xffffffffu, cur.ks, src);
+      vs[i] = __shfl_sync(0xffffffffu, cur.vs, src);
+      have[i] = __shfl_sync(0xffffffffu, cur.id, src) >= 0;
+      whole = whole && have[i];
+      vmax = fmaxf(vmax, vs[i]);
+    }
+    const int pos = begin + (st * lanes_of_steps + my) * TS;
+    whole = whole && pos >= lo_max && pos + TS <= hi_min;
+    if (!wait_bar(&s_full[grp * kStages + st % kStages], (st / kStages) & 1)) {
+      alive = false;
+      failed = st;
+      break;
+    }
+    const uint8_t* kb = ring + st % kStages * kStageBytes;
+    const uint8_t* vb = kb + TS * D;
+
+    float s[NB][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half) {
+        const uint4 w = *reinterpret_cast<const uint4*>(kb + (nb * 8 + g) * D + half * 64 + 16 * t);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b0, b1;
+          expand<F>(ws[j], b0, b1);
+          mma_f16(s[nb], q[half * 4 + j], b0, b1);
+        }
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = pos + nb * 8 + 2 * t + (i & 1), e = i >> 1;
+          if (!have[nb * 8 / kSubRows] || j < lo[e] || j >= hi[e]) s[nb][i] = -INFINITY;
+        }
+    }
+    // running maximum; the factors of the two rows
+    float f[kSub][2], top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[i][e] = fmaxf(rq[e] * ks[i], 1.17549435e-38f);   // -inf x 0 would be NaN
+        float x = -INFINITY;
+#pragma unroll
+        for (int nb = i * kSubRows / 8; nb < (i + 1) * kSubRows / 8; ++nb) x = fmaxf(x, fmaxf(s[nb][2 * e], s[nb][2 * e + 1]));
+        top[e] = fmaxf(top[e], x * f[i][e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+    }
+    float sub[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) sub[e] = top[e] == -INFINITY ? 0.f : top[e];
+    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]) || vmax > vref) {
+      const float vr = vmax > vref ? vref / vmax : 1.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float keep = ex2(m[e] - sub[e]);
+        l[e] *= keep;
+        m[e] = top[e];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][2 * e] *= keep * vr;
+          o[i][2 * e + 1] *= keep * vr;
+        }
+      }
+      vref = vmax;
+    }
+    float rv[kSub];
+    const float iv = vref > 0.f ? 32768.f / vref : 0.f;
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) rv[i] = vs[i] * iv;
+    uint32_t w[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int i = nb * 8 / kSubRows;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = ex2(fmaf(s[nb][2 * e], f[i][e], -sub[e])), y = ex2(fmaf(s[nb][2 * e + 1], f[i][e], -sub[e]));
+        l[e] += x + y;
+        w[nb][e] = pack_f16(x * rv[i], y * rv[i]);
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < NB / 2; ++kk) {
+      const uint32_t pa[4] = {w[2 * kk][0], w[2 * kk][1], w[2 * kk + 1][0], w[2 * kk + 1][1]};
+      uint32_t v[4][D / 32];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int row = kk * 16 + 2 * t + (x & 1) + 8 * (x >> 1);
+        const uint8_t* p = vb + row * D + g * (D / 8);
+        if constexpr (D == 64) {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          v[x][0] = u.x; v[x][1] = u.y;
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          v[x][0] = u.x; v[x][1] = u.y; v[x][2] = u.z; v[x][3] = u.w;
+        }
+        if (!whole) {
+          // What no row sees may hold anything: its codes count as 0.  A NaN
+          // that only some rows see is taken out here and put back at the end.
+          const bool dead = !have[row / kSubRows] || pos + row >= hi_all || pos + row < lo_all;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            if (dead) v[x][i] = 0;
+            if constexpr (F::kTopExp == 8) {
+              const uint32_t bad = nan_bytes(v[x][i]);
+              if (bad) {
+                nan_seen = 1;
+                v[x][i] &= ~((bad >> 7) * 0xffu);
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        // byte pairs of two positions: (d0, d1), (d2, d3)
+        uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+        expand<F>(__byte_perm(v[0][i], v[1][i], 0x5140), a0, a1);
+        expand<F>(__byte_perm(v[0][i], v[1][i], 0x7362), a2, a3);
+        expand<F>(__byte_perm(v[2][i], v[3][i], 0x5140), b0, b1);
+        expand<F>(__byte_perm(v[2][i], v[3][i], 0x7362), b2, b3);
+        mma_f16(o[4 * i], pa, a0, b0);
+        mma_f16(o[4 * i + 1], pa, a1, b1);
+        mma_f16(o[4 * i + 2], pa, a2, b2);
+        mma_f16(o[4 * i + 3], pa, a3, b3);
+      }
+    }
+    __syncwarp();
+    if constexpr (MW > 1) {
+      if (lane == 0) mk::mbar_arrive(&s_empty[grp * kStages + st % kStages]);
+      if (mw == 0) {
+        if (st + kStages < steps && !wait_bar(&s_empty[grp * kStages + st % kStages], (st / kStages) & 1)) {
+          alive = false;
+          failed = st + 1;
+          break;
+        }
+        fetch(st + kStages);
+      }
+    } else {
+      fetch(st + kStages);
+    }
   }
-  if (a.lse && threadIdx.x == 0)
-    a.lse[(long long)row * a.q_heads + hq] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+  if (!alive) {
+    // Leave no copy in flight: the block's shared memory is given away at its
+    // end.  (Waits are bounded; a copy that never lands is reported.)
+    report(a.status, MK_ERR_TIMEOUT);
+    for (int i = 0; i < kStages; ++i)
+      if (failed + i < steps) wait_bar(&s_full[grp * kStages + (failed + i) % kStages], ((failed + i) / kStages) & 1);
+  }
+  if (nan_seen) s_nan = 1;
+
+  // ---- join the warps, then the blocks of the cluster
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    if (t == 0) {
+      s_m[warp][g + 8 * e] = m[e];
+      s_l[warp][g + 8 * e] = l[e];
+    }
+  }
+  if (lane == 0) s_v[warp] = vref * (1.f / 32768.f);
+  __syncthreads();   // the ring is free
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      // n-block i, columns 2 t and 2 t + 1: dimensions (D / 8) (2 t + x) + i
+      part[(warp * 16 + g + 8 * e) * D + (D / 8) * (2 * t) + i] = o[i][2 * e];
+      part[(warp * 16 + g + 8 * e) * D + (D / 8) * (2 * t + 1) + i] = o[i][2 * e + 1];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < valid * D; i += kWarps * 32) {
+    const int r = i / D, w0 = r / 16;   // warps w0, w0 + MW, ... hold row r
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int x = 0; x < kGroups; ++x) top = fmaxf(top, s_m[w0 + x * MW][r % 16]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int x = 0; x < kGroups; ++x) {
+      const int ww = w0 + x * MW;
+      const float f = ex2(s_m[ww][r % 16] - ref);
+      sum += f * s_l[ww][r % 16];
+      acc += f * s_v[ww] * part[(ww * 16 + r % 16) * D + i % D];
+    }
+    part[(w0 * 16 + r % 16) * D + i % D] = acc;
+    if (i % D == 0) {
+      s_top[r] = top;
+      s_sum[r] = sum;
+    }
+  }
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+  const int nan_any = s_nan;
+  // block `rank` finishes every split-th run of 32 elements
+  for (int i = threadIdx.x; i < valid * D; i += kWarps * 32) {
+    if ((i >> 5) % (int)split != (int)rank) continue;
+    const int r = i / D, d = i % D, idx = ((r / 16) * 16 + r % 16) * D + d;
+    float top = s_top[r], sum = s_sum[r], acc = part[idx];
+    int bad = nan_any;
+    if (split > 1) {
+      top = -INFINITY;
+      for (uint32_t k = 0; k < split; ++k) top = fmaxf(top, remote_f32(&s_top[r], k));
+      const float ref = top == -INFINITY ? 0.f : top;
+      sum = acc = 0.f;
+      for (uint32_t k = 0; k < split; ++k) {
+        const float f = ex2(remote_f32(&s_top[r], k) - ref);
+        sum += f * remote_f32(&s_sum[r], k);
+        acc += f * remote_f32(&part[idx], k);
+        bad |= __float_as_int(remote_f32(reinterpret_cast<const float*>(&s_nan), k));
+      }
+    }
+    float v = sum == 0.f ? 0.f : acc / sum;   // nothing seen: 0
+    int rlo, rhi;
+    sees(m0 + r, rlo, rhi);
+    if (bad) {
+      // NaN codes of positions that this row sees and another row of the item does not
+      for (int j = rlo; j < rhi; ++j) {
+        if (j >= lo_max + TS && j < hi_min - TS) j = hi_min - TS;   // whole steps kept theirs
+        const int id = page_id(c, b, j / P, nullptr);
+        if (id < 0) continue;
+        const uint8_t code = c.codes[id * c.page_stride + ((long long)(c.kv_heads + h) * P + j % P) * D + d];
+        if (F::kTopExp == 8 && (code & 127) == 127) v = __int_as_float(0x7fffffff);
+      }
+    }
+    const long long at = (long long)(r0 + (m0 + r) / group) * a.q_heads + h * group + (m0 + r) % group;
+    store_out(a.out, at * D + d, v, a.bf16);
+    if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  }
+  if (split > 1) cluster_sync_all();   // peers have read this block's shared memory
 }
 
 int cache_of(const mk_kv8* m, Cache* c);
 
-template <class T, class F, int P, int D>
+template <class F, int P, int D, int MW>
+static int launch_rows(const Cache& c, const Attend& a, cudaStream_t stream) {
+  const int group = a.q_heads / c.kv_heads;
+  const long long items = (long long)c.rows * group / (16 * MW) + c.seqs;
+  const long long most = (long long)c.table_width * P;
+  // Blocks per item: until the grid fills the GPU three times over, but no
+  // more than one step of each group of warps per block at full capacity.
+  int split = 1;
+  while (split < 8 && items * c.kv_heads * split < 148 * 3 && most > (long long)split * (kWarps / MW) * (2048 / D)) split *= 2;
+  const long long blocks = items * c.kv_heads * split;
+  if (blocks > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
+  auto kernel = &attend_rows_kernel<F, P, D, MW>;
+  constexpr int bytes = rows_smem<D, MW>();
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return MK_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)split, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, c, a) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
+}
+
+template <class F, int P, int D>
 static int launch(const Cache& c, const Attend& a, cudaStream_t stream) {
-  attend_simple_kernel<T, F, P, D><<<dim3((unsigned)c.rows, (unsigned)a.q_heads), 128, 0, stream>>>(c, a);
-  return cudaGetLastError() == cudaSuccess ? MK_OK : MK_ERR_CUDA;
+  // rows of a sequence, once per query head of the group, on average
+  const long long per = ((long long)c.rows * (a.q_heads / c.kv_heads) + c.seqs - 1) / c.seqs;
+  if (per <= 16) return launch_rows<F, P, D, 1>(c, a, stream);
+  if (per <= 32) return launch_rows<F, P, D, 2>(c, a, stream);
+  return launch_rows<F, P, D, 4>(c, a, stream);
 }
 
 }  // namespace mkp
@@ -109,19 +582,17 @@ extern "C" int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long 
       q_head < 0)
     return MK_ERR_INVALID_ARG;
   const Attend a{d_q, d_out, d_lse, d_kv_lens, q_row, q_head, q_heads, causal, window,
-                 sm_scale * 1.4426950408889634f, d_status};
-  auto run = [&](auto t, auto f, auto p, auto d) {
-    return launch<decltype(t), decltype(f), decltype(p)::value, decltype(d)::value>(c, a, (cudaStream_t)stream);
+                 sm_scale * 1.4426950408889634f, type == MK_TYPE_BF16, d_status};
+  auto with_d = [&](auto f, auto p) {
+    using F = decltype(f);
+    constexpr int P = decltype(p)::value;
+    return cache->head_dim == 64 ? launch<F, P, 64>(c, a, (cudaStream_t)stream)
+                                 : launch<F, P, 128>(c, a, (cudaStream_t)stream);
   };
-  auto with_d = [&](auto t, auto f, auto p) {
-    return cache->head_dim == 64 ? run(t, f, p, std::integral_constant<int, 64>{})
-                                 : run(t, f, p, std::integral_constant<int, 128>{});
+  auto with_p = [&](auto f) {
+    if (cache->page_size == 16) return with_d(f, std::integral_constant<int, 16>{});
+    if (cache->page_size == 32) return with_d(f, std::integral_constant<int, 32>{});
+    return with_d(f, std::integral_constant<int, 64>{});
   };
-  auto with_p = [&](auto t, auto f) {
-    if (cache->page_size == 16) return with_d(t, f, std::integral_constant<int, 16>{});
-    if (cache->page_size == 32) return with_d(t, f, std::integral_constant<int, 32>{});
-    return with_d(t, f, std::integral_constant<int, 64>{});
-  };
-  auto with_f = [&](auto t) { return cache->format == MK_KV8_E4M3 ? with_p(t, E4M3{}) : with_p(t, I8{}); };
-  return type == MK_TYPE_BF16 ? with_f(__nv_bfloat16{}) : with_f(__half{});
+  return cache->format == MK_KV8_E4M3 ? with_p(E4M3{}) : with_p(I8{});
 }

@@ -430,3 +430,23 @@ def test_verify_many_drafts_and_sequences():
     tokens = r.randint(0, 50, st[-1]).tolist()
     u = (r.rand(st[-1]) * 0.01).astype(np.float32)
     verify_case(tokens, target, target.copy(), u, r.rand(len(rows)).astype(np.float32), st)
+
+
+@pytest.mark.parametrize("rows", [3, 150])
+def test_attend_nan_in_places_that_only_some_rows_see(rows):
+    """A NaN value code counts for the rows that see its position, and for them only."""
+    page, d, hq, hk, n = 16, 64, 2, 1, rows + 21
+    pages = -(-n // page)
+    g = torch.Generator().manual_seed(rows)
+    codes = torch.randn(pages, 2, hk, page, d, generator=g).clamp(-4, 4).mul(100).to(torch.float8_e4m3fn).view(torch.int8)
+    marks = [(n - 1, 5), (n - 2, 63), (n - rows + 1, 0)]
+    for pos, dim in marks:
+        codes[pos // page, 1, 0, pos % page, dim] = -1          # 0xff
+    q = torch.randn(rows, hq, d, generator=g).to(BF).to(DEV)
+    out = paged.kv8_attend(q, codes.to(DEV).view(torch.float8_e4m3fn), torch.full((pages, 2, hk), 2.0 ** -6, device=DEV),
+                           ints([list(range(pages))]), ints([0, rows]), ints([n - rows]))
+    paged.check(DEV)
+    want = torch.zeros(rows, d, dtype=torch.bool)
+    for pos, dim in marks:
+        want[max(0, pos - (n - rows)):, dim] = True
+    assert torch.equal(out.isnan().cpu(), want[:, None].expand(rows, hq, d))
