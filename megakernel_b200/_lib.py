@@ -145,10 +145,10 @@ def signatures() -> dict:
         "megakernel_tp_connect": ([vp, vp], c_int),
         "megakernel_tp_info": ([vp, ip, ip], c_int),
         "megakernel_tp_exchange_slots": ([vp, vp], c_int),
-        "megakernel_qk_norm_rope": ([ctypes.POINTER(MkQkNormRope), vp, vp], c_int),
-        "megakernel_kv8_append": ([ctypes.POINTER(MkKv8), vp, c_ll, c_ll, vp, c_ll, c_ll, c_int, vp, vp], c_int),
-        "megakernel_kv8_read": ([ctypes.POINTER(MkKv8), vp, vp, c_int, vp, vp], c_int),
-        "megakernel_kv8_attend": ([ctypes.POINTER(MkKv8), vp, c_ll, c_ll, c_int, c_int, ctypes.c_float, c_int,
+        "megakernel_qk_norm_rope": ([vp, vp, vp], c_int),
+        "megakernel_kv8_append": ([vp, vp, c_ll, c_ll, vp, c_ll, c_ll, c_int, vp, vp], c_int),
+        "megakernel_kv8_read": ([vp, vp, vp, c_int, vp, vp], c_int),
+        "megakernel_kv8_attend": ([vp, vp, c_ll, c_ll, c_int, c_int, ctypes.c_float, c_int,
                                    c_int, vp, vp, vp, vp, vp], c_int),
         "megakernel_verify_drafts": ([vp, vp, c_ll, vp, c_ll, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp, vp],
                                      c_int),

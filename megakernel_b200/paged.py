@@ -25,9 +25,8 @@ CPU path.
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
 import math
+import struct
 
 import torch
 
@@ -40,98 +39,117 @@ PAGE_SIZES = (16, 32, 64)
 HEAD_DIMS = (64, 128)
 
 _status = {}
+_lib_fns = None
+_get_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+# struct mk_kv8 and mk_qk_norm_rope in C order (include/megakernel.h)
+_pack_kv8 = struct.Struct("@5P3q8i").pack
+_pack_norm_rope = struct.Struct("@9P8q6if4x").pack
 
 
-def _status_of(device: torch.device) -> torch.Tensor:
-    """The device's status word; made (and waited for) at its first use."""
-    t = _status.get(device.index)
-    if t is None:
-        t = _status[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-        torch.cuda.current_stream(device).synchronize()
-    return t
+def _fns():
+    """The C entries, bound once, after the status word of the current device."""
+    global _lib_fns
+    if _lib_fns is None:
+        L = _lib.load()
+        _lib_fns = (L.megakernel_qk_norm_rope, L.megakernel_kv8_append, L.megakernel_kv8_read,
+                    L.megakernel_kv8_attend, L.megakernel_verify_drafts)
+    return _lib_fns
+
+
+def _status_of(idx: int) -> int:
+    """Address of device idx's status word; made (and waited for) at its first use."""
+    got = _status.get(idx)
+    if got is None:
+        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        torch.cuda.current_stream(idx).synchronize()
+        got = _status[idx] = (t, t.data_ptr())
+    return got[1]
 
 
 def check(device=None) -> None:
     """Wait for the device and raise if a kernel of this module met metadata
     out of range since the last check (page ids, positions, row starts)."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    t = _status_of(dev)
-    torch.cuda.synchronize(dev)
+    dev = torch.device("cuda" if device is None else device)
+    idx = torch.cuda.current_device() if dev.index is None else dev.index
+    _status_of(idx)
+    torch.cuda.synchronize(idx)
+    t = _status[idx][0]
     rc = int(t.item())
     if rc:
         t.zero_()
-        torch.cuda.synchronize(dev)
+        torch.cuda.synchronize(idx)
         _lib.check(rc, "paged operators")
 
 
-def _need(ok, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-@contextlib.contextmanager
-def _on(device, stream, tensors):
-    """Run on `device`, on `stream` if one is given; tensors used on a stream
-    that is not theirs are kept until it has passed."""
-    with torch.cuda.device(device):
+def _elsewhere(fn, idx, stream, args, kw):
+    """fn(*args, **kw) on device idx, and on `stream` if one is given; tensors
+    used on a stream that is not theirs are kept until it has passed."""
+    with torch.cuda.device(idx):
         if stream is None:
-            yield torch.cuda.current_stream(device).cuda_stream
-            return
+            return fn(*args, **kw)
+        for t in (*args, *kw.values()):
+            if isinstance(t, torch.Tensor) and t.is_cuda:
+                t.record_stream(stream)
         with torch.cuda.stream(stream):
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(stream)
-            yield stream.cuda_stream
+            return fn(*args, **kw)
 
 
-def _rows(t, name, heads_dim=True):
-    """A [rows, heads, head_dim] operand whose rows can be read in 16-byte vectors."""
-    _need(t.dim() == 3 and t.is_cuda, f"{name}: a CUDA tensor [rows, heads, head_dim]")
-    _need(t.dtype in TYPES, f"{name}: float32, bfloat16 or float16")
-    per = 16 // t.element_size()
-    s = t.stride()
-    one = t.shape[0] > 1
-    _need((t.shape[2] <= 1 or s[2] == 1) and (not one or s[0] % per == 0) and (t.shape[1] <= 1 or s[1] % per == 0)
-          and s[0] >= 0 and s[1] >= 0 and t.data_ptr() % 16 == 0,
-          f"{name}: head_dim contiguous, rows and heads at multiples of 16 bytes")
-    return (s[0] if one else 0, s[1] if t.shape[1] > 1 else 0)
+def _rows(t, name):
+    """Strides of a [rows, heads, head_dim] operand that is read in 16-byte
+    vectors (0 for an axis of one element)."""
+    if t.dim() != 3 or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor [rows, heads, head_dim]")
+    if t.dtype not in TYPES:
+        raise ValueError(f"{name}: float32, bfloat16 or float16")
+    s0, s1, s2 = t.stride()
+    per = 3 if t.dtype is torch.float32 else 7
+    if s2 != 1 or (s0 | s1) & per or s0 < 0 or s1 < 0 or t.data_ptr() & 15:
+        n, h, d = t.shape
+        s0, s1 = s0 if n > 1 else 0, s1 if h > 1 else 0
+        if (s2 != 1 and d > 1) or (s0 | s1) & per or s0 < 0 or s1 < 0 or t.data_ptr() & 15:
+            raise ValueError(f"{name}: head_dim contiguous, rows and heads at multiples of 16 bytes")
+    return s0, s1
 
 
-def _int32(t, name, shape, device):
-    _need(t.dtype == torch.int32 and t.device == device and tuple(t.shape) == shape and t.is_contiguous(),
-          f"{name}: contiguous int32 {list(shape)} on {device}")
+def _vector(t, name, dtype, n, idx):
+    if t.dtype is not dtype or t.get_device() != idx or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {str(dtype)[6:]} [{n}] on cuda:{idx}")
 
 
 def _cache(codes, scales, page_table, starts, first, rows):
-    _need(codes.dim() == 5 and codes.dtype in FORMATS and codes.is_cuda and codes.shape[1] == 2,
-          "codes: CUDA float8_e4m3fn or int8 [pages, 2, kv_heads, page_size, head_dim]")
-    pages, _, hk, page, d = codes.shape
-    _need(page in PAGE_SIZES, f"page_size: one of {PAGE_SIZES}")
-    _need(d in HEAD_DIMS, f"head_dim: one of {HEAD_DIMS}")
-    s = codes.stride()
-    _need(s[4] == 1 and s[3] == d and (hk == 1 or s[2] == page * d) and s[1] == hk * page * d,
-          "codes: a page's codes contiguous")
-    page_stride = s[0] if pages > 1 else 2 * hk * page * d
-    _need(page_stride >= 2 * hk * page * d and page_stride % 16 == 0 and codes.data_ptr() % 16 == 0,
-          "codes: pages at multiples of 16 bytes")
-    dev = codes.device
-    _need(scales.dtype == torch.float32 and scales.device == dev and tuple(scales.shape) == (pages, 2, hk)
-          and (hk == 1 or scales.stride(2) == 1) and scales.stride(1) == hk,
-          "scales: float32 [pages, 2, kv_heads], a page's scales contiguous")
-    scale_stride = scales.stride(0) if pages > 1 else 2 * hk
-    _need(scale_stride >= 2 * hk, "scales: pages must not overlap")
-    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == dev
-          and (page_table.shape[1] <= 1 or page_table.stride(1) == 1), "page_table: int32 [seqs, pages] on the cache's device")
+    """The checked cache arguments: (struct mk_kv8, device index, seqs, kv_heads, head_dim)."""
+    if codes.dim() != 5 or not codes.is_cuda or codes.dtype not in FORMATS:
+        raise ValueError("codes: CUDA float8_e4m3fn or int8 [pages, 2, kv_heads, page_size, head_dim]")
+    idx = codes.get_device()
+    pages, two, hk, page, d = codes.shape
+    if two != 2 or page not in PAGE_SIZES or d not in HEAD_DIMS or hk < 1:
+        raise ValueError(f"codes: [pages, 2, kv_heads, page_size, head_dim], page_size of {PAGE_SIZES}, head_dim of {HEAD_DIMS}")
+    s0, s1, s2, s3, s4 = codes.stride()
+    held = page * d
+    if s4 != 1 or s3 != d or (s2 != held and hk > 1) or s1 != hk * held:
+        raise ValueError("codes: a page's codes contiguous")
+    page_stride = s0 if pages > 1 else 2 * hk * held
+    if page_stride < 2 * hk * held or page_stride & 15 or codes.data_ptr() & 15:
+        raise ValueError("codes: pages at multiples of 16 bytes, not overlapping")
+    if scales.dtype is not torch.float32 or scales.get_device() != idx or tuple(scales.shape) != (pages, 2, hk):
+        raise ValueError("scales: float32 [pages, 2, kv_heads] on the cache's device")
+    z0, z1, z2 = scales.stride()
+    scale_stride = z0 if pages > 1 else 2 * hk
+    if (z2 != 1 and hk > 1) or z1 != hk or scale_stride < 2 * hk:
+        raise ValueError("scales: a page's scales contiguous, pages not overlapping")
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != idx:
+        raise ValueError("page_table: int32 [seqs, pages] on the cache's device")
     b, width = page_table.shape
-    table_stride = page_table.stride(0) if b > 1 else width
-    _need(table_stride >= width, "page_table: rows must not overlap")
-    _int32(starts, "starts", (b + 1,), dev)
-    _int32(first, "first", (b,), dev)
-    return _lib.MkKv8(codes.data_ptr(), scales.data_ptr(), page_table.data_ptr(), starts.data_ptr(),
-                      first.data_ptr(), page_stride, scale_stride, table_stride, pages, width, hk, page, d,
-                      FORMATS[codes.dtype], b, rows)
+    t0, t1 = page_table.stride()
+    table_stride = t0 if b > 1 else width
+    if (t1 != 1 and width > 1) or table_stride < width:
+        raise ValueError("page_table: a sequence's pages contiguous, rows not overlapping")
+    _vector(starts, "starts", torch.int32, b + 1, idx)
+    _vector(first, "first", torch.int32, b, idx)
+    return (_pack_kv8(codes.data_ptr(), scales.data_ptr(), page_table.data_ptr(), starts.data_ptr(), first.data_ptr(),
+                      page_stride, scale_stride, table_stride, pages, width, hk, page, d, FORMATS[codes.dtype], b, rows),
+            idx, b, hk, d)
 
 
 def qk_norm_rope(q, k, q_gain, k_gain, cos, sin, positions, *, eps=1e-6, q_out=None, k_out=None, stream=None):
@@ -142,33 +160,50 @@ def qk_norm_rope(q, k, q_gain, k_gain, cos, sin, positions, *, eps=1e-6, q_out=N
     of one packed projection, and an output may be its input.  cos, sin: fp32
     tables [positions, D / 2]; positions: int32 [rows].  D 64 or 128.  A row
     whose position is outside the tables is not written (see ``check``)."""
-    dev = q.device
-    qs, ks = _rows(q, "q"), _rows(k, "k")
+    q_row, q_head = _rows(q, "q")
+    k_row, k_head = _rows(k, "k")
+    idx = q.get_device()
+    if stream is not None or idx != _get_device():
+        return _elsewhere(qk_norm_rope, idx, stream, (q, k, q_gain, k_gain, cos, sin, positions),
+                          dict(eps=eps, q_out=q_out, k_out=k_out))
+    dtype = q.dtype
     rows, hq, d = q.shape
-    _need(k.shape[0] == rows and k.shape[2] == d and k.dtype == q.dtype and k.device == dev,
-          "k: q's rows, head_dim, dtype and device")
-    _need(d in HEAD_DIMS, f"head_dim: one of {HEAD_DIMS}")
-    for g, name in ((q_gain, "q_gain"), (k_gain, "k_gain")):
-        _need(g.dtype == q.dtype and g.device == dev and tuple(g.shape) == (d,) and g.is_contiguous()
-              and g.data_ptr() % 16 == 0, f"{name}: contiguous [{d}] of q's dtype")
-    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == d // 2 and cos.dtype == sin.dtype == torch.float32
-          and cos.device == dev and sin.device == dev and cos.is_contiguous() and sin.is_contiguous()
-          and cos.data_ptr() % 16 == 0 and sin.data_ptr() % 16 == 0, f"cos, sin: contiguous float32 [positions, {d // 2}]")
-    _int32(positions, "positions", (rows,), dev)
-    _need(eps >= 0.0, "eps: not negative")
-    with _on(dev, stream, (q, k, q_gain, k_gain, cos, sin, positions, q_out, k_out)) as st:
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        qo, ko = _rows(q_out, "q_out"), _rows(k_out, "k_out")
-        _need(q_out.shape == q.shape and k_out.shape == k.shape and q_out.dtype == k_out.dtype == q.dtype
-              and q_out.device == k_out.device == dev, "q_out, k_out: the shapes, dtype and device of q and k")
-        a = _lib.MkQkNormRope(q.data_ptr(), k.data_ptr(), q_gain.data_ptr(), k_gain.data_ptr(), q_out.data_ptr(),
-                              k_out.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), *qs, *ks, *qo,
-                              *ko, cos.shape[0], rows, hq, k.shape[1], d, TYPES[q.dtype], eps)
-        _lib.check(_lib.load().megakernel_qk_norm_rope(ctypes.byref(a), _status_of(dev).data_ptr(), st),
-                   "megakernel_qk_norm_rope")
+    k_rows, hk, k_d = k.shape
+    if k_rows != rows or k_d != d or k.dtype is not dtype or k.get_device() != idx:
+        raise ValueError("k: q's rows, head_dim, dtype and device")
+    if d not in HEAD_DIMS:
+        raise ValueError(f"head_dim: one of {HEAD_DIMS}")
+    _vector(q_gain, "q_gain", dtype, d, idx)
+    _vector(k_gain, "k_gain", dtype, d, idx)
+    size, half = cos.shape if cos.dim() == 2 else (0, 0)
+    if half != d // 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
+            or cos.get_device() != idx or sin.get_device() != idx or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError(f"cos, sin: contiguous float32 [positions, {d // 2}] on q's device")
+    if (q_gain.data_ptr() | k_gain.data_ptr() | cos.data_ptr() | sin.data_ptr()) & 15:
+        raise ValueError("q_gain, k_gain, cos, sin: 16-byte aligned")
+    _vector(positions, "positions", torch.int32, rows, idx)
+    if not eps >= 0.0:
+        raise ValueError("eps: not negative")
+    if q_out is None:
+        q_out = q.new_empty((rows, hq, d))
+        qo_row, qo_head = hq * d, d
+    else:
+        qo_row, qo_head = _rows(q_out, "q_out")
+        if q_out.shape != q.shape or q_out.dtype is not dtype or q_out.get_device() != idx:
+            raise ValueError("q_out: the shape, dtype and device of q")
+    if k_out is None:
+        k_out = k.new_empty((rows, hk, d))
+        ko_row, ko_head = hk * d, d
+    else:
+        ko_row, ko_head = _rows(k_out, "k_out")
+        if k_out.shape != k.shape or k_out.dtype is not dtype or k_out.get_device() != idx:
+            raise ValueError("k_out: the shape, dtype and device of k")
+    rc = _fns()[0](_pack_norm_rope(q.data_ptr(), k.data_ptr(), q_gain.data_ptr(), k_gain.data_ptr(), q_out.data_ptr(),
+                                   k_out.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), q_row, q_head,
+                                   k_row, k_head, qo_row, qo_head, ko_row, ko_head, size, rows, hq, hk, d, TYPES[dtype],
+                                   eps), _status_of(idx), _raw_stream(idx))
+    if rc:
+        _lib.check(rc, "megakernel_qk_norm_rope")
     return q_out, k_out
 
 
@@ -180,30 +215,35 @@ def kv8_append(codes, scales, k, v, page_table, starts, first, *, stream=None):
     of its scale and the new one, its earlier codes rounded again if that grows.
     ``codes`` and ``scales`` are updated in place.  No two sequences of a call
     may write to one page."""
-    ks, vs = _rows(k, "k"), _rows(v, "v")
-    c = _cache(codes, scales, page_table, starts, first, k.shape[0])
-    dev = codes.device
-    _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device == dev
-          and k.shape[1] == c.kv_heads and k.shape[2] == c.head_dim,
-          "k, v: one shape [rows, kv_heads, head_dim] and dtype, on the cache's device")
-    with _on(dev, stream, (codes, scales, k, v, page_table, starts, first)) as st:
-        _lib.check(_lib.load().megakernel_kv8_append(ctypes.byref(c), k.data_ptr(), *ks, v.data_ptr(), *vs,
-                                                     TYPES[k.dtype], _status_of(dev).data_ptr(), st),
-                   "megakernel_kv8_append")
+    k_row, k_head = _rows(k, "k")
+    v_row, v_head = _rows(v, "v")
+    rows, heads, dim = k.shape
+    cache, idx, _, hk, d = _cache(codes, scales, page_table, starts, first, rows)
+    if k.shape != v.shape or heads != hk or dim != d or k.dtype is not v.dtype or k.get_device() != idx \
+            or v.get_device() != idx:
+        raise ValueError("k, v: one shape [rows, kv_heads, head_dim] and dtype, on the cache's device")
+    if stream is not None or idx != _get_device():
+        return _elsewhere(kv8_append, idx, stream, (codes, scales, k, v, page_table, starts, first), {})
+    rc = _fns()[1](cache, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, TYPES[k.dtype], _status_of(idx),
+                   _raw_stream(idx))
+    if rc:
+        _lib.check(rc, "megakernel_kv8_append")
 
 
 def kv8_read(codes, scales, page_table, starts, first, rows, *, dtype=torch.bfloat16, stream=None):
     """The cached keys and values of the rows' positions: (k, v), each
     [rows, kv_heads, D] of `dtype`.  rows: starts[-1], as a number."""
-    c = _cache(codes, scales, page_table, starts, first, int(rows))
-    _need(rows >= 0, "rows: not negative")
-    _need(dtype in TYPES, "dtype: float32, bfloat16 or float16")
-    dev = codes.device
-    with _on(dev, stream, (codes, scales, page_table, starts, first)) as st:
-        kv = torch.empty(2, rows, c.kv_heads, c.head_dim, dtype=dtype, device=dev)
-        k, v = kv[0], kv[1]
-        _lib.check(_lib.load().megakernel_kv8_read(ctypes.byref(c), k.data_ptr(), v.data_ptr(), TYPES[dtype],
-                                                   _status_of(dev).data_ptr(), st), "megakernel_kv8_read")
+    if rows < 0:
+        raise ValueError("rows: not negative")
+    if dtype not in TYPES:
+        raise ValueError("dtype: float32, bfloat16 or float16")
+    cache, idx, _, hk, d = _cache(codes, scales, page_table, starts, first, rows)
+    if stream is not None or idx != _get_device():
+        return _elsewhere(kv8_read, idx, stream, (codes, scales, page_table, starts, first, rows), dict(dtype=dtype))
+    k, v = scales.new_empty((2, rows, hk, d), dtype=dtype).unbind(0)
+    rc = _fns()[2](cache, k.data_ptr(), v.data_ptr(), TYPES[dtype], _status_of(idx), _raw_stream(idx))
+    if rc:
+        _lib.check(rc, "megakernel_kv8_read")
     return k, v
 
 
@@ -217,30 +257,38 @@ def kv8_attend(q, codes, scales, page_table, starts, first, *, kv_lens=None, sm_
     h // (q_heads // kv_heads).  sm_scale defaults to D ** -0.5.  Returns out
     [rows, q_heads, D] of q's dtype, and with ``return_lse`` the fp32
     log-sum-exp [rows, q_heads]; a row that sees nothing gives 0 and -inf."""
-    qs = _rows(q, "q")
-    rows, hq, d = q.shape
-    c = _cache(codes, scales, page_table, starts, first, rows)
-    dev = codes.device
-    _need(q.dtype in (torch.bfloat16, torch.float16) and q.device == dev and d == c.head_dim,
-          "q: bfloat16 or float16 [rows, q_heads, head_dim] on the cache's device")
-    _need(hq >= 1 and hq % c.kv_heads == 0, "q_heads: a multiple of kv_heads")
-    _need(c.seqs > 0 or rows == 0, "rows without a sequence")
+    q_row, q_head = _rows(q, "q")
+    rows, hq, q_d = q.shape
+    cache, idx, seqs, hk, d = _cache(codes, scales, page_table, starts, first, rows)
+    if q.dtype is torch.float32 or q.get_device() != idx or q_d != d:
+        raise ValueError("q: bfloat16 or float16 [rows, q_heads, head_dim] on the cache's device")
+    if hq < 1 or hq % hk:
+        raise ValueError("q_heads: a multiple of kv_heads")
+    if seqs == 0 and rows > 0:
+        raise ValueError("rows without a sequence")
     if kv_lens is not None:
-        _int32(kv_lens, "kv_lens", (c.seqs,), dev)
-    _need(window >= 0, "window: not negative")
-    sm_scale = d ** -0.5 if sm_scale is None else float(sm_scale)
-    _need(0.0 < sm_scale < math.inf, "sm_scale: positive")
-    with _on(dev, stream, (q, codes, scales, page_table, starts, first, kv_lens, out)) as st:
-        if out is None:
-            out = torch.empty(rows, hq, d, dtype=q.dtype, device=dev)
-        else:
-            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.is_contiguous()
-                  and out.data_ptr() % 16 == 0, "out: contiguous, of q's shape, dtype and device")
-        lse = torch.empty(rows, hq, dtype=torch.float32, device=dev) if return_lse else None
-        _lib.check(_lib.load().megakernel_kv8_attend(
-            ctypes.byref(c), q.data_ptr(), *qs, hq, TYPES[q.dtype], sm_scale, int(bool(causal)), int(window),
-            None if kv_lens is None else kv_lens.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-            _status_of(dev).data_ptr(), st), "megakernel_kv8_attend")
+        _vector(kv_lens, "kv_lens", torch.int32, seqs, idx)
+    if window < 0:
+        raise ValueError("window: not negative")
+    if sm_scale is None:
+        sm_scale = d ** -0.5
+    elif not 0.0 < sm_scale < math.inf:
+        raise ValueError("sm_scale: positive")
+    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != idx
+                            or not out.is_contiguous() or out.data_ptr() & 15):
+        raise ValueError("out: contiguous, of q's shape, dtype and device")
+    if stream is not None or idx != _get_device():
+        return _elsewhere(kv8_attend, idx, stream, (q, codes, scales, page_table, starts, first),
+                          dict(kv_lens=kv_lens, sm_scale=sm_scale, causal=causal, window=window, out=out,
+                               return_lse=return_lse))
+    if out is None:
+        out = q.new_empty((rows, hq, d))
+    lse = scales.new_empty((rows, hq)) if return_lse else None
+    rc = _fns()[3](cache, q.data_ptr(), q_row, q_head, hq, TYPES[q.dtype], sm_scale, 1 if causal else 0, window,
+                   None if kv_lens is None else kv_lens.data_ptr(), out.data_ptr(),
+                   None if lse is None else lse.data_ptr(), _status_of(idx), _raw_stream(idx))
+    if rc:
+        _lib.check(rc, "megakernel_kv8_attend")
     return (out, lse) if return_lse else out
 
 
@@ -255,33 +303,43 @@ def verify_drafts(tokens, target_probs, draft_probs, uniforms, sample_u, starts,
     numbers in [0, 1).  out int32 [rows]: per sequence the kept drafts, the
     drawn token, then -1; accepted int32 [seqs].  The arithmetic is in whole
     numbers (units of 2^-36 and 2^-24), so results are exact and repeatable."""
-    _need(target_probs.dim() == 2 and target_probs.is_cuda and target_probs.dtype == torch.float32
-          and (target_probs.shape[1] == 1 or target_probs.stride(1) == 1), "target_probs: CUDA float32 [rows, vocab], vocab contiguous")
+    if target_probs.dim() != 2 or not target_probs.is_cuda or target_probs.dtype is not torch.float32:
+        raise ValueError("target_probs: CUDA float32 [rows, vocab]")
     rows, vocab = target_probs.shape
-    dev = target_probs.device
-    _need(vocab >= 1, "vocab: at least one token")
-    _need(starts.dim() == 1 and starts.shape[0] >= 1, "starts: int32 [seqs + 1]")
-    seqs = starts.shape[0] - 1
-    _int32(starts, "starts", (seqs + 1,), dev)
-    _int32(tokens, "tokens", (rows,), dev)
-    for t, name, n in ((uniforms, "uniforms", rows), (sample_u, "sample_u", seqs)):
-        _need(t.dtype == torch.float32 and t.device == dev and tuple(t.shape) == (n,) and t.is_contiguous(),
-              f"{name}: contiguous float32 [{n}] on {dev}")
+    idx = target_probs.get_device()
+    if vocab < 1 or starts.dim() != 1 or starts.numel() < 1:
+        raise ValueError("vocab: at least one token; starts: int32 [seqs + 1]")
+    seqs = starts.numel() - 1
+    _vector(starts, "starts", torch.int32, seqs + 1, idx)
+    _vector(tokens, "tokens", torch.int32, rows, idx)
+    _vector(uniforms, "uniforms", torch.float32, rows, idx)
+    _vector(sample_u, "sample_u", torch.float32, seqs, idx)
+    t0, t1 = target_probs.stride()
+    d0, d1 = vocab, 1
     if draft_probs is not None:
-        _need(draft_probs.shape == target_probs.shape and draft_probs.dtype == torch.float32
-              and draft_probs.device == dev and (vocab == 1 or draft_probs.stride(1) == 1),
-              "draft_probs: as target_probs")
-    stride = [vocab if t is None or rows <= 1 else t.stride(0) for t in (target_probs, draft_probs)]
-    _need(min(stride) >= vocab, "probabilities: rows must not overlap")
-    with _on(dev, stream, (tokens, target_probs, draft_probs, uniforms, sample_u, starts)) as st:
-        out = torch.empty(rows, dtype=torch.int32, device=dev)
-        accepted = torch.empty(seqs, dtype=torch.int32, device=dev)
-        _lib.check(_lib.load().megakernel_verify_drafts(
-            tokens.data_ptr(), target_probs.data_ptr(), stride[0],
-            None if draft_probs is None else draft_probs.data_ptr(), stride[1], uniforms.data_ptr(),
-            sample_u.data_ptr(), starts.data_ptr(), seqs, rows, vocab, out.data_ptr(), accepted.data_ptr(),
-            _status_of(dev).data_ptr(), st), "megakernel_verify_drafts")
+        if draft_probs.shape != target_probs.shape or draft_probs.dtype is not torch.float32 \
+                or draft_probs.get_device() != idx:
+            raise ValueError("draft_probs: float32, of target_probs' shape and device")
+        d0, d1 = draft_probs.stride()
+    if rows <= 1:
+        t0 = d0 = vocab
+    if ((t1 != 1 or d1 != 1) and vocab > 1) or t0 < vocab or d0 < vocab:
+        raise ValueError("probabilities: vocab contiguous, rows not overlapping")
+    if stream is not None or idx != _get_device():
+        return _elsewhere(verify_drafts, idx, stream, (tokens, target_probs, draft_probs, uniforms, sample_u, starts), {})
+    out = tokens.new_empty((rows,))
+    accepted = tokens.new_empty((seqs,))
+    rc = _fns()[4](tokens.data_ptr(), target_probs.data_ptr(), t0, None if draft_probs is None else draft_probs.data_ptr(),
+                   d0, uniforms.data_ptr(), sample_u.data_ptr(), starts.data_ptr(), seqs, rows, vocab, out.data_ptr(),
+                   accepted.data_ptr(), _status_of(idx), _raw_stream(idx))
+    if rc:
+        _lib.check(rc, "megakernel_verify_drafts")
     return out, accepted
+
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
 
 
 class PagedCache8:
