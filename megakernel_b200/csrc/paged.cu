@@ -3,6 +3,7 @@
 // verification of drafted tokens (C ABI in include/megakernel.h).  Attention
 // over the cache is in kv8_attend.cu.  The reference has no counterpart.
 #include "paged.cuh"
+#include "tc_ptx.cuh"
 
 namespace mkp {
 
@@ -195,8 +196,23 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, T* k, T* v, in
 // Products stay below 2^63 while a row's probabilities sum to less than 8.
 constexpr int kFix = 36, kFixU = 24;
 
+// rint(p 2^36) without a 64-bit conversion, as 2^23 (h - kMagicBits) +
+// (l - kMagicBits): p = H 2^-13 + rest, both parts exact in fp32; adding 2^23
+// leaves H (toward zero) and rint(rest 2^36) (to nearest even; the rest is 0 or
+// a whole number of units unless H is 0) in the low bits.  NaN counts as 0.
+constexpr uint32_t kMagicBits = 0x4b000000u;   // 2^23
+__device__ __forceinline__ float clamp01(float p) { return __saturatef(p); }   // NaN: 0
+__device__ __forceinline__ void fix_parts(float p, uint32_t& h, uint32_t& l) {
+  const float magic = 8388608.f, top = __fmaf_rz(p, 8192.f, magic);
+  const float rest = fmaf(top - magic, -1.f / 8192.f, p);
+  h = __float_as_uint(top);
+  l = __float_as_uint(fmaf(rest, 68719476736.f, magic));
+}
+__device__ __forceinline__ long long fix_join(int h, int l) { return (long long)h * (1LL << 23) + l; }
 __device__ __forceinline__ long long fix_p(float p) {
-  return p > 0.f ? __float2ll_rn(fminf(p, 1.f) * 68719476736.f) : 0;   // NaN: 0
+  uint32_t h, l;
+  fix_parts(clamp01(p), h, l);
+  return fix_join((int)(h - kMagicBits), (int)(l - kMagicBits));
 }
 __device__ __forceinline__ long long fix_u(float u) {
   return u > 0.f ? (long long)(fminf(u, 1.f) * 16777216.f) : 0;
@@ -211,30 +227,45 @@ struct Verify {
   int *out, *accepted, *status;
 };
 
-constexpr int kVerifyThreads = 1024;
+constexpr int kVerifyThreads = 512, kVerifyDeep = 16, kVerifyWarps = kVerifyThreads / 32, kVerifyChunks = 32;
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const Verify a) {
-  const int b = blockIdx.x, tid = threadIdx.x;
+// Inclusive sum over the warp.
+__device__ __forceinline__ long long warp_scan(long long v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long other = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += other;
+  }
+  return v;
+}
+
+// One cluster per sequence.  The vocabulary is cut into one run per block, each
+// run into one segment per warp, each segment into at most 32 chunks (of 512
+// tokens up to vocabularies of 262,144).  The rows are read once, 128 bytes per
+// warp and load (any alignment), 16 loads of each row in flight; the sum of
+// every chunk stays in shared memory.  The blocks add up through distributed
+// shared memory, and the block whose run holds the drawn point reads that one
+// chunk again, a token per thread.
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const Verify a) {
+  uint32_t rank, blocks;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+  const int b = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r0 = __ldg(a.starts + b), r1 = __ldg(a.starts + b + 1);
-  if (r0 < 0 || r1 < r0 || r1 > a.rows) {
-    if (tid == 0) {
-      report(a.status, MK_ERR_INVALID_ARG);
+  const bool bad = r0 < 0 || r1 < r0 || r1 > a.rows;
+  if (bad || r1 == r0) {   // the whole cluster
+    if (tid == 0 && rank == 0) {
+      if (bad) report(a.status, MK_ERR_INVALID_ARG);
       a.accepted[b] = 0;
     }
     return;
   }
   const int n = r1 - r0;
-  if (n == 0) {
-    if (tid == 0) a.accepted[b] = 0;
-    return;
-  }
-  // rows in order: the first draft that is refused
   __shared__ int s_acc;
-  __shared__ long long s_part[kVerifyThreads / 32], s_base;
-  __shared__ int s_token;
+  __shared__ long long s_chunk[kVerifyWarps][kVerifyChunks + 1], s_warp[kVerifyWarps], s_scan[kVerifyWarps], s_sum[2];
   if (tid == 0) s_acc = n - 1;
   __syncthreads();
-  for (int i = tid; i < n - 1; i += kVerifyThreads) {
+  for (int i = tid; i < n - 1; i += kVerifyThreads) {   // the first draft that is refused
     const int x = a.tokens[r0 + i + 1];
     bool keep = false;
     if (x >= 0 && x < a.vocab) {
@@ -250,64 +281,120 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const Verify a) 
   const float* p = a.target + (r0 + acc) * a.target_row;
   const float* q = refused && a.draft ? a.draft + (r0 + acc) * a.draft_row : nullptr;
   const int banned = refused && !a.draft ? a.tokens[r0 + acc + 1] : -1;
-  int token = -1;
-  for (int fallback = 0; fallback < 2; ++fallback) {
+
+  // run of this block, segment of this warp, chunk: multiples of kUnit tokens
+  constexpr int kUnit = 32 * kVerifyDeep;
+  const int parts = (int)blocks * kVerifyWarps;
+  const int chunk = (int)(((long long)a.vocab + (long long)parts * kVerifyChunks * kUnit - 1) /
+                          ((long long)parts * kVerifyChunks * kUnit)) * kUnit;
+  const int chunks = (int)(((long long)a.vocab + (long long)parts * chunk - 1) / ((long long)parts * chunk));
+  auto chunk_at = [&](int w, int i) {
+    return (int)min((((long long)rank * kVerifyWarps + w) * chunks + i) * chunk, (long long)a.vocab);
+  };
+
+  // The point lies in the first round unless every max(P - Q, 0) is zero; the
+  // second takes P itself.
+  for (int round = 0; round < 2; ++round) {
+    const float* less = round == 0 ? q : nullptr;
+    const int out = round == 0 ? banned : -1;
     auto weight = [&](int t) {
-      long long w = fix_p(p[t]);
-      if (!fallback) {
-        if (q) w = max(w - fix_p(q[t]), 0LL);
-        if (t == banned) w = 0;
-      }
-      return w;
+      long long w = fix_p(__ldg(p + t));
+      if (less) w = max(w - fix_p(__ldg(less + t)), 0LL);
+      return t == out ? 0LL : w;
     };
-    // each thread owns a contiguous run of tokens
-    const int run = (a.vocab + kVerifyThreads - 1) / kVerifyThreads;
-    const int t0 = min(tid * run, a.vocab), t1 = min(t0 + run, a.vocab);
     long long mine = 0;
-    for (int t = t0; t < t1; ++t) mine += weight(t);
-    long long upto = mine;
+    for (int ch = 0; ch < chunks; ++ch) {
+      const int t0 = chunk_at(warp, ch), t1 = chunk_at(warp, ch + 1);
+      long long sum = 0;
+      for (int t = t0 + lane; t - lane < t1; t += 32 * kVerifyDeep) {
+        float x[kVerifyDeep], y[kVerifyDeep];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-      if ((tid & 31) >= o) upto += other;
-    }
-    if ((tid & 31) == 31) s_part[tid >> 5] = upto;
-    if (tid == 0) s_token = -1;
-    __syncthreads();
-    if (tid < 32) {
-      long long w = s_part[tid];
+        for (int i = 0; i < kVerifyDeep; ++i) x[i] = t + 32 * i < t1 ? __ldg(p + t + 32 * i) : 0.f;
+        if (less) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, w, o);
-        if (tid >= o) w += other;
+          for (int i = 0; i < kVerifyDeep; ++i) y[i] = t + 32 * i < t1 ? __ldg(less + t + 32 * i) : 0.f;
+        }
+        // P - Q part by part in 32 bits (16 differences of at most 2^23); rounding
+        // keeps the order, so max(P - Q, 0) is P - Q exactly where p > q
+        int hs = 0, ls = 0;
+#pragma unroll
+        for (int i = 0; i < kVerifyDeep; ++i) {
+          const float u = t + 32 * i == out ? 0.f : clamp01(x[i]);
+          uint32_t h, l, h2 = kMagicBits, l2 = kMagicBits;
+          fix_parts(u, h, l);
+          float v = 0.f;
+          if (less) {
+            v = clamp01(y[i]);
+            fix_parts(v, h2, l2);
+          }
+          if (u > v) {
+            hs += (int)(h - h2);
+            ls += (int)(l - l2);
+          }
+        }
+        sum += fix_join(hs, ls);
       }
-      s_part[tid] = w;
-      if (tid == 31) s_base = w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s_chunk[warp][ch] = sum;
+      mine += sum;
     }
+    if (lane == 0) s_warp[warp] = mine;
     __syncthreads();
-    const long long total = s_base;
-    if (tid >= 32) upto += s_part[(tid >> 5) - 1];
-    if (total > 0) {
-      const long long bar = (fix_u(a.sample_u[b]) * total) >> kFixU;
-      if (upto - mine <= bar && bar < upto) {
-        long long sum = upto - mine;
-        for (int t = t0; t < t1; ++t) {
-          sum += weight(t);
-          if (sum > bar) {
-            s_token = t;
+    if (warp == 0) {
+      const long long v = warp_scan(lane < kVerifyWarps ? s_warp[lane] : 0LL);
+      if (lane < kVerifyWarps) s_scan[lane] = v;
+      if (lane == kVerifyWarps - 1) s_sum[round] = v;
+    }
+    mk::cluster_sync_all();
+    long long total = 0, before = 0;
+    for (uint32_t k = 0; k < blocks; ++k) {
+      long long v;
+      asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(mk::mapa_shared(mk::smem_u32(&s_sum[round]), k)) : "memory");
+      if (k < rank) before += v;
+      total += v;
+    }
+    if (total == 0) {
+      // nothing to draw from: P itself next, or no token
+      if (round == 1 && rank == 0 && tid == 0) a.out[r0 + acc] = -1;
+      __syncthreads();
+      continue;
+    }
+    const long long bar = ((fix_u(a.sample_u[b]) * total) >> kFixU) - before;
+    if (bar >= 0 && bar < s_sum[round]) {
+      int w = 0;
+      while (bar >= s_scan[w]) ++w;
+      long long rest = bar - (w ? s_scan[w - 1] : 0);
+      int ch = 0;
+      for (; rest >= s_chunk[w][ch]; ++ch) rest -= s_chunk[w][ch];
+      const int u0 = chunk_at(w, ch), u1 = chunk_at(w, ch + 1);
+      const int run = (u1 - u0 + kVerifyThreads - 1) / kVerifyThreads;
+      const int v0 = min(u0 + tid * run, u1), v1 = min(v0 + run, u1);
+      long long own = 0;
+      for (int i = v0; i < v1; ++i) own += weight(i);
+      long long upto = warp_scan(own);
+      if (lane == 31) s_warp[warp] = upto;
+      __syncthreads();
+      for (int i = 0; i < warp; ++i) upto += s_warp[i];
+      if (upto - own <= rest && rest < upto) {
+        long long sum = upto - own;
+        for (int i = v0; i < v1; ++i) {
+          sum += weight(i);
+          if (sum > rest) {
+            a.out[r0 + acc] = i;
             break;
           }
         }
       }
-      __syncthreads();
-      token = s_token;
-      break;
     }
-    __syncthreads();
+    break;
   }
-  for (int i = tid; i < n; i += kVerifyThreads)
-    a.out[r0 + i] = i < acc ? a.tokens[r0 + i + 1] : i == acc ? token : -1;
-  if (tid == 0) a.accepted[b] = acc;
+  if (rank == 0) {
+    for (int i = tid; i < n; i += kVerifyThreads)
+      if (i != acc) a.out[r0 + i] = i < acc ? a.tokens[r0 + i + 1] : -1;
+    if (tid == 0) a.accepted[b] = acc;
+  }
+  mk::cluster_sync_all();   // peers have read s_sum
 }
 
 // ---- host side -----------------------------------------------------------------------
@@ -470,7 +557,7 @@ int megakernel_verify_drafts(const int* d_tokens, const float* d_target, long lo
                              long long draft_row, const float* d_uniforms, const float* d_sample_u,
                              const int* d_starts, int seqs, int rows, int vocab, int* d_out, int* d_accepted,
                              int* d_status, void* stream) {
-  if (seqs < 0 || rows < 0 || vocab < 1 || rows > (1 << 30)) return MK_ERR_INVALID_ARG;
+  if (seqs < 0 || rows < 0 || vocab < 1 || rows > (1 << 30) || vocab > (1 << 29) || seqs > (1 << 24)) return MK_ERR_INVALID_ARG;
   if (seqs == 0) return MK_OK;
   if (!d_starts || !d_accepted) return MK_ERR_INVALID_ARG;
   if (rows > 0 && (!d_tokens || !d_target || !d_uniforms || !d_sample_u || !d_out || target_row < vocab ||
@@ -478,8 +565,20 @@ int megakernel_verify_drafts(const int* d_tokens, const float* d_target, long lo
     return MK_ERR_INVALID_ARG;
   const Verify a{d_tokens, d_target, d_draft, d_uniforms, d_sample_u, target_row, draft_row,
                  d_starts, seqs, rows, vocab, d_out, d_accepted, d_status};
-  verify_kernel<<<(unsigned)seqs, kVerifyThreads, 0, (cudaStream_t)stream>>>(a);
-  return launched();
+  // Blocks per sequence: 4, or 8 while all of them fit the GPU at once (two per
+  // SM), but none with less than 8,192 tokens.
+  unsigned blocks = 1;
+  while (blocks < 8 && vocab > (int)blocks * 8192 && (blocks < 4 || seqs * blocks * 2 <= 2 * 148)) blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)seqs * blocks);
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {blocks, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, verify_kernel, a) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
 }
 
 }  // extern "C"
