@@ -227,7 +227,7 @@ struct Verify {
   int *out, *accepted, *status;
 };
 
-constexpr int kVerifyThreads = 512, kVerifyDeep = 16, kVerifyWarps = kVerifyThreads / 32, kVerifyChunks = 32;
+constexpr int kVerifyThreads = 256, kVerifyDeep = 16, kVerifyWarps = kVerifyThreads / 32, kVerifyChunks = 32;
 
 // Inclusive sum over the warp.
 __device__ __forceinline__ long long warp_scan(long long v) {
@@ -241,12 +241,13 @@ __device__ __forceinline__ long long warp_scan(long long v) {
 
 // One cluster per sequence.  The vocabulary is cut into one run per block, each
 // run into one segment per warp, each segment into at most 32 chunks (of 512
-// tokens up to vocabularies of 262,144).  The rows are read once, 128 bytes per
-// warp and load (any alignment), 16 loads of each row in flight; the sum of
+// tokens up to vocabularies of 262,144).  The rows are read once in 16-byte
+// vectors (single words at the ends, or where p and q lie differently), 16
+// tokens of each row per thread in flight; the sum of
 // every chunk stays in shared memory.  The blocks add up through distributed
 // shared memory, and the block whose run holds the drawn point reads that one
 // chunk again, a token per thread.
-__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const Verify a) {
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const Verify a) {
   uint32_t rank, blocks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
@@ -285,11 +286,23 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const Verify 
   // run of this block, segment of this warp, chunk: multiples of kUnit tokens
   constexpr int kUnit = 32 * kVerifyDeep;
   const int parts = (int)blocks * kVerifyWarps;
-  const int chunk = (int)(((long long)a.vocab + (long long)parts * kVerifyChunks * kUnit - 1) /
+  const int chunk = (int)(((long long)a.vocab + 3 + (long long)parts * kVerifyChunks * kUnit - 1) /
                           ((long long)parts * kVerifyChunks * kUnit)) * kUnit;
-  const int chunks = (int)(((long long)a.vocab + (long long)parts * chunk - 1) / ((long long)parts * chunk));
-  auto chunk_at = [&](int w, int i) {
-    return (int)min((((long long)rank * kVerifyWarps + w) * chunks + i) * chunk, (long long)a.vocab);
+  const int chunks = (int)(((long long)a.vocab + 3 + (long long)parts * chunk - 1) / ((long long)parts * chunk));
+  // A chunk begins where p's address is a multiple of 16 bytes (but for the first).
+  const int shift = (int)(((uintptr_t)p >> 2) & 3);
+  const bool q_vec = (((uintptr_t)p ^ (uintptr_t)q) & 15) == 0;
+  auto chunk_raw = [&](int w, int i) { return (((long long)rank * kVerifyWarps + w) * chunks + i) * chunk - shift; };
+  auto chunk_at = [&](int w, int i) { return (int)min(max(chunk_raw(w, i), 0LL), (long long)a.vocab); };
+  // four tokens from t on; what lies outside [0, vocab) counts as 0
+  auto four = [&](const float* row, long long t, bool vec, float* x) {
+    if (vec && t >= 0 && t + 4 <= a.vocab) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(row + t));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = t + i >= 0 && t + i < a.vocab ? __ldg(row + t + i) : 0.f;
+    }
   };
 
   // The point lies in the first round unless every max(P - Q, 0) is zero; the
@@ -304,22 +317,22 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const Verify 
     };
     long long mine = 0;
     for (int ch = 0; ch < chunks; ++ch) {
-      const int t0 = chunk_at(warp, ch), t1 = chunk_at(warp, ch + 1);
       long long sum = 0;
-      for (int t = t0 + lane; t - lane < t1; t += 32 * kVerifyDeep) {
+      for (long long t = chunk_raw(warp, ch) + 4 * lane; t - 4 * lane < chunk_raw(warp, ch + 1); t += kUnit) {
+        if (t - 4 * lane >= a.vocab) break;
         float x[kVerifyDeep], y[kVerifyDeep];
 #pragma unroll
-        for (int i = 0; i < kVerifyDeep; ++i) x[i] = t + 32 * i < t1 ? __ldg(p + t + 32 * i) : 0.f;
+        for (int i = 0; i < kVerifyDeep; i += 4) four(p, t + 32 * i, true, x + i);
         if (less) {
 #pragma unroll
-          for (int i = 0; i < kVerifyDeep; ++i) y[i] = t + 32 * i < t1 ? __ldg(less + t + 32 * i) : 0.f;
+          for (int i = 0; i < kVerifyDeep; i += 4) four(less, t + 32 * i, q_vec, y + i);
         }
         // P - Q part by part in 32 bits (16 differences of at most 2^23); rounding
         // keeps the order, so max(P - Q, 0) is P - Q exactly where p > q
         int hs = 0, ls = 0;
 #pragma unroll
         for (int i = 0; i < kVerifyDeep; ++i) {
-          const float u = t + 32 * i == out ? 0.f : clamp01(x[i]);
+          const float u = t + 32 * (i & ~3) + (i & 3) == out ? 0.f : clamp01(x[i]);
           uint32_t h, l, h2 = kMagicBits, l2 = kMagicBits;
           fix_parts(u, h, l);
           float v = 0.f;
@@ -565,10 +578,11 @@ int megakernel_verify_drafts(const int* d_tokens, const float* d_target, long lo
     return MK_ERR_INVALID_ARG;
   const Verify a{d_tokens, d_target, d_draft, d_uniforms, d_sample_u, target_row, draft_row,
                  d_starts, seqs, rows, vocab, d_out, d_accepted, d_status};
-  // Blocks per sequence: 4, or 8 while all of them fit the GPU at once (two per
-  // SM), but none with less than 8,192 tokens.
+  // Blocks per sequence: up to 8, at least 8,192 tokens each (32 per thread).
+  // 64 sequences x 151,936: 23.0 us; 4 blocks of 512 threads 23.6, 8 of 512
+  // (two waves) 32.5, 8 of 128 25.2.
   unsigned blocks = 1;
-  while (blocks < 8 && vocab > (int)blocks * 8192 && (blocks < 4 || seqs * blocks * 2 <= 2 * 148)) blocks *= 2;
+  while (blocks < 8 && vocab > (int)blocks * 8192) blocks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)seqs * blocks);
   cfg.blockDim = dim3(kVerifyThreads);
