@@ -1,5 +1,10 @@
 // Attention over the paged 8-bit cache (megakernel_kv8_attend).
 #include "paged.cuh"
+#include "tc_ptx.cuh"
+
+#ifndef ATT_FILL
+#define ATT_FILL 3
+#endif
 
 namespace mkp {
 
@@ -63,10 +68,6 @@ __device__ __forceinline__ void store_out(void* o, long long i, float v, bool bf
   else ((__half*)o)[i] = __float2half_rn(v);
 }
 
-// Every thread of every block of the cluster arrives and waits.
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // The word at p's place in the shared memory of block `rank` of the cluster.
 __device__ __forceinline__ float remote_f32(const float* p, uint32_t rank) {
   uint32_t at;
@@ -82,10 +83,12 @@ __device__ __forceinline__ uint64_t policy_evict_normal() {
   return pol;
 }
 
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 constexpr int kWarps = 4;
-constexpr int kStageBytes = 4096;      // K and V of one step
+constexpr int kStageBytes = 8192;      // K and V codes of one step
 constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr float kNone = -1e30f;        // running reference of a row that has seen nothing
+constexpr float kSlack = 5.f;          // weights may reach 2^kSlack before the reference moves
 
 // Bounded wait; each probe may itself suspend for a while.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
@@ -94,45 +97,58 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-template <int D, int MW>
+template <int D, int NT, int MW>
 constexpr int rows_smem() {
-  constexpr int ring = (kWarps / MW) * kStages * kStageBytes, parts = kWarps * 16 * D * 4;
+  constexpr int ring = (kWarps / MW) * kStages * kStageBytes, parts = kWarps * 8 * NT * D * 4;
   return ring > parts ? ring : parts;
+}
+
+// 8 x 8 f16 matrix, lane (g, t) holding row g, columns 2 t and 2 t + 1 -> its transpose.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // ---- attention of few rows per sequence -------------------------------------------------
 //
-// Work item: (16 MW rows of one sequence and kv head, counting a row once per
+// Work item: (8 NT MW rows of one sequence and kv head, counting a row once per
 // query head of the group; the positions split over the S blocks of a cluster
-// and their warps).  MW warps that hold 16 rows each share a stream of steps
+// and their warps).  MW warps that hold 8 NT rows each share a stream of steps
 // of TS positions; the 4 / MW such groups of a block, and the blocks of the
 // cluster, take every (4 / MW) S-th step.
 //
 // The codes of a step, contiguous in a page, arrive by bulk copies in a ring
-// of four stages per group (K 2 KB and V 2 KB each): nothing of the stream
-// passes through registers before it is used.  Scores and output are
-// m16n8k16 f16 products with fp32 accumulation.  The order of the head
-// dimension in the first product and of the output columns in the second is
-// free, so a lane reads 16 consecutive bytes of K (its part of four k-steps)
-// and 8 or 16 consecutive bytes of V from each of four positions; the code
-// bytes become f16 in registers, exactly.  q is brought to 2^14 by a power of
-// two per row (bf16 values fit f16 then, 2^-39 of the row's largest lost at
-// most).
+// per group (K 4 KB and V 4 KB a stage): nothing of the stream passes through
+// registers before it is used.  Both products have the positions or the head
+// dimension as the 16 rows of an m16n8k16 f16 product and the query rows as
+// its 8 columns, fp32 accumulation:
+//   S^T [positions x rows] = K Q^T,   O^T [dims x rows] += V^T P^T,
+// so that 8 rows (a decode step of 8 query heads per kv head) waste nothing.
+// The order of the head dimension in the first product and of the output's
+// rows in the second is free, so a lane reads 16 consecutive bytes of K (its
+// part of four k-steps) and D / 8 consecutive bytes of V from each of four
+// positions; the code bytes become f16 in registers, exactly.  q is brought to
+// 2^14 by a power of two per row (bf16 values fit f16 then, 2^-39 of the row's
+// largest lost at most).
 //
-// Softmax per row with running maximum m and sum l of p = 2^(s - m), fp32.
-// The scale of a K page multiplies the scores, that of a V page the weights:
-// w = 2^15 p scale / vref, vref the largest V scale so far, goes into the second
-// product in f16: 11 bits down to 2^-29 of the row's largest, an absolute 2^-40
-// below that (at 1 instead of 2^15 it was 2^-25, which rows with one dominant
-// position showed).  The sum l takes the unrounded p.
-template <class F, int P, int D, int MW>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kernel(const Cache c, const Attend a) {
-  constexpr int TS = 2048 / D, NB = TS / 8, kSub = TS > P ? TS / P : 1, kGroups = kWarps / MW;
+// Softmax per row relative to a running reference m: p = 2^(s - m), l = sum p,
+// fp32.  m moves to the maximum only when some p would pass 2^5 (one vote per
+// 32 positions), so most steps have no exchange between lanes at all.  The
+// scale of a K page multiplies the scores, that of a V page the weights:
+// w = 2^10 p scale / vref, vref the largest V scale so far, goes into the second
+// product in f16: 11 bits down to 2^-29 of the row's largest, an absolute 2^-35
+// below that (at p scale / vref alone it was 2^-25, which rows with one
+// dominant position showed).  The sum l takes the unrounded p.
+template <class F, int P, int D, int NT, int MW>
+__global__ void __launch_bounds__(kWarps * 32, D == 64 || NT == 1 ? 3 : 2) attend_rows_kernel(const Cache c, const Attend a) {
+  constexpr int TS = kStageBytes / 2 / D, kSub = TS > P ? TS / P : 1, kGroups = kWarps / MW;
   constexpr int kSubRows = TS / kSub;               // positions of a step in one page
   constexpr int kBatch = 32 / kSub;                 // steps whose pages the lanes hold
+  constexpr int R = 8 * NT;                         // rows of a warp
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t s_full[kGroups * kStages], s_empty[kGroups * kStages];
-  __shared__ float s_m[kWarps][16], s_l[kWarps][16], s_v[kWarps], s_top[MW * 16], s_sum[MW * 16];
+  __shared__ float s_m[kWarps][R], s_l[kWarps][R], s_v[kWarps], s_top[MW * R], s_sum[MW * R];
   __shared__ int s_nan;
 
   uint32_t rank, split;
@@ -143,17 +159,17 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
   const int group = a.q_heads / c.kv_heads;
   const int cta = blockIdx.x / split, h = cta % c.kv_heads, item = cta / c.kv_heads;
 
-  // sequence b owns the items from starts[b] group / (16 MW) + b on
-  auto key = [&](int i) { return (int)((long long)__ldg(c.starts + i) * group / (16 * MW)) + i; };
+  // sequence b owns the items from starts[b] group / (R MW) + b on
+  auto key = [&](int i) { return (int)((long long)__ldg(c.starts + i) * group / (R * MW)) + i; };
   const int b = warp_search(c.seqs, item, key);
   const int r0 = __ldg(c.starts + b), r1 = __ldg(c.starts + b + 1), first = __ldg(c.first + b);
   if (r0 < 0 || r1 < r0 || r1 > c.rows || first > (1 << 30)) {
     report(a.status, MK_ERR_INVALID_ARG);
     return;   // the whole cluster: every block of it has this item
   }
-  const int n = r1 - r0, m0 = (item - key(b)) * 16 * MW;
+  const int n = r1 - r0, m0 = (item - key(b)) * R * MW;
   if (m0 < 0 || m0 >= n * group) return;
-  const int valid = min(n * group - m0, 16 * MW);
+  const int valid = min(n * group - m0, R * MW);
   int len = a.kv_lens ? __ldg(a.kv_lens + b) : first + n;
   if (len > c.table_width * P) {
     report(a.status, MK_ERR_CAPACITY);
@@ -173,30 +189,31 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
   sees(m0, lo_all, hi_min);
   const int begin = lo_all / TS * TS;
   const int all_steps = hi_all > begin ? (hi_all - begin + TS - 1) / TS : 0;
-  const int lanes_of_steps = (int)split * kGroups, my = (int)rank * kGroups + grp;
-  const int steps = all_steps > my ? (all_steps - my - 1) / lanes_of_steps + 1 : 0;
+  const int stride = (int)split * kGroups, my = (int)rank * kGroups + grp;
+  const int steps = all_steps > my ? (all_steps - my - 1) / stride + 1 : 0;
 
   if (threadIdx.x == 0) {
     s_nan = 0;
     for (int i = 0; i < kGroups * kStages; ++i) {
-      mk::mbar_init(&s_full[i], 1);
+      mk::mbar_init(&s_full[i], kSub);
       mk::mbar_init(&s_empty[i], MW);
     }
     mk::fence_mbar_init();
   }
   __syncthreads();
 
-  // pages of kBatch steps, one per lane: id (-1: not wanted, or reported), scales
+  // Pages of kBatch steps, one per lane: id (-1: not wanted, or reported) and
+  // scales (a K scale of 0 marks a page that is not there).
   struct Page { int id; float ks, vs; };
   auto pages_from = [&](int step) {
-    Page p{-1, 1.f, 0.f};   // a V scale of 0 leaves vref alone
+    Page p{-1, 0.f, 0.f};
     const int st = step + lane / kSub;
-    const int pos = begin + (st * lanes_of_steps + my) * TS + (lane % kSub) * kSubRows;
+    const int pos = begin + (st * stride + my) * TS + (lane % kSub) * kSubRows;
     if (st < steps && pos < hi_all && pos + kSubRows > lo_all) {
       p.id = page_id(c, b, pos / P, a.status);
       if (p.id >= 0) {
         const float* sc = c.scales + p.id * c.scale_stride + h;
-        p.ks = __ldg(sc);
+        p.ks = fmaxf(__ldg(sc), 1.17549435e-38f);
         p.vs = __ldg(sc + c.kv_heads);
       }
     }
@@ -206,43 +223,35 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
   int base = 0;
   uint8_t* ring = smem + grp * kStages * kStageBytes;
   // Codes that no other item reads do not stay in the L2 cache.
-  const uint64_t policy = n * group <= 16 * MW ? mk::policy_evict_first() : policy_evict_normal();
-  auto fetch = [&](int st) {   // by the whole first warp of a group
-    if (st >= steps) return;
-    const int pos = begin + (st * lanes_of_steps + my) * TS;
-    int ids[kSub];
-    uint32_t bytes = 0;
-#pragma unroll
-    for (int i = 0; i < kSub; ++i) {
-      const int src = (st - base) * kSub + i;
-      ids[i] = src < 32 ? __shfl_sync(0xffffffffu, cur.id, src) : __shfl_sync(0xffffffffu, nxt.id, src - 32);
-      bytes += ids[i] >= 0 ? 2 * kSubRows * D : 0;
-    }
-    if (lane == 0) {
+  const uint64_t policy = n * group <= R * MW ? mk::policy_evict_first() : policy_evict_normal();
+  // The lanes that hold the pages of step st copy their part of it.
+  auto fetch = [&](int st) {
+    const int id = st - base < kBatch ? cur.id : nxt.id;
+    if (st < steps && lane / kSub == (st - base) % kBatch) {
       uint64_t* bar = &s_full[grp * kStages + st % kStages];
-      uint8_t* dst = ring + st % kStages * kStageBytes;
-      mk::mbar_arrive_expect_tx(bar, bytes);
-#pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        if (ids[i] < 0) continue;
-        const uint8_t* k = c.codes + ids[i] * c.page_stride + ((long long)h * P + (pos + i * kSubRows) % P) * D;
-        mk::bulk_g2s(dst + i * kSubRows * D, k, kSubRows * D, bar, policy);
-        mk::bulk_g2s(dst + TS * D + i * kSubRows * D, k + (long long)c.kv_heads * P * D, kSubRows * D, bar, policy);
+      const int sub = lane % kSub;
+      mk::mbar_arrive_expect_tx(bar, id >= 0 ? 2 * kSubRows * D : 0);
+      if (id >= 0) {
+        const int pos = begin + (st * stride + my) * TS + sub * kSubRows;
+        uint8_t* dst = ring + st % kStages * kStageBytes + sub * kSubRows * D;
+        const uint8_t* k = c.codes + id * c.page_stride + ((long long)h * P + pos % P) * D;
+        mk::bulk_g2s(dst, k, kSubRows * D, bar, policy);
+        mk::bulk_g2s(dst + TS * D, k + (long long)c.kv_heads * P * D, kSubRows * D, bar, policy);
       }
     }
   };
   if (mw == 0)
     for (int i = 0; i < kStages; ++i) fetch(i);
 
-  // q fragments of rows g and g + 8 of this warp's tile: k-step j holds
-  // dimensions 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1 | 2, 3}
-  uint32_t q[D / 16][4];
-  float rq[2];
-  int lo[2], hi[2];
+  // q fragments, row 8 nt + g of this warp: k-step j holds dimensions
+  // 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1 | 2, 3}.  rq, lo, hi: rows 2 t and
+  // 2 t + 1, whose scores this lane will hold.
+  uint32_t q[NT][D / 16][2];
+  float rq[NT][2];
+  int lo[NT][2], hi[NT][2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int m = m0 + mw * 16 + g + 8 * e;
-    sees(m, lo[e], hi[e]);
+  for (int nt = 0; nt < NT; ++nt) {
+    const int m = m0 + mw * R + 8 * nt + g;
     const bool real = m < n * group;
     const long long at = real ? (long long)(r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head : 0;
     float v[D / 4];
@@ -257,16 +266,24 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
     // power of two that brings the largest to [2^14, 2^15)
     const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);
     const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
-    rq[e] = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
-      q[j][e] = pack_f16(v[4 * j] * up, v[4 * j + 1] * up);
-      q[j][2 + e] = pack_f16(v[4 * j + 2] * up, v[4 * j + 3] * up);
+      q[nt][j][0] = pack_f16(v[4 * j] * up, v[4 * j + 1] * up);
+      q[nt][j][1] = pack_f16(v[4 * j + 2] * up, v[4 * j + 3] * up);
+    }
+    const float back = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      rq[nt][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
+      sees(m0 + mw * R + 8 * nt + 2 * t + e, lo[nt][e], hi[nt][e]);
     }
   }
 
-  float o[D / 8][4] = {};
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f;
+  float o[NT][D / 16][4] = {};
+  float m[NT][2], l[NT][2], vref = 0.f, iv = 0.f;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+    for (int e = 0; e < 2; ++e) m[nt][e] = kNone, l[nt][e] = 0.f;
   bool alive = true;
   int nan_seen = 0, failed = 0;
   for (int st = 0; st < steps; ++st) {
@@ -276,18 +293,28 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
       nxt = pages_from(base + kBatch);
     }
     float ks[kSub], vs[kSub];
-    bool have[kSub], whole = true;
     float vmax = vref;
+    bool whole = true;
 #pragma unroll
     for (int i = 0; i < kSub; ++i) {
       const int src = (st - base) * kSub + i;
       ks[i] = __shfl_sync(0xffffffffu, cur.ks, src);
       vs[i] = __shfl_sync(0xffffffffu, cur.vs, src);
-      have[i] = __shfl_sync(0xffffffffu, cur.id, src) >= 0;
-      whole = whole && have[i];
+      whole = whole && ks[i] > 0.f;
       vmax = fmaxf(vmax, vs[i]);
     }
-    const int pos = begin + (st * lanes_of_steps + my) * TS;
+    if (vmax > vref) {
+      const float r = vref / vmax;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[nt][i][x] *= r;
+      vref = vmax;
+      iv = 1024.f / vmax;
+    }
+    const int pos = begin + (st * stride + my) * TS;
     whole = whole && pos >= lo_max && pos + TS <= hi_min;
     if (!wait_bar(&s_full[grp * kStages + st % kStages], (st / kStages) & 1)) {
       alive = false;
@@ -297,126 +324,130 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
     const uint8_t* kb = ring + st % kStages * kStageBytes;
     const uint8_t* vb = kb + TS * D;
 
-    float s[NB][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+    for (int half = 0; half < TS / 32; ++half) {   // 32 positions
+      float s[2][NT][4];
 #pragma unroll
-      for (int half = 0; half < D / 64; ++half) {
-        const uint4 w = *reinterpret_cast<const uint4*>(kb + (nb * 8 + g) * D + half * 64 + 16 * t);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+      for (int mt = 0; mt < 2; ++mt) {
+        const uint8_t* k0 = kb + (half * 32 + mt * 16 + g) * D + 16 * t;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t b0, b1;
-          expand<F>(ws[j], b0, b1);
-          mma_f16(s[nb], q[half * 4 + j], b0, b1);
+        for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) {
+          const uint4 x = *reinterpret_cast<const uint4*>(k0 + d * 64);
+          const uint4 y = *reinterpret_cast<const uint4*>(k0 + d * 64 + 8 * D);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t ka[4];
+            expand<F>(xs[j], ka[0], ka[2]);
+            expand<F>(ys[j], ka[1], ka[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[mt][nt], ka, q[nt][d * 4 + j][0], q[nt][d * 4 + j][1]);
+          }
         }
       }
-    }
-    if (!whole) {
+      float f[2][NT][2];
+      bool over = false;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int mt = 0; mt < 2; ++mt) {
+        const int i = (half * 32 + mt * 16) / kSubRows;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = pos + nb * 8 + 2 * t + (i & 1), e = i >> 1;
-          if (!have[nb * 8 / kSubRows] || j < lo[e] || j >= hi[e]) s[nb][i] = -INFINITY;
-        }
-    }
-    // running maximum; the factors of the two rows
-    float f[kSub][2], top[2] = {m[0], m[1]};
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int i = 0; i < kSub; ++i) {
+          for (int e = 0; e < 2; ++e) f[mt][nt][e] = fmaxf(rq[nt][e] * ks[i], 1.17549435e-38f);   // -inf x 0 would be NaN
+          if (!whole) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        f[i][e] = fmaxf(rq[e] * ks[i], 1.17549435e-38f);   // -inf x 0 would be NaN
-        float x = -INFINITY;
+            for (int x = 0; x < 4; ++x) {
+              const int j = pos + half * 32 + mt * 16 + g + 8 * (x >> 1);
+              if (ks[i] == 0.f || j < lo[nt][x & 1] || j >= hi[nt][x & 1]) s[mt][nt][x] = -INFINITY;
+            }
+          }
 #pragma unroll
-        for (int nb = i * kSubRows / 8; nb < (i + 1) * kSubRows / 8; ++nb) x = fmaxf(x, fmaxf(s[nb][2 * e], s[nb][2 * e + 1]));
-        top[e] = fmaxf(top[e], x * f[i][e]);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-      top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-    }
-    float sub[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) sub[e] = top[e] == -INFINITY ? 0.f : top[e];
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]) || vmax > vref) {
-      const float vr = vmax > vref ? vref / vmax : 1.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float keep = ex2(m[e] - sub[e]);
-        l[e] *= keep;
-        m[e] = top[e];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][2 * e] *= keep * vr;
-          o[i][2 * e + 1] *= keep * vr;
+          for (int x = 0; x < 4; ++x) over = over || fmaf(s[mt][nt][x], f[mt][nt][x & 1], -m[nt][x & 1]) > kSlack;
         }
       }
-      vref = vmax;
-    }
-    float rv[kSub];
-    const float iv = vref > 0.f ? 32768.f / vref : 0.f;
+      if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-    for (int i = 0; i < kSub; ++i) rv[i] = vs[i] * iv;
-    uint32_t w[NB][2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int i = nb * 8 / kSubRows;
+          for (int e = 0; e < 2; ++e) {
+            float top = m[nt][e];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float x = ex2(fmaf(s[nb][2 * e], f[i][e], -sub[e])), y = ex2(fmaf(s[nb][2 * e + 1], f[i][e], -sub[e]));
-        l[e] += x + y;
-        w[nb][e] = pack_f16(x * rv[i], y * rv[i]);
+            for (int mt = 0; mt < 2; ++mt)
+              top = fmaxf(top, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]) * f[mt][nt][e]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float keep = ex2(m[nt][e] - top);
+            m[nt][e] = top;
+            l[nt][e] *= keep;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              o[nt][i][e] *= keep;
+              o[nt][i][2 + e] *= keep;
+            }
+          }
       }
-    }
 #pragma unroll
-    for (int kk = 0; kk < NB / 2; ++kk) {
-      const uint32_t pa[4] = {w[2 * kk][0], w[2 * kk][1], w[2 * kk + 1][0], w[2 * kk + 1][1]};
-      uint32_t v[4][D / 32];
+      for (int mt = 0; mt < 2; ++mt) {
+        const int at = half * 32 + mt * 16, i = at / kSubRows;
+        const float rv = vs[i] * iv;
+        uint32_t pb[NT][2];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int row = kk * 16 + 2 * t + (x & 1) + 8 * (x >> 1);
-        const uint8_t* p = vb + row * D + g * (D / 8);
-        if constexpr (D == 64) {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          v[x][0] = u.x; v[x][1] = u.y;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(p);
-          v[x][0] = u.x; v[x][1] = u.y; v[x][2] = u.z; v[x][3] = u.w;
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            p[x] = ex2(fmaf(s[mt][nt][x], f[mt][nt][x & 1], -m[nt][x & 1]));
+            l[nt][x & 1] += p[x];
+          }
+          pb[nt][0] = transpose8(pack_f16(p[0] * rv, p[1] * rv));
+          pb[nt][1] = transpose8(pack_f16(p[2] * rv, p[3] * rv));
         }
-        if (!whole) {
-          // What no row sees may hold anything: its codes count as 0.  A NaN
-          // that only some rows see is taken out here and put back at the end.
-          const bool dead = !have[row / kSubRows] || pos + row >= hi_all || pos + row < lo_all;
+        uint32_t v[4][D / 32];   // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            if (dead) v[x][i] = 0;
-            if constexpr (F::kTopExp == 8) {
-              const uint32_t bad = nan_bytes(v[x][i]);
-              if (bad) {
-                nan_seen = 1;
-                v[x][i] &= ~((bad >> 7) * 0xffu);
+        for (int x = 0; x < 4; ++x) {
+          const int row = at + 2 * t + (x & 1) + 8 * (x >> 1);
+          const uint8_t* vp = vb + row * D + g * (D / 8);
+          if constexpr (D == 64) {
+            const uint2 u = *reinterpret_cast<const uint2*>(vp);
+            v[x][0] = u.x; v[x][1] = u.y;
+          } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(vp);
+            v[x][0] = u.x; v[x][1] = u.y; v[x][2] = u.z; v[x][3] = u.w;
+          }
+          if (!whole) {
+            // What no row sees may hold anything: its codes count as 0.  A NaN
+            // that only some rows see is taken out here and put back at the end.
+            const bool dead = ks[i] == 0.f || pos + row >= hi_all || pos + row < lo_all;
+#pragma unroll
+            for (int y = 0; y < D / 32; ++y) {
+              if (dead) v[x][y] = 0;
+              if constexpr (F::kTopExp == 8) {
+                const uint32_t bad = nan_bytes(v[x][y]);
+                if (bad) {
+                  nan_seen = 1;
+                  v[x][y] &= ~((bad >> 7) * 0xffu);
+                }
               }
             }
           }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        // byte pairs of two positions: (d0, d1), (d2, d3)
-        uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
-        expand<F>(__byte_perm(v[0][i], v[1][i], 0x5140), a0, a1);
-        expand<F>(__byte_perm(v[0][i], v[1][i], 0x7362), a2, a3);
-        expand<F>(__byte_perm(v[2][i], v[3][i], 0x5140), b0, b1);
-        expand<F>(__byte_perm(v[2][i], v[3][i], 0x7362), b2, b3);
-        mma_f16(o[4 * i], pa, a0, b0);
-        mma_f16(o[4 * i + 1], pa, a1, b1);
-        mma_f16(o[4 * i + 2], pa, a2, b2);
-        mma_f16(o[4 * i + 3], pa, a3, b3);
+        for (int y = 0; y < D / 32; ++y) {
+          // byte pairs of two positions; dimensions 4 y + {0, 1} and {2, 3} of this lane
+          uint32_t va[4], vc[4];
+          expand<F>(__byte_perm(v[0][y], v[1][y], 0x5140), va[0], va[1]);
+          expand<F>(__byte_perm(v[2][y], v[3][y], 0x5140), va[2], va[3]);
+          expand<F>(__byte_perm(v[0][y], v[1][y], 0x7362), vc[0], vc[1]);
+          expand<F>(__byte_perm(v[2][y], v[3][y], 0x7362), vc[2], vc[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(o[nt][2 * y], va, pb[nt][0], pb[nt][1]);
+            mma_f16(o[nt][2 * y + 1], vc, pb[nt][0], pb[nt][1]);
+          }
+        }
       }
     }
     __syncwarp();
@@ -445,71 +476,73 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
 
   // ---- join the warps, then the blocks of the cluster
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    if (t == 0) {
-      s_m[warp][g + 8 * e] = m[e];
-      s_l[warp][g + 8 * e] = l[e];
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[nt][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (g == 0) {
+        s_m[warp][8 * nt + 2 * t + e] = m[nt][e];
+        s_l[warp][8 * nt + 2 * t + e] = x;
+      }
     }
-  }
-  if (lane == 0) s_v[warp] = vref * (1.f / 32768.f);
+  if (lane == 0) s_v[warp] = vref * (1.f / 1024.f);
   __syncthreads();   // the ring is free
   float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      // n-block i, columns 2 t and 2 t + 1: dimensions (D / 8) (2 t + x) + i
-      part[(warp * 16 + g + 8 * e) * D + (D / 8) * (2 * t) + i] = o[i][2 * e];
-      part[(warp * 16 + g + 8 * e) * D + (D / 8) * (2 * t + 1) + i] = o[i][2 * e + 1];
-    }
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < D / 16; i += 2)   // dimensions (D / 8) g + 2 i .. + 3 of row 2 t + e
+        *reinterpret_cast<float4*>(part + (warp * R + 8 * nt + 2 * t + e) * D + (D / 8) * g + 2 * i) =
+            make_float4(o[nt][i][e], o[nt][i][2 + e], o[nt][i + 1][e], o[nt][i + 1][2 + e]);
   __syncthreads();
   for (int i = threadIdx.x; i < valid * D; i += kWarps * 32) {
-    const int r = i / D, w0 = r / 16;   // warps w0, w0 + MW, ... hold row r
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
+    const int r = i / D, w0 = r / R;   // warps w0, w0 + MW, ... hold row r
+    float top = kNone, sum = 0.f, acc = 0.f;
 #pragma unroll
-    for (int x = 0; x < kGroups; ++x) top = fmaxf(top, s_m[w0 + x * MW][r % 16]);
-    const float ref = top == -INFINITY ? 0.f : top;
+    for (int x = 0; x < kGroups; ++x) top = fmaxf(top, s_m[w0 + x * MW][r % R]);
 #pragma unroll
     for (int x = 0; x < kGroups; ++x) {
-      const int ww = w0 + x * MW;
-      const float f = ex2(s_m[ww][r % 16] - ref);
-      sum += f * s_l[ww][r % 16];
-      acc += f * s_v[ww] * part[(ww * 16 + r % 16) * D + i % D];
+      const int w = w0 + x * MW;
+      const float f = ex2(s_m[w][r % R] - top);
+      sum += f * s_l[w][r % R];
+      acc += f * s_v[w] * part[(w * R + r % R) * D + i % D];
     }
-    part[(w0 * 16 + r % 16) * D + i % D] = acc;
+    part[(w0 * R + r % R) * D + i % D] = acc;
     if (i % D == 0) {
       s_top[r] = top;
       s_sum[r] = sum;
     }
   }
-  if (split > 1) cluster_sync_all();
+  if (split > 1) mk::cluster_sync_all();
   else __syncthreads();
   const int nan_any = s_nan;
   // block `rank` finishes every split-th run of 32 elements
   for (int i = threadIdx.x; i < valid * D; i += kWarps * 32) {
     if ((i >> 5) % (int)split != (int)rank) continue;
-    const int r = i / D, d = i % D, idx = ((r / 16) * 16 + r % 16) * D + d;
-    float top = s_top[r], sum = s_sum[r], acc = part[idx];
+    const int r = i / D, d = i % D;
+    float top = s_top[r], sum = s_sum[r], acc = part[i];   // rows of warps 0 .. MW - 1 lie in order
     int bad = nan_any;
     if (split > 1) {
-      top = -INFINITY;
+      top = kNone;
       for (uint32_t k = 0; k < split; ++k) top = fmaxf(top, remote_f32(&s_top[r], k));
-      const float ref = top == -INFINITY ? 0.f : top;
       sum = acc = 0.f;
       for (uint32_t k = 0; k < split; ++k) {
-        const float f = ex2(remote_f32(&s_top[r], k) - ref);
+        const float f = ex2(remote_f32(&s_top[r], k) - top);
         sum += f * remote_f32(&s_sum[r], k);
-        acc += f * remote_f32(&part[idx], k);
+        acc += f * remote_f32(&part[i], k);
         bad |= __float_as_int(remote_f32(reinterpret_cast<const float*>(&s_nan), k));
       }
     }
     float v = sum == 0.f ? 0.f : acc / sum;   // nothing seen: 0
-    int rlo, rhi;
-    sees(m0 + r, rlo, rhi);
     if (bad) {
       // NaN codes of positions that this row sees and another row of the item does not
+      int rlo, rhi;
+      sees(m0 + r, rlo, rhi);
       for (int j = rlo; j < rhi; ++j) {
         if (j >= lo_max + TS && j < hi_min - TS) j = hi_min - TS;   // whole steps kept theirs
         const int id = page_id(c, b, j / P, nullptr);
@@ -522,24 +555,24 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 3 : 2) attend_rows_kern
     store_out(a.out, at * D + d, v, a.bf16);
     if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
   }
-  if (split > 1) cluster_sync_all();   // peers have read this block's shared memory
+  if (split > 1) mk::cluster_sync_all();   // peers have read this block's shared memory
 }
 
 int cache_of(const mk_kv8* m, Cache* c);
 
-template <class F, int P, int D, int MW>
+template <class F, int P, int D, int NT, int MW>
 static int launch_rows(const Cache& c, const Attend& a, cudaStream_t stream) {
   const int group = a.q_heads / c.kv_heads;
-  const long long items = (long long)c.rows * group / (16 * MW) + c.seqs;
+  const long long items = (long long)c.rows * group / (8 * NT * MW) + c.seqs;
   const long long most = (long long)c.table_width * P;
-  // Blocks per item: until the grid fills the GPU three times over, but no
+  // Blocks per item: until the grid fills the GPU ATT_FILL times over, but no
   // more than one step of each group of warps per block at full capacity.
   int split = 1;
-  while (split < 8 && items * c.kv_heads * split < 148 * 3 && most > (long long)split * (kWarps / MW) * (2048 / D)) split *= 2;
+  while (split < 8 && items * c.kv_heads * split < 148 * ATT_FILL && most > (long long)split * (kWarps / MW) * (kStageBytes / 2 / D)) split *= 2;
   const long long blocks = items * c.kv_heads * split;
   if (blocks > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
-  auto kernel = &attend_rows_kernel<F, P, D, MW>;
-  constexpr int bytes = rows_smem<D, MW>();
+  auto kernel = &attend_rows_kernel<F, P, D, NT, MW>;
+  constexpr int bytes = rows_smem<D, NT, MW>();
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return MK_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
@@ -558,9 +591,10 @@ template <class F, int P, int D>
 static int launch(const Cache& c, const Attend& a, cudaStream_t stream) {
   // rows of a sequence, once per query head of the group, on average
   const long long per = ((long long)c.rows * (a.q_heads / c.kv_heads) + c.seqs - 1) / c.seqs;
-  if (per <= 16) return launch_rows<F, P, D, 1>(c, a, stream);
-  if (per <= 32) return launch_rows<F, P, D, 2>(c, a, stream);
-  return launch_rows<F, P, D, 4>(c, a, stream);
+  if (per <= 8) return launch_rows<F, P, D, 1, 1>(c, a, stream);
+  if (per <= 16) return launch_rows<F, P, D, 2, 1>(c, a, stream);
+  if (per <= 32) return launch_rows<F, P, D, 2, 2>(c, a, stream);
+  return launch_rows<F, P, D, 2, 4>(c, a, stream);
 }
 
 }  // namespace mkp
