@@ -257,9 +257,9 @@ int megakernel_tp_info(void* handle, int* rank, int* size);
 int megakernel_tp_exchange_slots(void* handle, float* d_out);
 
 /* ---- paged 8-bit serving operators (no reference counterpart) --------------
- * The parts of a serving step with drafted tokens, each one launch on
- * `stream` (cudaStream_t, NULL = the default stream) of the current device,
- * asynchronous, without allocation; all may be captured into a CUDA graph.
+ * The parts of a serving step with drafted tokens, on `stream` (cudaStream_t,
+ * NULL = the default stream) of the current device, asynchronous, without
+ * allocation; all may be captured into a CUDA graph.
  *
  * Rows are packed over sequences: sequence b owns rows
  * [d_starts[b], d_starts[b + 1]), and its first row stands at position
@@ -331,10 +331,16 @@ int megakernel_kv8_read(const mk_kv8* cache, void* d_k, void* d_v, int type, int
  * j > p - window; len_b = d_kv_lens[b], or the position after the sequence's
  * last row where d_kv_lens is NULL.  d_out [rows][q_heads][head_dim]
  * contiguous; d_lse (may be NULL) [rows][q_heads] = ln sum exp of the scaled
- * scores.  A row that sees nothing gives 0 and -inf. */
+ * scores.  A row that sees nothing gives 0 and -inf.  d_work: 16-byte aligned
+ * scratch of at least megakernel_kv8_attend_workspace(cache, q_heads) bytes
+ * (the same for every call with this page size, head_dim, format, kv_heads,
+ * q_heads and device),
+ * in use until the call has finished on the stream; its contents do not
+ * matter. */
+long long megakernel_kv8_attend_workspace(const mk_kv8* cache, int q_heads);   /* bytes, or MK_ERR_* */
 int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long long q_row, long long q_head, int q_heads,
                           int type, float sm_scale, int causal, int window, const int* d_kv_lens, void* d_out,
-                          float* d_lse, int* d_status, void* stream);
+                          float* d_lse, void* d_work, long long work_bytes, int* d_status, void* stream);
 
 /* Keep or refuse drafted tokens.  Row i of sequence b was fed token
  * d_tokens[starts[b] + i]: row 0 the last confirmed one, the others drafts.

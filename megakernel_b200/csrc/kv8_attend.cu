@@ -1,10 +1,9 @@
 // Attention over the paged 8-bit cache (megakernel_kv8_attend).
+#include <algorithm>
+#include <atomic>
+
 #include "paged.cuh"
 #include "tc_ptx.cuh"
-
-#ifndef ATT_FILL
-#define ATT_FILL 3
-#endif
 
 namespace mkp {
 
@@ -60,21 +59,24 @@ template <> __device__ __forceinline__ void expand<I8>(uint32_t w, uint32_t& lo,
 // Bits 7 of the bytes of w that are e4m3 NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-__device__ __forceinline__ float load_q(const void* q, long long i, bool bf16) {
-  return bf16 ? __bfloat162float(((const __nv_bfloat16*)q)[i]) : __half2float(((const __half*)q)[i]);
+// Eight 16-bit elements as floats, times f.
+__device__ __forceinline__ void load8(const void* q, long long i, bool bf16, float* v) {
+  const uint4 w = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)q + i));
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (bf16) {
+      v[2 * k] = __uint_as_float(ws[k] << 16);
+      v[2 * k + 1] = __uint_as_float(ws[k] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ws[k]));
+      v[2 * k] = f.x;
+      v[2 * k + 1] = f.y;
+    }
+  }
 }
-__device__ __forceinline__ void store_out(void* o, long long i, float v, bool bf16) {
-  if (bf16) ((__nv_bfloat16*)o)[i] = __float2bfloat16_rn(v);
-  else ((__half*)o)[i] = __float2half_rn(v);
-}
-
-// The word at p's place in the shared memory of block `rank` of the cluster.
-__device__ __forceinline__ float remote_f32(const float* p, uint32_t rank) {
-  uint32_t at;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mk::smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi, bool bf16) {
+  return bf16 ? mk::pack_bf16x2(lo, hi) : pack_f16(lo, hi);
 }
 
 __device__ __forceinline__ uint64_t policy_evict_normal() {
@@ -83,9 +85,10 @@ __device__ __forceinline__ uint64_t policy_evict_normal() {
   return pol;
 }
 
-constexpr int kStages = 2;
 constexpr int kWarps = 4;
-constexpr int kStageBytes = 8192;      // K and V codes of one step
+constexpr int kUnits = 3;              // ring of a warp, in units
+constexpr int kUnitBytes = 4096;       // the K or the V codes of one step
+constexpr int kMaxParts = 64;          // warps that may share an item
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr float kNone = -1e30f;        // running reference of a row that has seen nothing
 constexpr float kSlack = 5.f;          // weights may reach 2^kSlack before the reference moves
@@ -97,10 +100,158 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-template <int D, int NT, int MW>
-constexpr int rows_smem() {
-  constexpr int ring = (kWarps / MW) * kStages * kStageBytes, parts = kWarps * 8 * NT * D * 4;
-  return ring > parts ? ring : parts;
+// The same by a whole warp, which leaves it together: the products that follow
+// are .aligned, and a lane's own way out of a loop would not bring it back.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity));
+}
+
+// ---- how the work is cut -------------------------------------------------------------
+//
+// Item: (sequence, tile of R rows counted once per query head of the group, kv
+// head).  All items of a sequence take the same number of steps of TS positions,
+// those that its rows see together.  The steps of all items, in order, are cut
+// into equal runs, one per warp of the grid; a warp with parts of several items
+// takes them one after the other.  Only the first and the last item of a run
+// can be shared with other warps: their parts go to the workspace (slot 2 w for
+// a part that continues an item, 2 w + 1 for one that begins it) and a second
+// small kernel joins them in order.
+struct SeqWork {
+  int r0, n, first, len;   // rows, position of the first, positions held
+  int begin, steps;        // first position and number of the steps, at least one step if there are rows
+  int tiles;
+  int error;               // MK_OK, or what is wrong with the sequence
+};
+
+template <int P, int TS, int R>
+__device__ __forceinline__ SeqWork seq_work(const Cache& c, const Attend& a, int b, int group) {
+  SeqWork w;
+  w.r0 = __ldg(c.starts + b);
+  const int r1 = __ldg(c.starts + b + 1);
+  w.first = __ldg(c.first + b);
+  w.n = r1 - w.r0;
+  w.len = a.kv_lens ? __ldg(a.kv_lens + b) : 0;
+  w.begin = w.steps = w.tiles = 0;
+  w.error = w.r0 < 0 || r1 < w.r0 || r1 > c.rows || w.first > (1 << 30) ? MK_ERR_INVALID_ARG : MK_OK;
+  if (w.error != MK_OK || w.n == 0) {
+    w.n = 0;
+    return w;
+  }
+  if (!a.kv_lens) w.len = w.first + w.n;
+  if (w.len > c.table_width * P) {
+    w.len = c.table_width * P;
+    w.error = MK_ERR_CAPACITY;
+  }
+  const int last = w.first + w.n - 1, low = max(w.first, 0);
+  const int hi = last < 0 ? 0 : a.causal ? min(w.len, last + 1) : w.len;
+  const int lo = a.window ? max(low - a.window + 1, 0) : 0;
+  w.begin = lo / TS * TS;
+  w.steps = hi > w.begin ? (hi - w.begin + TS - 1) / TS : 1;
+  w.tiles = (int)(((long long)w.n * group + R - 1) / R);
+  return w;
+}
+
+struct Total {
+  long long steps;   // of all items
+  int workers;       // warps that share them
+};
+
+__device__ __forceinline__ long long warp_scan(long long v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long other = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += other;
+  }
+  return v;
+}
+
+// Steps of all sequences, by one warp, and how many of `warps` share them: each
+// has at least one step, and the longest item at most kMaxParts + 2 parts.
+template <int P, int TS, int R>
+__device__ __forceinline__ Total total_work(const Cache& c, const Attend& a, int group, int warps, int* status) {
+  long long steps = 0;
+  int longest = 1;
+  for (int b = threadIdx.x & 31; b < c.seqs; b += 32) {
+    const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
+    if (w.error != MK_OK) report(status, w.error);
+    steps += (long long)w.tiles * w.steps;
+    longest = max(longest, w.steps);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    steps += __shfl_xor_sync(0xffffffffu, steps, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  steps *= c.kv_heads;
+  return {steps, (int)min((long long)warps, max(steps * min(kMaxParts, longest) / longest, 1LL))};
+}
+
+// The sequence that step (or, with by_item, item) number x falls into, and the
+// number of its first one.  x is less than the total.
+template <int P, int TS, int R>
+__device__ __forceinline__ int seq_at(const Cache& c, const Attend& a, int group, long long x, bool by_item, long long* base) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int b0 = 0; b0 < c.seqs; b0 += 32) {
+    long long mine = 0;
+    if (b0 + lane < c.seqs) {
+      const SeqWork w = seq_work<P, TS, R>(c, a, b0 + lane, group);
+      mine = (long long)w.tiles * (by_item ? 1 : w.steps) * c.kv_heads;
+    }
+    const long long upto = warp_scan(mine) + before;
+    const unsigned hit = __ballot_sync(0xffffffffu, x < upto);
+    if (hit) {
+      const int k = __ffs(hit) - 1;
+      *base = __shfl_sync(0xffffffffu, upto - mine, k);
+      return b0 + k;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  *base = before;
+  return -1;
+}
+
+// Run of worker w: [run_begin(w), run_begin(w + 1)); the worker whose run holds step x.
+__device__ __forceinline__ long long run_begin(const Total& t, int w) { return t.steps / t.workers * w + t.steps % t.workers * w / t.workers; }
+__device__ __forceinline__ int worker_of(const Total& t, long long x) {
+  int w = (int)min((double)t.workers - 1, (double)x / (double)t.steps * t.workers);
+  while (run_begin(t, w) > x) --w;
+  while (w + 1 < t.workers && run_begin(t, w + 1) <= x) ++w;
+  return w;
+}
+
+// A part in the workspace: R x D sums, then m and l of each row, then whether a NaN was taken out.
+template <int D, int R>
+__host__ __device__ constexpr int part_floats() { return R * D + 2 * R + 4; }
+
+// What row index m of a sequence sees: [lo, hi).
+__device__ __forceinline__ void row_sees(const SeqWork& w, const Attend& a, int group, int m, int& lo, int& hi) {
+  const int pos = w.first + m / group;
+  lo = hi = 0;
+  if (m < w.n * group && pos >= 0) {
+    hi = max(a.causal ? min(w.len, pos + 1) : w.len, 0);
+    lo = a.window ? max(pos - a.window + 1, 0) : 0;
+  }
+}
+
+// Whether a position that row index m sees holds a NaN code in dimension d of V.  Only
+// positions of steps that some row of the tile does not see wholly are looked at.
+template <class F, int P, int TS, int D>
+__device__ __noinline__ bool sees_nan(const Cache& c, const Attend& a, const SeqWork& w, int b, int h, int group, int tile_first,
+                                      int tile_last, int m, int d) {
+  if (F::kTopExp != 8) return false;
+  int lo, hi, lo_max, hi_min, x;
+  row_sees(w, a, group, m, lo, hi);
+  row_sees(w, a, group, tile_last, lo_max, x);
+  row_sees(w, a, group, tile_first, x, hi_min);
+  for (int j = lo; j < hi; ++j) {
+    if (j >= lo_max + TS && j < hi_min - TS) j = hi_min - TS;
+    const int id = page_id(c, b, j / P, nullptr);
+    if (id < 0) continue;
+    const uint8_t code = c.codes[id * c.page_stride + ((long long)(c.kv_heads + h) * P + j % P) * D + d];
+    if ((code & 127) == 127) return true;
+  }
+  return false;
 }
 
 // 8 x 8 f16 matrix, lane (g, t) holding row g, columns 2 t and 2 t + 1 -> its transpose.
@@ -112,17 +263,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 // ---- attention of few rows per sequence -------------------------------------------------
 //
-// Work item: (8 NT MW rows of one sequence and kv head, counting a row once per
-// query head of the group; the positions split over the S blocks of a cluster
-// and their warps).  MW warps that hold 8 NT rows each share a stream of steps
-// of TS positions; the 4 / MW such groups of a block, and the blocks of the
-// cluster, take every (4 / MW) S-th step.
-//
-// The codes of a step, contiguous in a page, arrive by bulk copies in a ring
-// per group (K 4 KB and V 4 KB a stage): nothing of the stream passes through
-// registers before it is used.  Both products have the positions or the head
-// dimension as the 16 rows of an m16n8k16 f16 product and the query rows as
-// its 8 columns, fp32 accumulation:
+// Every warp works by itself.  The codes of a step, contiguous in a page, arrive
+// by bulk copies in a ring of three units of 4 KB (the K or the V codes of a
+// step): nothing of the stream passes through registers before it is used.
+// Both products have the positions or the head dimension as the 16 rows of an
+// m16n8k16 f16 product and the query rows as its 8 columns, fp32 accumulation:
 //   S^T [positions x rows] = K Q^T,   O^T [dims x rows] += V^T P^T,
 // so that 8 rows (a decode step of 8 query heads per kv head) waste nothing.
 // The order of the head dimension in the first product and of the output's
@@ -134,208 +279,201 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 //
 // Softmax per row relative to a running reference m: p = 2^(s - m), l = sum p,
 // fp32.  m moves to the maximum only when some p would pass 2^5 (one vote per
-// 32 positions), so most steps have no exchange between lanes at all.  The
-// scale of a K page multiplies the scores, that of a V page the weights:
+// step), so most steps have no exchange between lanes at all.  The scale of a
+// K page multiplies the scores, that of a V page the weights:
 // w = 2^10 p scale / vref, vref the largest V scale so far, goes into the second
 // product in f16: 11 bits down to 2^-29 of the row's largest, an absolute 2^-35
 // below that (at p scale / vref alone it was 2^-25, which rows with one
 // dominant position showed).  The sum l takes the unrounded p.
-template <class F, int P, int D, int NT, int MW>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 || NT == 1 ? 3 : 2) attend_rows_kernel(const Cache c, const Attend a) {
-  constexpr int TS = kStageBytes / 2 / D, kSub = TS > P ? TS / P : 1, kGroups = kWarps / MW;
+template <class F, int P, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2))
+attend_rows_kernel(const Cache c, const Attend a, float* work) {
+  constexpr int TS = kUnitBytes / D, kSub = TS > P ? TS / P : 1;
   constexpr int kSubRows = TS / kSub;               // positions of a step in one page
   constexpr int kBatch = 32 / kSub;                 // steps whose pages the lanes hold
-  constexpr int R = 8 * NT;                         // rows of a warp
+  constexpr int R = 8 * NT, MT = TS / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t s_full[kGroups * kStages], s_empty[kGroups * kStages];
-  __shared__ float s_m[kWarps][R], s_l[kWarps][R], s_v[kWarps], s_top[MW * R], s_sum[MW * R];
-  __shared__ int s_nan;
+  __shared__ __align__(8) uint64_t s_full[kWarps][kUnits];
+  mk::pdl_launch();   // the joining kernel may take its place; it waits for this one's end
 
-  uint32_t rank, split;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int mw = warp % MW, grp = warp / MW;
   const int group = a.q_heads / c.kv_heads;
-  const int cta = blockIdx.x / split, h = cta % c.kv_heads, item = cta / c.kv_heads;
-
-  // sequence b owns the items from starts[b] group / (R MW) + b on
-  auto key = [&](int i) { return (int)((long long)__ldg(c.starts + i) * group / (R * MW)) + i; };
-  const int b = warp_search(c.seqs, item, key);
-  const int r0 = __ldg(c.starts + b), r1 = __ldg(c.starts + b + 1), first = __ldg(c.first + b);
-  if (r0 < 0 || r1 < r0 || r1 > c.rows || first > (1 << 30)) {
-    report(a.status, MK_ERR_INVALID_ARG);
-    return;   // the whole cluster: every block of it has this item
-  }
-  const int n = r1 - r0, m0 = (item - key(b)) * R * MW;
-  if (m0 < 0 || m0 >= n * group) return;
-  const int valid = min(n * group - m0, R * MW);
-  int len = a.kv_lens ? __ldg(a.kv_lens + b) : first + n;
-  if (len > c.table_width * P) {
-    report(a.status, MK_ERR_CAPACITY);
-    len = c.table_width * P;
-  }
-  // what the row of index m sees: [lo, hi)
-  auto sees = [&](int m, int& lo, int& hi) {
-    const int pos = first + m / group;
-    lo = hi = 0;
-    if (m < n * group && pos >= 0) {
-      hi = max(a.causal ? min(len, pos + 1) : len, 0);
-      lo = a.window ? max(pos - a.window + 1, 0) : 0;
-    }
-  };
-  int lo_all, hi_all, lo_max, hi_min;
-  sees(m0 + valid - 1, lo_max, hi_all);
-  sees(m0, lo_all, hi_min);
-  const int begin = lo_all / TS * TS;
-  const int all_steps = hi_all > begin ? (hi_all - begin + TS - 1) / TS : 0;
-  const int stride = (int)split * kGroups, my = (int)rank * kGroups + grp;
-  const int steps = all_steps > my ? (all_steps - my - 1) / stride + 1 : 0;
-
-  if (threadIdx.x == 0) {
-    s_nan = 0;
-    for (int i = 0; i < kGroups * kStages; ++i) {
-      mk::mbar_init(&s_full[i], kSub);
-      mk::mbar_init(&s_empty[i], MW);
-    }
+  uint8_t* ring = smem + warp * kUnits * kUnitBytes;
+  uint64_t* full = s_full[warp];
+  if (lane == 0) {
+    for (int i = 0; i < kUnits; ++i) mk::mbar_init(&full[i], kSub);
     mk::fence_mbar_init();
   }
-  __syncthreads();
+  __syncwarp();
 
-  // Pages of kBatch steps, one per lane: id (-1: not wanted, or reported) and
-  // scales (a K scale of 0 marks a page that is not there).
-  struct Page { int id; float ks, vs; };
-  auto pages_from = [&](int step) {
-    Page p{-1, 0.f, 0.f};
-    const int st = step + lane / kSub;
-    const int pos = begin + (st * stride + my) * TS + (lane % kSub) * kSubRows;
-    if (st < steps && pos < hi_all && pos + kSubRows > lo_all) {
-      p.id = page_id(c, b, pos / P, a.status);
-      if (p.id >= 0) {
-        const float* sc = c.scales + p.id * c.scale_stride + h;
-        p.ks = fmaxf(__ldg(sc), 1.17549435e-38f);
-        p.vs = __ldg(sc + c.kv_heads);
+  const Total all = total_work<P, TS, R>(c, a, group, (int)gridDim.x * kWarps, blockIdx.x == 0 && warp == 0 ? a.status : nullptr);
+  const int worker = warp * (int)gridDim.x + (int)blockIdx.x;   // neighbours on different SMs
+  if (worker >= all.workers || all.steps == 0) return;
+  long long at = run_begin(all, worker);
+  const long long end = run_begin(all, worker + 1);
+  if (at >= end) return;
+  long long seq_base;
+  int b = seq_at<P, TS, R>(c, a, group, at, false, &seq_base);
+  int slot = 0;
+  uint32_t phase = 0;   // of ring slot `slot`; slots are used in turn over all items
+
+  for (; at < end; ) {
+    const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
+    const long long size = (long long)w.tiles * c.kv_heads * w.steps;
+    if (at >= seq_base + size) {   // also sequences without rows
+      seq_base += size;
+      ++b;
+      continue;
+    }
+    const int item = (int)((at - seq_base) / w.steps);
+    const long long item_base = seq_base + (long long)item * w.steps;
+    const int h = item % c.kv_heads, tile_first = item / c.kv_heads * R, tile_last = min(tile_first + R, w.n * group) - 1;
+    const int s0 = (int)(at - item_base), s1 = (int)min((long long)w.steps, s0 + (end - at));
+    at += s1 - s0;
+    // steps of the part that some row of the tile sees
+    int lo_all, hi_all, lo_max, hi_min;
+    row_sees(w, a, group, tile_last, lo_max, hi_all);
+    row_sees(w, a, group, tile_first, lo_all, hi_min);
+    const int sb = max(s0, lo_all > w.begin ? (lo_all - w.begin) / TS : 0);
+    const int steps = min(s1, hi_all > w.begin ? (hi_all - w.begin + TS - 1) / TS : 0) - sb;
+
+    // Pages of kBatch steps, one per lane: id (-1: not wanted, or reported) and
+    // scales (a K scale of 0 marks a page that is not there).
+    struct Page { int id; float ks, vs; };
+    auto pages_from = [&](int i) {
+      Page p{-1, 0.f, 0.f};
+      i += lane / kSub;
+      const int pos = w.begin + (sb + i) * TS + (lane % kSub) * kSubRows;
+      if (i < steps && pos < hi_all && pos + kSubRows > lo_all) {
+        p.id = page_id(c, b, pos / P, a.status);
+        if (p.id >= 0) {
+          const float* sc = c.scales + p.id * c.scale_stride + h;
+          p.ks = fmaxf(__ldg(sc), 1.17549435e-38f);
+          p.vs = __ldg(sc + c.kv_heads);
+        }
+      }
+      return p;
+    };
+    Page cur = pages_from(0), nxt = pages_from(kBatch);
+    int base = 0;
+    // Codes that no other item reads do not stay in the L2 cache.
+    const uint64_t policy = w.tiles == 1 ? mk::policy_evict_first() : policy_evict_normal();
+    int put = slot;   // slot of the next unit to fetch
+    // Unit u: the K (even) or V codes of step u / 2; the lanes that hold the
+    // step's pages copy their part of it.
+    auto fetch = [&](int u) {
+      const int i = u >> 1;
+      if (i >= steps) return;
+      const int id = i - base < kBatch ? cur.id : nxt.id;
+      if (lane / kSub == (i - base) % kBatch) {
+        const int sub = lane % kSub;
+        mk::mbar_arrive_expect_tx(&full[put], id >= 0 ? kSubRows * D : 0);
+        if (id >= 0) {
+          const int pos = w.begin + (sb + i) * TS + sub * kSubRows;
+          const uint8_t* src = c.codes + id * c.page_stride + ((long long)((u & 1) * c.kv_heads + h) * P + pos % P) * D;
+          mk::bulk_g2s(ring + put * kUnitBytes + sub * kSubRows * D, src, kSubRows * D, &full[put], policy);
+        }
+      }
+      put = put + 1 == kUnits ? 0 : put + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) fetch(i);
+
+    // q fragments, row 8 nt + g: k-step j holds dimensions 64 (j / 4) + 16 t +
+    // 4 (j % 4) + {0, 1 | 2, 3}.  rq, lo, hi: rows 2 t and 2 t + 1, whose scores
+    // this lane will hold.
+    uint32_t q[NT][D / 16][2];
+    float rq[NT][2];
+    int lo[NT][2], hi[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int m = tile_first + 8 * nt + g;
+      const bool real = m <= tile_last;
+      const long long src = real ? (long long)(w.r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head + 16 * t : 0;
+      float v[D / 4];
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        if (real) {
+          load8(a.q, src + i / 2 * 64 + i % 2 * 8, a.bf16, v + 8 * i);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[8 * i + x] = 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(v[8 * i + x]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // power of two that brings the largest to [2^14, 2^15)
+      const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);
+      const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        q[nt][j][0] = pack_f16(v[4 * j] * up, v[4 * j + 1] * up);
+        q[nt][j][1] = pack_f16(v[4 * j + 2] * up, v[4 * j + 3] * up);
+      }
+      const float back = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rq[nt][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
+        row_sees(w, a, group, tile_first + 8 * nt + 2 * t + e, lo[nt][e], hi[nt][e]);
       }
     }
-    return p;
-  };
-  Page cur = pages_from(0), nxt = pages_from(kBatch);
-  int base = 0;
-  uint8_t* ring = smem + grp * kStages * kStageBytes;
-  // Codes that no other item reads do not stay in the L2 cache.
-  const uint64_t policy = n * group <= R * MW ? mk::policy_evict_first() : policy_evict_normal();
-  // The lanes that hold the pages of step st copy their part of it.
-  auto fetch = [&](int st) {
-    const int id = st - base < kBatch ? cur.id : nxt.id;
-    if (st < steps && lane / kSub == (st - base) % kBatch) {
-      uint64_t* bar = &s_full[grp * kStages + st % kStages];
-      const int sub = lane % kSub;
-      mk::mbar_arrive_expect_tx(bar, id >= 0 ? 2 * kSubRows * D : 0);
-      if (id >= 0) {
-        const int pos = begin + (st * stride + my) * TS + sub * kSubRows;
-        uint8_t* dst = ring + st % kStages * kStageBytes + sub * kSubRows * D;
-        const uint8_t* k = c.codes + id * c.page_stride + ((long long)h * P + pos % P) * D;
-        mk::bulk_g2s(dst, k, kSubRows * D, bar, policy);
-        mk::bulk_g2s(dst + TS * D, k + (long long)c.kv_heads * P * D, kSubRows * D, bar, policy);
+
+    float o[NT][D / 16][4] = {};
+    float m[NT][2], l[NT][2], vref = 0.f, iv = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[nt][e] = kNone, l[nt][e] = 0.f;
+    int nan_seen = 0;
+    bool alive = true;
+    for (int i = 0; i < steps; ++i) {
+      if (i - base == kBatch) {
+        base += kBatch;
+        cur = nxt;
+        nxt = pages_from(base + kBatch);
       }
-    }
-  };
-  if (mw == 0)
-    for (int i = 0; i < kStages; ++i) fetch(i);
+      float ks[kSub], vs[kSub];
+      float vmax = vref;
+      bool whole = true;
+#pragma unroll
+      for (int x = 0; x < kSub; ++x) {
+        ks[x] = __shfl_sync(0xffffffffu, cur.ks, (i - base) * kSub + x);
+        vs[x] = __shfl_sync(0xffffffffu, cur.vs, (i - base) * kSub + x);
+        whole = whole && ks[x] > 0.f;
+        vmax = fmaxf(vmax, vs[x]);
+      }
+      if (vmax > vref) {
+        const float r = vref / vmax;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int y = 0; y < D / 16; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[nt][y][x] *= r;
+        vref = vmax;
+        iv = 1024.f / vmax;
+      }
+      const int pos = w.begin + (sb + i) * TS;
+      whole = whole && pos >= lo_max && pos + TS <= hi_min;
 
-  // q fragments, row 8 nt + g of this warp: k-step j holds dimensions
-  // 64 (j / 4) + 16 t + 4 (j % 4) + {0, 1 | 2, 3}.  rq, lo, hi: rows 2 t and
-  // 2 t + 1, whose scores this lane will hold.
-  uint32_t q[NT][D / 16][2];
-  float rq[NT][2];
-  int lo[NT][2], hi[NT][2];
+      // ---- scores
+      if (!warp_wait(&full[slot], phase)) {
+        alive = false;
+        break;
+      }
+      float s[MT][NT][4];
+      const uint8_t* kb = ring + slot * kUnitBytes + g * D + 16 * t;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int m = m0 + mw * R + 8 * nt + g;
-    const bool real = m < n * group;
-    const long long at = real ? (long long)(r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head : 0;
-    float v[D / 4];
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      v[i] = real ? load_q(a.q, at + i / 16 * 64 + 16 * t + i % 16, a.bf16) : 0.f;
-      top = fmaxf(top, fabsf(v[i]));
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // power of two that brings the largest to [2^14, 2^15)
-    const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);
-    const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      q[nt][j][0] = pack_f16(v[4 * j] * up, v[4 * j + 1] * up);
-      q[nt][j][1] = pack_f16(v[4 * j + 2] * up, v[4 * j + 3] * up);
-    }
-    const float back = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      rq[nt][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
-      sees(m0 + mw * R + 8 * nt + 2 * t + e, lo[nt][e], hi[nt][e]);
-    }
-  }
-
-  float o[NT][D / 16][4] = {};
-  float m[NT][2], l[NT][2], vref = 0.f, iv = 0.f;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-    for (int e = 0; e < 2; ++e) m[nt][e] = kNone, l[nt][e] = 0.f;
-  bool alive = true;
-  int nan_seen = 0, failed = 0;
-  for (int st = 0; st < steps; ++st) {
-    if (st - base == kBatch) {
-      base += kBatch;
-      cur = nxt;
-      nxt = pages_from(base + kBatch);
-    }
-    float ks[kSub], vs[kSub];
-    float vmax = vref;
-    bool whole = true;
-#pragma unroll
-    for (int i = 0; i < kSub; ++i) {
-      const int src = (st - base) * kSub + i;
-      ks[i] = __shfl_sync(0xffffffffu, cur.ks, src);
-      vs[i] = __shfl_sync(0xffffffffu, cur.vs, src);
-      whole = whole && ks[i] > 0.f;
-      vmax = fmaxf(vmax, vs[i]);
-    }
-    if (vmax > vref) {
-      const float r = vref / vmax;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) o[nt][i][x] *= r;
-      vref = vmax;
-      iv = 1024.f / vmax;
-    }
-    const int pos = begin + (st * stride + my) * TS;
-    whole = whole && pos >= lo_max && pos + TS <= hi_min;
-    if (!wait_bar(&s_full[grp * kStages + st % kStages], (st / kStages) & 1)) {
-      alive = false;
-      failed = st;
-      break;
-    }
-    const uint8_t* kb = ring + st % kStages * kStageBytes;
-    const uint8_t* vb = kb + TS * D;
-
-#pragma unroll
-    for (int half = 0; half < TS / 32; ++half) {   // 32 positions
-      float s[2][NT][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const uint8_t* k0 = kb + (half * 32 + mt * 16 + g) * D + 16 * t;
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
 #pragma unroll
         for (int d = 0; d < D / 64; ++d) {
-          const uint4 x = *reinterpret_cast<const uint4*>(k0 + d * 64);
-          const uint4 y = *reinterpret_cast<const uint4*>(k0 + d * 64 + 8 * D);
+          const uint4 x = *reinterpret_cast<const uint4*>(kb + mt * 16 * D + d * 64);
+          const uint4 y = *reinterpret_cast<const uint4*>(kb + mt * 16 * D + 8 * D + d * 64);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -347,25 +485,32 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 || NT == 1 ? 3 : 2) atten
           }
         }
       }
-      float f[2][NT][2];
+      __syncwarp();
+      if (++slot == kUnits) slot = 0, phase ^= 1;
+      fetch(2 * i + kUnits);
+
+      // ---- weights
+      float f[kSub][NT][2];
       bool over = false;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int i = (half * 32 + mt * 16) / kSubRows;
+      for (int x = 0; x < kSub; ++x)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) f[mt][nt][e] = fmaxf(rq[nt][e] * ks[i], 1.17549435e-38f);   // -inf x 0 would be NaN
-          if (!whole) {
+          for (int e = 0; e < 2; ++e) f[x][nt][e] = fmaxf(rq[nt][e] * ks[x], 1.17549435e-38f);   // -inf x 0 would be NaN
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int j = pos + half * 32 + mt * 16 + g + 8 * (x >> 1);
-              if (ks[i] == 0.f || j < lo[nt][x & 1] || j >= hi[nt][x & 1]) s[mt][nt][x] = -INFINITY;
+      for (int mt = 0; mt < MT; ++mt) {
+        const int sub = mt * 16 / kSubRows;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (!whole) {
+              const int j = pos + mt * 16 + g + 8 * (x >> 1);
+              if (ks[sub] == 0.f || j < lo[nt][x & 1] || j >= hi[nt][x & 1]) s[mt][nt][x] = -INFINITY;
             }
+            over = over || fmaf(s[mt][nt][x], f[sub][nt][x & 1], -m[nt][x & 1]) > kSlack;
           }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) over = over || fmaf(s[mt][nt][x], f[mt][nt][x & 1], -m[nt][x & 1]) > kSlack;
-        }
       }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -374,8 +519,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 || NT == 1 ? 3 : 2) atten
           for (int e = 0; e < 2; ++e) {
             float top = m[nt][e];
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-              top = fmaxf(top, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]) * f[mt][nt][e]);
+            for (int mt = 0; mt < MT; ++mt)
+              top = fmaxf(top, fmaxf(s[mt][nt][e], s[mt][nt][2 + e]) * f[mt * 16 / kSubRows][nt][e]);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -383,44 +528,54 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 || NT == 1 ? 3 : 2) atten
             m[nt][e] = top;
             l[nt][e] *= keep;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              o[nt][i][e] *= keep;
-              o[nt][i][2 + e] *= keep;
+            for (int y = 0; y < D / 16; ++y) {
+              o[nt][y][e] *= keep;
+              o[nt][y][2 + e] *= keep;
             }
           }
       }
+      uint32_t pb[MT][NT][2];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int at = half * 32 + mt * 16, i = at / kSubRows;
-        const float rv = vs[i] * iv;
-        uint32_t pb[NT][2];
+      for (int mt = 0; mt < MT; ++mt) {
+        const int sub = mt * 16 / kSubRows;
+        const float rv = vs[sub] * iv;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float p[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            p[x] = ex2(fmaf(s[mt][nt][x], f[mt][nt][x & 1], -m[nt][x & 1]));
+            p[x] = ex2(fmaf(s[mt][nt][x], f[sub][nt][x & 1], -m[nt][x & 1]));
             l[nt][x & 1] += p[x];
           }
-          pb[nt][0] = transpose8(pack_f16(p[0] * rv, p[1] * rv));
-          pb[nt][1] = transpose8(pack_f16(p[2] * rv, p[3] * rv));
+          pb[mt][nt][0] = transpose8(pack_f16(p[0] * rv, p[1] * rv));
+          pb[mt][nt][1] = transpose8(pack_f16(p[2] * rv, p[3] * rv));
         }
+      }
+
+      // ---- output
+      if (!warp_wait(&full[slot], phase)) {
+        alive = false;
+        break;
+      }
+      const uint8_t* vb = ring + slot * kUnitBytes + 2 * t * D + g * (D / 8);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
         uint32_t v[4][D / 32];   // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int row = at + 2 * t + (x & 1) + 8 * (x >> 1);
-          const uint8_t* vp = vb + row * D + g * (D / 8);
+          const int row = mt * 16 + (x & 1) + 8 * (x >> 1);
           if constexpr (D == 64) {
-            const uint2 u = *reinterpret_cast<const uint2*>(vp);
+            const uint2 u = *reinterpret_cast<const uint2*>(vb + row * D);
             v[x][0] = u.x; v[x][1] = u.y;
           } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(vp);
+            const uint4 u = *reinterpret_cast<const uint4*>(vb + row * D);
             v[x][0] = u.x; v[x][1] = u.y; v[x][2] = u.z; v[x][3] = u.w;
           }
           if (!whole) {
             // What no row sees may hold anything: its codes count as 0.  A NaN
             // that only some rows see is taken out here and put back at the end.
-            const bool dead = ks[i] == 0.f || pos + row >= hi_all || pos + row < lo_all;
+            const int j = pos + 2 * t + row;
+            const bool dead = ks[mt * 16 / kSubRows] == 0.f || j >= hi_all || j < lo_all;
 #pragma unroll
             for (int y = 0; y < D / 32; ++y) {
               if (dead) v[x][y] = 0;
@@ -444,172 +599,227 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 || NT == 1 ? 3 : 2) atten
           expand<F>(__byte_perm(v[2][y], v[3][y], 0x7362), vc[2], vc[3]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(o[nt][2 * y], va, pb[nt][0], pb[nt][1]);
-            mma_f16(o[nt][2 * y + 1], vc, pb[nt][0], pb[nt][1]);
+            mma_f16(o[nt][2 * y], va, pb[mt][nt][0], pb[mt][nt][1]);
+            mma_f16(o[nt][2 * y + 1], vc, pb[mt][nt][0], pb[mt][nt][1]);
           }
         }
       }
+      __syncwarp();
+      if (++slot == kUnits) slot = 0, phase ^= 1;
+      fetch(2 * i + 1 + kUnits);
     }
-    __syncwarp();
-    if constexpr (MW > 1) {
-      if (lane == 0) mk::mbar_arrive(&s_empty[grp * kStages + st % kStages]);
-      if (mw == 0) {
-        if (st + kStages < steps && !wait_bar(&s_empty[grp * kStages + st % kStages], (st / kStages) & 1)) {
-          alive = false;
-          failed = st + 1;
-          break;
-        }
-        fetch(st + kStages);
+    if (!alive) {
+      // Waits are bounded; a copy that never lands is reported, and none is left
+      // in flight unwaited: the block's shared memory is given away at its end.
+      if (lane == 0) report(a.status, MK_ERR_TIMEOUT);
+      for (int i = 0; i < kUnits; ++i) {
+        wait_bar(&full[slot], phase);
+        if (++slot == kUnits) slot = 0, phase ^= 1;
       }
-    } else {
-      fetch(st + kStages);
+      return;
     }
-  }
-  if (!alive) {
-    // Leave no copy in flight: the block's shared memory is given away at its
-    // end.  (Waits are bounded; a copy that never lands is reported.)
-    report(a.status, MK_ERR_TIMEOUT);
-    for (int i = 0; i < kStages; ++i)
-      if (failed + i < steps) wait_bar(&s_full[grp * kStages + (failed + i) % kStages], ((failed + i) / kStages) & 1);
-  }
-  if (nan_seen) s_nan = 1;
+    nan_seen = __any_sync(0xffffffffu, nan_seen);
 
-  // ---- join the warps, then the blocks of the cluster
+    // ---- rows 2 t and 2 t + 1, dimensions (D / 8) g .. of the item, or its part
+    const bool is_part = s0 > 0 || s1 < w.steps;
+    float* part = work + (long long)(2 * worker + (s0 > 0 ? 0 : 1)) * part_floats<D, R>();
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float x = l[nt][e];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) {
-        s_m[warp][8 * nt + 2 * t + e] = m[nt][e];
-        s_l[warp][8 * nt + 2 * t + e] = x;
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int r = 8 * nt + 2 * t + e, mm = tile_first + r;
+        if (mm > tile_last) continue;
+        if (is_part) {
+          const float k = vref * (1.f / 1024.f);
+#pragma unroll
+          for (int y = 0; y < D / 16; y += 2)
+            *reinterpret_cast<float4*>(part + r * D + (D / 8) * g + 2 * y) =
+                make_float4(o[nt][y][e] * k, o[nt][y][2 + e] * k, o[nt][y + 1][e] * k, o[nt][y + 1][2 + e] * k);
+          if (g == 0) {
+            part[R * D + r] = m[nt][e];
+            part[R * D + R + r] = sum;
+            if (r == 0) part[R * D + 2 * R] = __int_as_float(nan_seen);
+          }
+          continue;
+        }
+        const float k = sum == 0.f ? 0.f : vref * (1.f / 1024.f) / sum;   // nothing seen: 0
+        const long long row = (long long)(w.r0 + mm / group) * a.q_heads + h * group + mm % group;
+        float v[D / 8];
+#pragma unroll
+        for (int y = 0; y < D / 8; ++y) v[y] = o[nt][y / 2][2 * (y & 1) + e] * k;
+        if (nan_seen) {
+          for (int y = 0; y < D / 8; ++y)
+            if (sees_nan<F, P, TS, D>(c, a, w, b, h, group, tile_first, tile_last, mm, (D / 8) * g + y)) v[y] = __int_as_float(0x7fffffff);
+        }
+        uint4* out = reinterpret_cast<uint4*>((uint16_t*)a.out + row * D + (D / 8) * g);
+#pragma unroll
+        for (int y = 0; y < D / 64; ++y)
+          out[y] = make_uint4(pack_out(v[8 * y], v[8 * y + 1], a.bf16), pack_out(v[8 * y + 2], v[8 * y + 3], a.bf16),
+                              pack_out(v[8 * y + 4], v[8 * y + 5], a.bf16), pack_out(v[8 * y + 6], v[8 * y + 7], a.bf16));
+        if (a.lse && g == 0) a.lse[row] = sum == 0.f ? -INFINITY : (m[nt][e] + log2f(sum)) * 0.6931471805599453f;
       }
-    }
-  if (lane == 0) s_v[warp] = vref * (1.f / 1024.f);
-  __syncthreads();   // the ring is free
-  float* part = reinterpret_cast<float*>(smem);
+  }
+}
+
+// Joins the parts of an item that several warps shared, in their order.
+constexpr int kJoinThreads = 256;
+template <class F, int P, int D, int NT>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const Cache c, const Attend a, const float* work, int warps) {
+  constexpr int TS = kUnitBytes / D, R = 8 * NT, kFloats = part_floats<D, R>();
+  __shared__ float s_f[R][kMaxParts + 2], s_top[R], s_sum[R];
+  __shared__ int s_nan;
+  const int group = a.q_heads / c.kv_heads, tid = threadIdx.x;
+  const Total all = total_work<P, TS, R>(c, a, group, warps, nullptr);
+  long long item_base;
+  const int b = seq_at<P, TS, R>(c, a, group, blockIdx.x, true, &item_base);
+  if (b < 0) {   // a spare block
+    mk::pdl_wait();
+    return;
+  }
+  const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
+  const int item = (int)(blockIdx.x - item_base), h = item % c.kv_heads;
+  const int tile_first = item / c.kv_heads * R, tile_last = min(tile_first + R, w.n * group) - 1;
+  // the number of the sequence's first step: as seq_at, over the steps
+  long long step = 0;
+  for (int i = tid & 31; i < b; i += 32) {
+    const SeqWork x = seq_work<P, TS, R>(c, a, i, group);
+    step += (long long)x.tiles * x.steps;
+  }
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int i = 0; i < D / 16; i += 2)   // dimensions (D / 8) g + 2 i .. + 3 of row 2 t + e
-        *reinterpret_cast<float4*>(part + (warp * R + 8 * nt + 2 * t + e) * D + (D / 8) * g + 2 * i) =
-            make_float4(o[nt][i][e], o[nt][i][2 + e], o[nt][i + 1][e], o[nt][i + 1][2 + e]);
+  for (int o = 16; o > 0; o >>= 1) step += __shfl_xor_sync(0xffffffffu, step, o);
+  step = step * c.kv_heads + (long long)item * w.steps;
+  const int w0 = worker_of(all, step), w1 = worker_of(all, step + w.steps - 1);
+  const int parts = min(w1 - w0 + 1, kMaxParts + 2);   // never more, see total_work
+  if (tid == 0) s_nan = 0;
+  mk::pdl_wait();   // every block: the end of this kernel stands for the end of both
+  if (parts == 1) return;   // written whole
   __syncthreads();
-  for (int i = threadIdx.x; i < valid * D; i += kWarps * 32) {
-    const int r = i / D, w0 = r / R;   // warps w0, w0 + MW, ... hold row r
-    float top = kNone, sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int x = 0; x < kGroups; ++x) top = fmaxf(top, s_m[w0 + x * MW][r % R]);
-#pragma unroll
-    for (int x = 0; x < kGroups; ++x) {
-      const int w = w0 + x * MW;
-      const float f = ex2(s_m[w][r % R] - top);
-      sum += f * s_l[w][r % R];
-      acc += f * s_v[w] * part[(w * R + r % R) * D + i % D];
+  auto part_of = [&](int x) { return work + (long long)(2 * (w0 + x) + (x == 0 ? 1 : 0)) * kFloats; };
+  const int rows = tile_last - tile_first + 1;
+  for (int i = tid; i < rows * parts; i += kJoinThreads) s_f[i % rows][i / rows] = part_of(i / rows)[R * D + i % rows];
+  for (int i = tid; i < parts; i += kJoinThreads)
+    if (__float_as_int(part_of(i)[R * D + 2 * R])) s_nan = 1;
+  __syncthreads();
+  // one warp per row: maximum, factors, sum
+  for (int r = tid >> 5; r < rows; r += kJoinThreads / 32) {
+    float top = kNone, sum = 0.f;
+    for (int i = tid & 31; i < parts; i += 32) top = fmaxf(top, s_f[r][i]);
+    top = mk::warp_max(top);
+    for (int i = tid & 31; i < parts; i += 32) {
+      const float f = ex2(s_f[r][i] - top);
+      s_f[r][i] = f;
+      sum += f * part_of(i)[R * D + R + r];
     }
-    part[(w0 * R + r % R) * D + i % D] = acc;
-    if (i % D == 0) {
-      s_top[r] = top;
-      s_sum[r] = sum;
-    }
+    sum = mk::warp_sum(sum);
+    if ((tid & 31) == 0) s_top[r] = top, s_sum[r] = sum;
   }
-  if (split > 1) mk::cluster_sync_all();
-  else __syncthreads();
-  const int nan_any = s_nan;
-  // block `rank` finishes every split-th run of 32 elements
-  for (int i = threadIdx.x; i < valid * D; i += kWarps * 32) {
-    if ((i >> 5) % (int)split != (int)rank) continue;
-    const int r = i / D, d = i % D;
-    float top = s_top[r], sum = s_sum[r], acc = part[i];   // rows of warps 0 .. MW - 1 lie in order
-    int bad = nan_any;
-    if (split > 1) {
-      top = kNone;
-      for (uint32_t k = 0; k < split; ++k) top = fmaxf(top, remote_f32(&s_top[r], k));
-      sum = acc = 0.f;
-      for (uint32_t k = 0; k < split; ++k) {
-        const float f = ex2(remote_f32(&s_top[r], k) - top);
-        sum += f * remote_f32(&s_sum[r], k);
-        acc += f * remote_f32(&part[i], k);
-        bad |= __float_as_int(remote_f32(reinterpret_cast<const float*>(&s_nan), k));
-      }
+  __syncthreads();
+  for (int i = tid; i < rows * D / 2; i += kJoinThreads) {
+    const int r = i / (D / 2), d = i % (D / 2) * 2, mm = tile_first + r;
+    float x = 0.f, y = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) {
+      const float2 v = *reinterpret_cast<const float2*>(part_of(k) + r * D + d);
+      x += s_f[r][k] * v.x;
+      y += s_f[r][k] * v.y;
     }
-    float v = sum == 0.f ? 0.f : acc / sum;   // nothing seen: 0
-    if (bad) {
-      // NaN codes of positions that this row sees and another row of the item does not
-      int rlo, rhi;
-      sees(m0 + r, rlo, rhi);
-      for (int j = rlo; j < rhi; ++j) {
-        if (j >= lo_max + TS && j < hi_min - TS) j = hi_min - TS;   // whole steps kept theirs
-        const int id = page_id(c, b, j / P, nullptr);
-        if (id < 0) continue;
-        const uint8_t code = c.codes[id * c.page_stride + ((long long)(c.kv_heads + h) * P + j % P) * D + d];
-        if (F::kTopExp == 8 && (code & 127) == 127) v = __int_as_float(0x7fffffff);
-      }
+    const float sum = s_sum[r], inv = sum == 0.f ? 0.f : 1.f / sum;
+    x *= inv;
+    y *= inv;
+    if (s_nan) {
+      if (sees_nan<F, P, TS, D>(c, a, w, b, h, group, tile_first, tile_last, mm, d)) x = __int_as_float(0x7fffffff);
+      if (sees_nan<F, P, TS, D>(c, a, w, b, h, group, tile_first, tile_last, mm, d + 1)) y = __int_as_float(0x7fffffff);
     }
-    const long long at = (long long)(r0 + (m0 + r) / group) * a.q_heads + h * group + (m0 + r) % group;
-    store_out(a.out, at * D + d, v, a.bf16);
-    if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    const long long row = (long long)(w.r0 + mm / group) * a.q_heads + h * group + mm % group;
+    *reinterpret_cast<uint32_t*>((uint16_t*)a.out + row * D + d) = pack_out(x, y, a.bf16);
+    if (a.lse && d == 0) a.lse[row] = sum == 0.f ? -INFINITY : (s_top[r] + log2f(sum)) * 0.6931471805599453f;
   }
-  if (split > 1) mk::cluster_sync_all();   // peers have read this block's shared memory
 }
 
 int cache_of(const mk_kv8* m, Cache* c);
 
-template <class F, int P, int D, int NT, int MW>
-static int launch_rows(const Cache& c, const Attend& a, cudaStream_t stream) {
+// SMs of a device and blocks of a kernel per SM, asked for once.
+template <class F, int P, int D, int NT, class K>
+static int resident_blocks(K kernel, int threads, int smem, int* blocks) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return MK_ERR_CUDA;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    int sms = 0, per = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess || per < 1)
+      return MK_ERR_CUDA;
+    n = sms * per;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  *blocks = n;
+  return MK_OK;
+}
+
+template <class F, int P, int D, int NT>
+static int launch_rows(const Cache& c, const Attend& a, void* work, size_t work_bytes, size_t* need, cudaStream_t stream) {
+  constexpr int smem = kWarps * kUnits * kUnitBytes;
+  auto kernel = &attend_rows_kernel<F, P, D, NT>;
+  int blocks = 0;
+  const int rc = resident_blocks<F, P, D, NT>(kernel, kWarps * 32, smem, &blocks);
+  if (rc != MK_OK) return rc;
+  *need = std::max(*need, (size_t)blocks * kWarps * 2 * part_floats<D, 8 * NT>() * sizeof(float));
+  if (!work) return MK_OK;
+  if (work_bytes < *need || ((uintptr_t)work & 15)) return MK_ERR_INVALID_ARG;
   const int group = a.q_heads / c.kv_heads;
-  const long long items = (long long)c.rows * group / (8 * NT * MW) + c.seqs;
-  const long long most = (long long)c.table_width * P;
-  // Blocks per item: until the grid fills the GPU ATT_FILL times over, but no
-  // more than one step of each group of warps per block at full capacity.
-  int split = 1;
-  while (split < 8 && items * c.kv_heads * split < 148 * ATT_FILL && most > (long long)split * (kWarps / MW) * (kStageBytes / 2 / D)) split *= 2;
-  const long long blocks = items * c.kv_heads * split;
-  if (blocks > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
-  auto kernel = &attend_rows_kernel<F, P, D, NT, MW>;
-  constexpr int bytes = rows_smem<D, NT, MW>();
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return MK_ERR_CUDA;
+  const long long items = ((long long)c.rows * group / (8 * NT) + c.seqs) * c.kv_heads;
+  if (items > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = bytes;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
+  if (cudaLaunchKernelEx(&cfg, kernel, c, a, (float*)work) != cudaSuccess) return MK_ERR_CUDA;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)split, 1, 1};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)items);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, c, a) == cudaSuccess ? MK_OK : MK_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, &attend_join_kernel<F, P, D, NT>, c, a, (const float*)work, blocks * kWarps) == cudaSuccess
+             ? MK_OK : MK_ERR_CUDA;
 }
 
 template <class F, int P, int D>
-static int launch(const Cache& c, const Attend& a, cudaStream_t stream) {
+static int launch(const Cache& c, const Attend& a, void* work, size_t work_bytes, size_t* need, cudaStream_t stream) {
+  if (!work) {   // what any number of rows needs
+    const int rc = launch_rows<F, P, D, 1>(c, a, work, work_bytes, need, stream);
+    return rc != MK_OK ? rc : launch_rows<F, P, D, 2>(c, a, work, work_bytes, need, stream);
+  }
   // rows of a sequence, once per query head of the group, on average
   const long long per = ((long long)c.rows * (a.q_heads / c.kv_heads) + c.seqs - 1) / c.seqs;
-  if (per <= 8) return launch_rows<F, P, D, 1, 1>(c, a, stream);
-  if (per <= 16) return launch_rows<F, P, D, 2, 1>(c, a, stream);
-  if (per <= 32) return launch_rows<F, P, D, 2, 2>(c, a, stream);
-  return launch_rows<F, P, D, 2, 4>(c, a, stream);
+  return per <= 8 ? launch_rows<F, P, D, 1>(c, a, work, work_bytes, need, stream)
+                  : launch_rows<F, P, D, 2>(c, a, work, work_bytes, need, stream);
 }
 
 }  // namespace mkp
 
 using namespace mkp;
 
-extern "C" int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long long q_row, long long q_head,
-                                     int q_heads, int type, float sm_scale, int causal, int window,
-                                     const int* d_kv_lens, void* d_out, float* d_lse, int* d_status, void* stream) {
+static int attend(const mk_kv8* cache, const void* d_q, long long q_row, long long q_head, int q_heads, int type,
+                  float sm_scale, int causal, int window, const int* d_kv_lens, void* d_out, float* d_lse, void* d_work,
+                  size_t work_bytes, size_t* need, int* d_status, void* stream) {
+  *need = 0;
   Cache c;
   const int rc = cache_of(cache, &c);
   if (rc != MK_OK) return rc;
   if (type != MK_TYPE_BF16 && type != MK_TYPE_F16) return MK_ERR_INVALID_ARG;
   if (q_heads < 1 || q_heads % c.kv_heads || q_heads > 65535 || window < 0 || !(sm_scale > 0.f))
     return MK_ERR_INVALID_ARG;
+  if ((long long)c.rows * q_heads > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
   if (c.rows == 0) return MK_OK;
   if (c.seqs == 0) return MK_ERR_INVALID_ARG;
   if (!d_q || !d_out || ((uintptr_t)d_q & 15) || ((uintptr_t)d_out & 15) || q_row % 8 || q_head % 8 || q_row < 0 ||
@@ -620,8 +830,8 @@ extern "C" int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long 
   auto with_d = [&](auto f, auto p) {
     using F = decltype(f);
     constexpr int P = decltype(p)::value;
-    return cache->head_dim == 64 ? launch<F, P, 64>(c, a, (cudaStream_t)stream)
-                                 : launch<F, P, 128>(c, a, (cudaStream_t)stream);
+    return cache->head_dim == 64 ? launch<F, P, 64>(c, a, d_work, work_bytes, need, (cudaStream_t)stream)
+                                 : launch<F, P, 128>(c, a, d_work, work_bytes, need, (cudaStream_t)stream);
   };
   auto with_p = [&](auto f) {
     if (cache->page_size == 16) return with_d(f, std::integral_constant<int, 16>{});
@@ -630,3 +840,31 @@ extern "C" int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long 
   };
   return cache->format == MK_KV8_E4M3 ? with_p(E4M3{}) : with_p(I8{});
 }
+
+extern "C" {
+
+long long megakernel_kv8_attend_workspace(const mk_kv8* cache, int q_heads) {
+  if (!cache) return MK_ERR_INVALID_ARG;
+  // a call without a workspace: every argument check, no launch
+  size_t need = 0;
+  mk_kv8 m = *cache;
+  void* some = (void*)(uintptr_t)256;
+  if (!m.d_codes) m.d_codes = some;
+  if (!m.d_scales) m.d_scales = (float*)some;
+  if (!m.d_page_table) m.d_page_table = (const int*)some;
+  if (!m.d_starts) m.d_starts = (const int*)some;
+  if (!m.d_first) m.d_first = (const int*)some;
+  const int rc = attend(&m, some, 0, 0, q_heads, MK_TYPE_BF16, 1.f, 1, 0, nullptr, some, nullptr, nullptr, 0, &need, nullptr, nullptr);
+  return rc == MK_OK ? (long long)need : rc;
+}
+
+int megakernel_kv8_attend(const mk_kv8* cache, const void* d_q, long long q_row, long long q_head, int q_heads, int type,
+                          float sm_scale, int causal, int window, const int* d_kv_lens, void* d_out, float* d_lse,
+                          void* d_work, long long work_bytes, int* d_status, void* stream) {
+  if (cache && cache->rows > 0 && (!d_work || work_bytes < 0)) return MK_ERR_INVALID_ARG;
+  size_t need = 0;
+  return attend(cache, d_q, q_row, q_head, q_heads, type, sm_scale, causal, window, d_kv_lens, d_out, d_lse, d_work,
+                (size_t)work_bytes, &need, d_status, stream);
+}
+
+}  // extern "C"

@@ -39,6 +39,7 @@ PAGE_SIZES = (16, 32, 64)
 HEAD_DIMS = (64, 128)
 
 _status = {}
+_work_floats = {}   # scratch of kv8_attend by what it depends on
 _lib_fns = None
 _get_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -53,7 +54,7 @@ def _fns():
     if _lib_fns is None:
         L = _lib.load()
         _lib_fns = (L.megakernel_qk_norm_rope, L.megakernel_kv8_append, L.megakernel_kv8_read,
-                    L.megakernel_kv8_attend, L.megakernel_verify_drafts)
+                    L.megakernel_kv8_attend, L.megakernel_verify_drafts, L.megakernel_kv8_attend_workspace)
     return _lib_fns
 
 
@@ -284,9 +285,19 @@ def kv8_attend(q, codes, scales, page_table, starts, first, *, kv_lens=None, sm_
     if out is None:
         out = q.new_empty((rows, hq, d))
     lse = scales.new_empty((rows, hq)) if return_lse else None
+    key = (idx, codes.dtype, codes.shape[3], d, hk, hq)
+    floats = _work_floats.get(key)
+    if floats is None:
+        floats = _fns()[5](cache, hq)
+        if floats < 0:
+            _lib.check(floats, "megakernel_kv8_attend_workspace")
+        if rows and seqs:
+            _work_floats[key] = floats = -(-floats // 4)
+    work = scales.new_empty((floats,))
     rc = _fns()[3](cache, q.data_ptr(), q_row, q_head, hq, TYPES[q.dtype], sm_scale, 1 if causal else 0, window,
                    None if kv_lens is None else kv_lens.data_ptr(), out.data_ptr(),
-                   None if lse is None else lse.data_ptr(), _status_of(idx), _raw_stream(idx))
+                   None if lse is None else lse.data_ptr(), work.data_ptr(), 4 * floats, _status_of(idx),
+                   _raw_stream(idx))
     if rc:
         _lib.check(rc, "megakernel_kv8_attend")
     return (out, lse) if return_lse else out

@@ -31,7 +31,8 @@ def test_c_entries_refuse_bad_caches(bad):
     L = lib()
     assert L.megakernel_kv8_append(kv8(**bad), FAKE, 128, 64, FAKE, 128, 64, 1, None, None) == -1
     assert L.megakernel_kv8_read(kv8(**bad), FAKE, FAKE, 1, None, None) == -1
-    assert L.megakernel_kv8_attend(kv8(**bad), FAKE, 256, 64, 4, 1, 0.125, 1, 0, None, FAKE, None, None, None) == -1
+    assert L.megakernel_kv8_attend(kv8(**bad), FAKE, 256, 64, 4, 1, 0.125, 1, 0, None, FAKE, None, FAKE, 1 << 30, None, None) == -1
+    assert L.megakernel_kv8_attend_workspace(kv8(**bad), 4) == -1 or set(bad) & {"codes", "scales", "page_table", "starts", "first"}
 
 
 def test_c_entries_refuse_bad_operands():
@@ -47,12 +48,12 @@ def test_c_entries_refuse_bad_operands():
     assert read(kv8(), FAKE, FAKE + 2, 1, None, None) == -1
     assert read(kv8(), FAKE, FAKE, -1, None, None) == -1
 
-    def attend(q=FAKE, row=256, head=64, hq=4, type=1, scale=0.125, window=0, out=FAKE):
-        return att(kv8(), q, row, head, hq, type, scale, 1, window, None, out, None, None, None)
+    def attend(q=FAKE, row=256, head=64, hq=4, type=1, scale=0.125, window=0, out=FAKE, work=FAKE, size=1 << 30):
+        return att(kv8(), q, row, head, hq, type, scale, 1, window, None, out, None, work, size, None, None)
 
     for bad in (dict(q=None), dict(q=FAKE + 2), dict(row=255), dict(head=60), dict(hq=3), dict(hq=0), dict(type=0),
                 dict(type=7), dict(scale=0.0), dict(scale=float("nan")), dict(window=-1), dict(out=None),
-                dict(out=FAKE + 8)):
+                dict(out=FAKE + 8), dict(work=None), dict(size=-1)):
         assert attend(**bad) == -1, bad
 
 
@@ -88,9 +89,9 @@ def test_empty_calls_do_nothing():
         c = kv8(codes=None, scales=None, page_table=None, starts=None, first=None, **none)
         assert L.megakernel_kv8_append(c, None, 0, 0, None, 0, 0, 1, None, None) == 0
         assert L.megakernel_kv8_read(c, None, None, 1, None, None) == 0
-    assert L.megakernel_kv8_attend(kv8(rows=0), None, 0, 0, 4, 1, 0.1, 1, 0, None, None, None, None, None) == 0
+    assert L.megakernel_kv8_attend(kv8(rows=0), None, 0, 0, 4, 1, 0.1, 1, 0, None, None, None, None, 0, None, None) == 0
     # rows that belong to no sequence
-    assert L.megakernel_kv8_attend(kv8(seqs=0), FAKE, 256, 64, 4, 1, 0.1, 1, 0, None, FAKE, None, None, None) == -1
+    assert L.megakernel_kv8_attend(kv8(seqs=0), FAKE, 256, 64, 4, 1, 0.1, 1, 0, None, FAKE, None, FAKE, 1 << 30, None, None) == -1
     assert L.megakernel_verify_drafts(None, None, 5, None, 5, None, None, None, 0, 0, 5, None, None, None, None) == 0
 
 
