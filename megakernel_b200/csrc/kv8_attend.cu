@@ -59,9 +59,8 @@ template <> __device__ __forceinline__ void expand<I8>(uint32_t w, uint32_t& lo,
 // Bits 7 of the bytes of w that are e4m3 NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// Eight 16-bit elements as floats, times f.
-__device__ __forceinline__ void load8(const void* q, long long i, bool bf16, float* v) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)q + i));
+// Eight 16-bit elements as floats.
+__device__ __forceinline__ void unpack8(const uint4& w, bool bf16, float* v) {
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -86,9 +85,8 @@ __device__ __forceinline__ uint64_t policy_evict_normal() {
 }
 
 constexpr int kWarps = 4;
-constexpr int kUnits = 3;              // ring of a warp, in units
 constexpr int kUnitBytes = 4096;       // the K or the V codes of one step
-constexpr int kMaxParts = 64;          // warps that may share an item
+constexpr int kMaxParts = 64;          // of an item
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr float kNone = -1e30f;        // running reference of a row that has seen nothing
 constexpr float kSlack = 5.f;          // weights may reach 2^kSlack before the reference moves
@@ -110,12 +108,15 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 //
 // Item: (sequence, tile of R rows counted once per query head of the group, kv
 // head).  All items of a sequence take the same number of steps of TS positions,
-// those that its rows see together.  The steps of all items, in order, are cut
-// into equal runs, one per warp of the grid; a warp with parts of several items
-// takes them one after the other.  Only the first and the last item of a run
-// can be shared with other warps: their parts go to the workspace (slot 2 w for
-// a part that continues an item, 2 w + 1 for one that begins it) and a second
-// small kernel joins them in order.
+// those that its rows see together.  An item of S steps is cut into ceil(S / run)
+// parts, run the smallest length for which the parts are sure to be no more than
+// the warps of the grid (steps / run + items of them at most), and each warp
+// takes one part: no warp waits for the plan of a second one, and the warps of
+// an SM, whose loads share its bandwidth, hold much the same in sum.  (Equal
+// runs over item borders: 64 x ~1,150 positions 32.7 us, see DESIGN.)  More items
+// than warps: one part each, taken in turn.  An item of one part is written
+// where it is computed; the parts of the others go to the workspace, and a
+// second small kernel joins them in order.
 struct SeqWork {
   int r0, n, first, len;   // rows, position of the first, positions held
   int begin, steps;        // first position and number of the steps, at least one step if there are rows
@@ -151,73 +152,125 @@ __device__ __forceinline__ SeqWork seq_work(const Cache& c, const Attend& a, int
   return w;
 }
 
-struct Total {
-  long long steps;   // of all items
-  int workers;       // warps that share them
+struct Plan {
+  int run;     // steps of a part, at most
+  int parts;   // of all items
 };
 
-__device__ __forceinline__ long long warp_scan(long long v) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) >= o) v += other;
-  }
-  return v;
+// ceil(steps / run), one fp32 division's worth of work: the quotient of numbers
+// up to 2^25 is at most one off.  The parts of an item have even shares of its steps.
+__device__ __forceinline__ int parts_of(int steps, int run) {
+  int n = (int)__fdividef((float)steps, (float)run);
+  n += n * run < steps;
+  n += n * run < steps;
+  return n - ((n - 1) * run >= steps && n > 0);
 }
 
-// Steps of all sequences, by one warp, and how many of `warps` share them: each
-// has at least one step, and the longest item at most kMaxParts + 2 parts.
-template <int P, int TS, int R>
-__device__ __forceinline__ Total total_work(const Cache& c, const Attend& a, int group, int warps, int* status) {
-  long long steps = 0;
-  int longest = 1;
-  for (int b = threadIdx.x & 31; b < c.seqs; b += 32) {
-    const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
-    if (w.error != MK_OK) report(status, w.error);
-    steps += (long long)w.tiles * w.steps;
-    longest = max(longest, w.steps);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    steps += __shfl_xor_sync(0xffffffffu, steps, o);
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  steps *= c.kv_heads;
-  return {steps, (int)min((long long)warps, max(steps * min(kMaxParts, longest) / longest, 1LL))};
-}
+// The sequences 128 at a time, four to a lane, so that their loads do not wait
+// for one another.
+constexpr int kPer = 4;
+struct Chunk { int steps[kPer], tiles[kPer]; };
 
-// The sequence that step (or, with by_item, item) number x falls into, and the
-// number of its first one.  x is less than the total.
 template <int P, int TS, int R>
-__device__ __forceinline__ int seq_at(const Cache& c, const Attend& a, int group, long long x, bool by_item, long long* base) {
-  const int lane = threadIdx.x & 31;
-  long long before = 0;
-  for (int b0 = 0; b0 < c.seqs; b0 += 32) {
-    long long mine = 0;
-    if (b0 + lane < c.seqs) {
-      const SeqWork w = seq_work<P, TS, R>(c, a, b0 + lane, group);
-      mine = (long long)w.tiles * (by_item ? 1 : w.steps) * c.kv_heads;
+__device__ __forceinline__ Chunk load_chunk(const Cache& c, const Attend& a, int base, int group, int* status) {
+  Chunk k;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = base + (threadIdx.x & 31) * kPer + i;
+    k.steps[i] = k.tiles[i] = 0;
+    if (b < c.seqs) {
+      const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
+      if (w.error != MK_OK) report(status, w.error);
+      k.steps[i] = w.steps;
+      k.tiles[i] = w.tiles;
     }
-    const long long upto = warp_scan(mine) + before;
-    const unsigned hit = __ballot_sync(0xffffffffu, x < upto);
+  }
+  return k;
+}
+
+// The plan, by one warp; *first gets the first chunk.
+template <int P, int TS, int R>
+__device__ __forceinline__ Plan make_plan(const Cache& c, const Attend& a, int group, int warps, int* status, Chunk* first) {
+  long long steps = 0, items = 0;
+  int longest = 1;
+  Chunk k = *first = load_chunk<P, TS, R>(c, a, 0, group, status);
+  for (int base = 0;;) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      steps += (long long)k.tiles[i] * k.steps[i];
+      items += k.tiles[i];
+      longest = max(longest, k.steps[i]);
+    }
+    base += 32 * kPer;
+    if (base >= c.seqs) break;
+    k = load_chunk<P, TS, R>(c, a, base, group, status);
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  Plan p;
+  p.run = longest;
+  // Above 2^25 steps or items in a lane nothing is cut.
+  const long long most = 1 << 25;
+  if (!__any_sync(0xffffffffu, steps * c.kv_heads > most || items * c.kv_heads > most)) {
+    const unsigned all = __reduce_add_sync(0xffffffffu, (unsigned)(steps * c.kv_heads));
+    const unsigned n = __reduce_add_sync(0xffffffffu, (unsigned)(items * c.kv_heads));
+    if (n < (unsigned)warps) p.run = (int)min(all / ((unsigned)warps - n) + 1, (unsigned)longest);
+  }
+  p.run = max(p.run, (longest + kMaxParts - 1) / kMaxParts);
+  int parts = 0;
+  k = *first;
+  for (int base = 0;;) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) parts += k.tiles[i] * parts_of(k.steps[i], p.run);
+    base += 32 * kPer;
+    if (base >= c.seqs) break;
+    k = load_chunk<P, TS, R>(c, a, base, group, nullptr);
+  }
+  // at most the items, or the warps: the host keeps rows x query heads below 2^31
+  p.parts = (int)__reduce_add_sync(0xffffffffu, (unsigned)parts) * c.kv_heads;
+  return p;
+}
+
+// The sequence that part number x falls into, and the number of its first
+// part; with seq >= 0, only that sequence's.
+template <int P, int TS, int R>
+__device__ __forceinline__ int seq_of_part(const Cache& c, const Attend& a, int group, const Plan& p, const Chunk& first, int x,
+                                           int seq, int* base_part) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  Chunk k = first;
+  for (int base = 0; base < c.seqs; base += 32 * kPer) {
+    if (base > 0 || c.seqs > 32 * kPer) k = load_chunk<P, TS, R>(c, a, base, group, nullptr);
+    int n[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      n[i] = k.tiles[i] * parts_of(k.steps[i], p.run) * c.kv_heads;
+      mine += n[i];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    upto += before;
+    // the sequence within the lane's four, and what lies before it
+    int at = upto - mine, found = kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (found < kPer) continue;
+      if (seq >= 0 ? base + lane * kPer + i == seq : x < at + n[i]) found = i;
+      else at += n[i];
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, found < kPer);
     if (hit) {
-      const int k = __ffs(hit) - 1;
-      *base = __shfl_sync(0xffffffffu, upto - mine, k);
-      return b0 + k;
+      const int src = __ffs(hit) - 1;
+      *base_part = __shfl_sync(0xffffffffu, at, src);
+      return base + src * kPer + __shfl_sync(0xffffffffu, found, src);
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
   }
-  *base = before;
+  *base_part = before;
   return -1;
-}
-
-// Run of worker w: [run_begin(w), run_begin(w + 1)); the worker whose run holds step x.
-__device__ __forceinline__ long long run_begin(const Total& t, int w) { return t.steps / t.workers * w + t.steps % t.workers * w / t.workers; }
-__device__ __forceinline__ int worker_of(const Total& t, long long x) {
-  int w = (int)min((double)t.workers - 1, (double)x / (double)t.steps * t.workers);
-  while (run_begin(t, w) > x) --w;
-  while (w + 1 < t.workers && run_begin(t, w + 1) <= x) ++w;
-  return w;
 }
 
 // A part in the workspace: R x D sums, then m and l of each row, then whether a NaN was taken out.
@@ -264,7 +317,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // ---- attention of few rows per sequence -------------------------------------------------
 //
 // Every warp works by itself.  The codes of a step, contiguous in a page, arrive
-// by bulk copies in a ring of three units of 4 KB (the K or the V codes of a
+// by bulk copies in a ring of 3 to 6 units of 4 KB (the K or the V codes of a
 // step): nothing of the stream passes through registers before it is used.
 // Both products have the positions or the head dimension as the 16 rows of an
 // m16n8k16 f16 product and the query rows as its 8 columns, fp32 accumulation:
@@ -285,10 +338,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // product in f16: 11 bits down to 2^-29 of the row's largest, an absolute 2^-35
 // below that (at p scale / vref alone it was 2^-25, which rows with one
 // dominant position showed).  The sum l takes the unrounded p.
+// Blocks per SM and ring units of a warp: what the registers leave room for, and
+// the shared memory of that many blocks.
+__host__ __device__ constexpr int rows_blocks(int D, int NT) { return D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2); }
+__host__ __device__ constexpr int rows_units(int D, int NT) { return rows_blocks(D, NT) == 4 ? 3 : rows_blocks(D, NT) == 3 ? 4 : 6; }
+
 template <class F, int P, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2))
+__global__ void __launch_bounds__(kWarps * 32, rows_blocks(D, NT))
 attend_rows_kernel(const Cache c, const Attend a, float* work) {
-  constexpr int TS = kUnitBytes / D, kSub = TS > P ? TS / P : 1;
+  constexpr int TS = kUnitBytes / D, kSub = TS > P ? TS / P : 1, kUnits = rows_units(D, NT);
   constexpr int kSubRows = TS / kSub;               // positions of a step in one page
   constexpr int kBatch = 32 / kSub;                 // steps whose pages the lanes hold
   constexpr int R = 8 * NT, MT = TS / 16;
@@ -306,30 +364,36 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
   }
   __syncwarp();
 
-  const Total all = total_work<P, TS, R>(c, a, group, (int)gridDim.x * kWarps, blockIdx.x == 0 && warp == 0 ? a.status : nullptr);
-  const int worker = warp * (int)gridDim.x + (int)blockIdx.x;   // neighbours on different SMs
-  if (worker >= all.workers || all.steps == 0) return;
-  long long at = run_begin(all, worker);
-  const long long end = run_begin(all, worker + 1);
-  if (at >= end) return;
-  long long seq_base;
-  int b = seq_at<P, TS, R>(c, a, group, at, false, &seq_base);
+  int x = warp * (int)gridDim.x + (int)blockIdx.x;   // the part; neighbours go to different SMs
+  int b, base_part;
+  Plan plan;
+  {
+    Chunk chunk;
+    plan = make_plan<P, TS, R>(c, a, group, (int)gridDim.x * kWarps,
+                               blockIdx.x == 0 && warp == 0 ? a.status : nullptr, &chunk);
+    if (x >= plan.parts) return;
+    b = seq_of_part<P, TS, R>(c, a, group, plan, chunk, x, -1, &base_part);
+  }
   int slot = 0;
-  uint32_t phase = 0;   // of ring slot `slot`; slots are used in turn over all items
+  uint32_t phase = 0;   // of ring slot `slot`; slots are used in turn over all parts
 
-  for (; at < end; ) {
+  while (b >= 0) {
     const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
-    const long long size = (long long)w.tiles * c.kv_heads * w.steps;
-    if (at >= seq_base + size) {   // also sequences without rows
-      seq_base += size;
-      ++b;
-      continue;
-    }
-    const int item = (int)((at - seq_base) / w.steps);
-    const long long item_base = seq_base + (long long)item * w.steps;
+    const int parts = parts_of(w.steps, plan.run);
+    const int item = (x - base_part) / parts, part_no = (x - base_part) % parts;
     const int h = item % c.kv_heads, tile_first = item / c.kv_heads * R, tile_last = min(tile_first + R, w.n * group) - 1;
-    const int s0 = (int)(at - item_base), s1 = (int)min((long long)w.steps, s0 + (end - at));
-    at += s1 - s0;
+    const int s0 = (int)((long long)w.steps * part_no / parts), s1 = (int)((long long)w.steps * (part_no + 1) / parts);
+
+    // q of rows 8 nt + g: dimensions 64 d + 16 t .. + 15, on the way while the pages are looked up
+    uint4 raw[NT][D / 32];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int m = tile_first + 8 * nt + g;
+      const uint16_t* src = (const uint16_t*)a.q + (long long)(w.r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head + 16 * t;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        raw[nt][i] = m <= tile_last ? __ldg(reinterpret_cast<const uint4*>(src + i / 2 * 64 + i % 2 * 8)) : make_uint4(0, 0, 0, 0);
+    }
     // steps of the part that some row of the tile sees
     int lo_all, hi_all, lo_max, hi_min;
     row_sees(w, a, group, tile_last, lo_max, hi_all);
@@ -387,19 +451,11 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
     int lo[NT][2], hi[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int m = tile_first + 8 * nt + g;
-      const bool real = m <= tile_last;
-      const long long src = real ? (long long)(w.r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head + 16 * t : 0;
       float v[D / 4];
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        if (real) {
-          load8(a.q, src + i / 2 * 64 + i % 2 * 8, a.bf16, v + 8 * i);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 8; ++x) v[8 * i + x] = 0.f;
-        }
+        unpack8(raw[nt][i], a.bf16, v + 8 * i);
 #pragma unroll
         for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(v[8 * i + x]));
       }
@@ -621,8 +677,8 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
     nan_seen = __any_sync(0xffffffffu, nan_seen);
 
     // ---- rows 2 t and 2 t + 1, dimensions (D / 8) g .. of the item, or its part
-    const bool is_part = s0 > 0 || s1 < w.steps;
-    float* part = work + (long long)(2 * worker + (s0 > 0 ? 0 : 1)) * part_floats<D, R>();
+    const bool is_part = parts > 1;   // then x is below the number of warps
+    float* part = work + (long long)x * part_floats<D, R>();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -662,82 +718,89 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
                               pack_out(v[8 * y + 4], v[8 * y + 5], a.bf16), pack_out(v[8 * y + 6], v[8 * y + 7], a.bf16));
         if (a.lse && g == 0) a.lse[row] = sum == 0.f ? -INFINITY : (m[nt][e] + log2f(sum)) * 0.6931471805599453f;
       }
+    x += (int)gridDim.x * kWarps;
+    if (x >= plan.parts) return;
+    b = seq_of_part<P, TS, R>(c, a, group, plan, load_chunk<P, TS, R>(c, a, 0, group, nullptr), x, -1, &base_part);
   }
 }
 
-// Joins the parts of an item that several warps shared, in their order.
+// Joins the parts of the items that have several, in their order: one warp per
+// (row, query head).  Everything up to the wait overlaps the first kernel's end.
 constexpr int kJoinThreads = 256;
 template <class F, int P, int D, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const Cache c, const Attend a, const float* work, int warps) {
-  constexpr int TS = kUnitBytes / D, R = 8 * NT, kFloats = part_floats<D, R>();
-  __shared__ float s_f[R][kMaxParts + 2], s_top[R], s_sum[R];
-  __shared__ int s_nan;
-  const int group = a.q_heads / c.kv_heads, tid = threadIdx.x;
-  const Total all = total_work<P, TS, R>(c, a, group, warps, nullptr);
-  long long item_base;
-  const int b = seq_at<P, TS, R>(c, a, group, blockIdx.x, true, &item_base);
-  if (b < 0) {   // a spare block
-    mk::pdl_wait();
-    return;
+  constexpr int TS = kUnitBytes / D, R = 8 * NT, kFloats = part_floats<D, R>(), V = D / 32;
+  const int group = a.q_heads / c.kv_heads, lane = threadIdx.x & 31;
+  const long long unit = (long long)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  const int row = (int)(unit / a.q_heads), hq = (int)(unit % a.q_heads), h = hq / group;
+  int b = -1, parts = 1, first_part = 0, m = 0, tile_first = 0;
+  SeqWork w;
+  if (row < c.rows) {
+    Chunk chunk;
+    const Plan plan = make_plan<P, TS, R>(c, a, group, warps, nullptr, &chunk);
+    b = warp_search(c.seqs, row, [&](int i) { return __ldg(c.starts + i); });
+    w = seq_work<P, TS, R>(c, a, b, group);
+    if (row < w.r0 || row >= w.r0 + w.n) b = -1;   // of no sequence
+    if (b >= 0) {
+      int base_part;
+      seq_of_part<P, TS, R>(c, a, group, plan, chunk, 0, b, &base_part);
+      m = (row - w.r0) * group + hq % group;
+      tile_first = m / R * R;
+      parts = parts_of(w.steps, plan.run);
+      first_part = base_part + (m / R * c.kv_heads + h) * parts;
+    }
   }
-  const SeqWork w = seq_work<P, TS, R>(c, a, b, group);
-  const int item = (int)(blockIdx.x - item_base), h = item % c.kv_heads;
-  const int tile_first = item / c.kv_heads * R, tile_last = min(tile_first + R, w.n * group) - 1;
-  // the number of the sequence's first step: as seq_at, over the steps
-  long long step = 0;
-  for (int i = tid & 31; i < b; i += 32) {
-    const SeqWork x = seq_work<P, TS, R>(c, a, i, group);
-    step += (long long)x.tiles * x.steps;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) step += __shfl_xor_sync(0xffffffffu, step, o);
-  step = step * c.kv_heads + (long long)item * w.steps;
-  const int w0 = worker_of(all, step), w1 = worker_of(all, step + w.steps - 1);
-  const int parts = min(w1 - w0 + 1, kMaxParts + 2);   // never more, see total_work
-  if (tid == 0) s_nan = 0;
   mk::pdl_wait();   // every block: the end of this kernel stands for the end of both
-  if (parts == 1) return;   // written whole
-  __syncthreads();
-  auto part_of = [&](int x) { return work + (long long)(2 * (w0 + x) + (x == 0 ? 1 : 0)) * kFloats; };
-  const int rows = tile_last - tile_first + 1;
-  for (int i = tid; i < rows * parts; i += kJoinThreads) s_f[i % rows][i / rows] = part_of(i / rows)[R * D + i % rows];
-  for (int i = tid; i < parts; i += kJoinThreads)
-    if (__float_as_int(part_of(i)[R * D + 2 * R])) s_nan = 1;
-  __syncthreads();
-  // one warp per row: maximum, factors, sum
-  for (int r = tid >> 5; r < rows; r += kJoinThreads / 32) {
-    float top = kNone, sum = 0.f;
-    for (int i = tid & 31; i < parts; i += 32) top = fmaxf(top, s_f[r][i]);
-    top = mk::warp_max(top);
-    for (int i = tid & 31; i < parts; i += 32) {
-      const float f = ex2(s_f[r][i] - top);
-      s_f[r][i] = f;
-      sum += f * part_of(i)[R * D + R + r];
+  if (b < 0 || parts == 1) return;   // written whole
+  const float* part = work + (long long)first_part * kFloats;
+  const int r = m % R, d = V * lane;
+  float acc[V] = {}, top = kNone, sum = 0.f;
+  int bad = 0;
+  constexpr int kDeep = 8;
+  for (int k0 = 0; k0 < parts; k0 += kDeep) {
+    float pm[kDeep], pl[kDeep], po[kDeep][V];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const float* q = part + (long long)min(k0 + i, parts - 1) * kFloats;
+      pm[i] = k0 + i < parts ? q[R * D + r] : kNone;
+      pl[i] = k0 + i < parts ? q[R * D + R + r] : 0.f;
+      bad |= __float_as_int(q[R * D + 2 * R]);
+#pragma unroll
+      for (int y = 0; y < V; y += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(q + r * D + d + y);
+        po[i][y] = v.x;
+        po[i][y + 1] = v.y;
+      }
     }
-    sum = mk::warp_sum(sum);
-    if ((tid & 31) == 0) s_top[r] = top, s_sum[r] = sum;
+    float now = top;
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) now = fmaxf(now, pm[i]);
+    const float keep = ex2(top - now);
+    sum *= keep;
+#pragma unroll
+    for (int y = 0; y < V; ++y) acc[y] *= keep;
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const float f = k0 + i < parts ? ex2(pm[i] - now) : 0.f;
+      if (k0 + i >= parts) continue;
+      sum += f * pl[i];
+#pragma unroll
+      for (int y = 0; y < V; ++y) acc[y] += f * po[i][y];
+    }
+    top = now;
   }
-  __syncthreads();
-  for (int i = tid; i < rows * D / 2; i += kJoinThreads) {
-    const int r = i / (D / 2), d = i % (D / 2) * 2, mm = tile_first + r;
-    float x = 0.f, y = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < parts; ++k) {
-      const float2 v = *reinterpret_cast<const float2*>(part_of(k) + r * D + d);
-      x += s_f[r][k] * v.x;
-      y += s_f[r][k] * v.y;
-    }
-    const float sum = s_sum[r], inv = sum == 0.f ? 0.f : 1.f / sum;
-    x *= inv;
-    y *= inv;
-    if (s_nan) {
-      if (sees_nan<F, P, TS, D>(c, a, w, b, h, group, tile_first, tile_last, mm, d)) x = __int_as_float(0x7fffffff);
-      if (sees_nan<F, P, TS, D>(c, a, w, b, h, group, tile_first, tile_last, mm, d + 1)) y = __int_as_float(0x7fffffff);
-    }
-    const long long row = (long long)(w.r0 + mm / group) * a.q_heads + h * group + mm % group;
-    *reinterpret_cast<uint32_t*>((uint16_t*)a.out + row * D + d) = pack_out(x, y, a.bf16);
-    if (a.lse && d == 0) a.lse[row] = sum == 0.f ? -INFINITY : (s_top[r] + log2f(sum)) * 0.6931471805599453f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int y = 0; y < V; ++y) {
+    acc[y] *= inv;
+    if (bad && sees_nan<F, P, TS, D>(c, a, w, b, h, group, tile_first, min(tile_first + R, w.n * group) - 1, m, d + y))
+      acc[y] = __int_as_float(0x7fffffff);
   }
+  const long long at = (long long)row * a.q_heads + hq;
+  uint32_t* out = reinterpret_cast<uint32_t*>((uint16_t*)a.out + at * D + d);
+#pragma unroll
+  for (int y = 0; y < V; y += 2) out[y / 2] = pack_out(acc[y], acc[y + 1], a.bf16);
+  if (a.lse && lane == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 int cache_of(const mk_kv8* m, Cache* c);
@@ -764,17 +827,14 @@ static int resident_blocks(K kernel, int threads, int smem, int* blocks) {
 
 template <class F, int P, int D, int NT>
 static int launch_rows(const Cache& c, const Attend& a, void* work, size_t work_bytes, size_t* need, cudaStream_t stream) {
-  constexpr int smem = kWarps * kUnits * kUnitBytes;
+  constexpr int smem = kWarps * rows_units(D, NT) * kUnitBytes;
   auto kernel = &attend_rows_kernel<F, P, D, NT>;
   int blocks = 0;
   const int rc = resident_blocks<F, P, D, NT>(kernel, kWarps * 32, smem, &blocks);
   if (rc != MK_OK) return rc;
-  *need = std::max(*need, (size_t)blocks * kWarps * 2 * part_floats<D, 8 * NT>() * sizeof(float));
+  *need = std::max(*need, (size_t)blocks * kWarps * part_floats<D, 8 * NT>() * sizeof(float));
   if (!work) return MK_OK;
   if (work_bytes < *need || ((uintptr_t)work & 15)) return MK_ERR_INVALID_ARG;
-  const int group = a.q_heads / c.kv_heads;
-  const long long items = ((long long)c.rows * group / (8 * NT) + c.seqs) * c.kv_heads;
-  if (items > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kWarps * 32);
@@ -784,7 +844,7 @@ static int launch_rows(const Cache& c, const Attend& a, void* work, size_t work_
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)items);
+  cfg.gridDim = dim3((unsigned)(((long long)c.rows * a.q_heads + kJoinThreads / 32 - 1) / (kJoinThreads / 32)));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.attrs = at;

@@ -229,16 +229,6 @@ struct Verify {
 
 constexpr int kVerifyThreads = 256, kVerifyDeep = 16, kVerifyWarps = kVerifyThreads / 32, kVerifyChunks = 32;
 
-// Inclusive sum over the warp.
-__device__ __forceinline__ long long warp_scan(long long v) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) >= o) v += other;
-  }
-  return v;
-}
-
 // One cluster per sequence.  The vocabulary is cut into one run per block, each
 // run into one segment per warp, each segment into at most 32 chunks (of 512
 // tokens up to vocabularies of 262,144).  The rows are read once in 16-byte

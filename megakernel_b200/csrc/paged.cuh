@@ -92,6 +92,16 @@ __device__ __forceinline__ int warp_search(int n, int x, F key) {
   return lo;
 }
 
+// Inclusive sum over the warp.
+__device__ __forceinline__ long long warp_scan(long long v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long other = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += other;
+  }
+  return v;
+}
+
 // The rows of sequence b as the kernels may use them: packed rows
 // [row, row + count) at positions [pos, pos + count).  Rows at negative
 // positions are left out (they stand for padding).
