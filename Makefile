@@ -10,7 +10,8 @@ NVCC ?= nvcc
 ARCH_FLAGS = -gencode arch=compute_100a,code=sm_100a
 NVCC_FLAGS = -O3 -std=c++17 -lineinfo -Xcompiler -fPIC
 CSRC = megakernel_b200/csrc
-UNITS = $(CSRC)/megakernel.cu $(CSRC)/tp.cu $(CSRC)/paged.cu $(CSRC)/kv8_attend.cu
+UNITS = $(CSRC)/megakernel.cu $(CSRC)/tp.cu $(CSRC)/paged.cu $(CSRC)/kv8_attend.cu \
+        $(CSRC)/kv8_prompt.cu
 DEPS = $(wildcard $(CSRC)/*.cu $(CSRC)/*.cuh) include/megakernel.h
 BUILD ?= _build
 LIB_OUT ?= megakernel.so

@@ -17,9 +17,11 @@ LIB_PATH = os.path.join(PKG_DIR, "libmegakernel.so")
 HEADER = os.path.join(ROOT, "include", "megakernel.h")
 SOURCES = [os.path.join(CSRC, f) for f in ("megakernel.cu", "noalloc.cu", "decode_kernel.cuh", "ptx.cuh",
                                                   "shapes.cuh", "batch.cu", "tc_gemm.cuh", "tc_ptx.cuh",
-                                                  "tp.cu", "paged.cuh", "paged.cu", "kv8_attend.cu")]
+                                                  "tp.cu", "paged.cuh", "paged.cu", "kv8_attend.cuh",
+                                                  "kv8_attend.cu", "kv8_prompt.cu")]
 # Translation units, compiled in parallel and linked into one library.
-UNITS = ["megakernel.cu", "tp.cu", "paged.cu", "kv8_attend.cu"]
+UNITS = ["megakernel.cu", "tp.cu", "paged.cu", "kv8_attend.cu",
+         "kv8_prompt.cu"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]

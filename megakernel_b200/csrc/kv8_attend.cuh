@@ -1,0 +1,148 @@
+// Pieces shared by the kernels of attention over the paged 8-bit cache.
+#pragma once
+#include "paged.cuh"
+#include "tc_ptx.cuh"
+
+namespace mkp {
+
+struct Attend {
+  const void* q;
+  void* out;
+  float* lse;
+  const int* kv_lens;
+  long long q_row, q_head;
+  int q_heads, causal, window;
+  float scale;   // log2(e) x the softmax scale
+  int bf16;      // q and out: bf16, else f16
+  int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two codes (the low or the high half of w) -> f16x2, exactly: e4m3 and the
+// whole numbers to 127 are f16 values.
+template <class F> __device__ __forceinline__ void expand(uint32_t w, uint32_t& lo, uint32_t& hi);
+template <> __device__ __forceinline__ void expand<E4M3>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// 0x6400 + b is the f16 value 1024 + b for a byte b; codes are biased by 128.
+template <> __device__ __forceinline__ void expand<I8>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 bias = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+  uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 a = __hsub2(*reinterpret_cast<__half2*>(&x), bias);
+  const __half2 b = __hsub2(*reinterpret_cast<__half2*>(&y), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Bits 7 of the bytes of w that are e4m3 NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// Eight 16-bit elements as floats.
+__device__ __forceinline__ void unpack8(const uint4& w, bool bf16, float* v) {
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (bf16) {
+      v[2 * k] = __uint_as_float(ws[k] << 16);
+      v[2 * k + 1] = __uint_as_float(ws[k] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ws[k]));
+      v[2 * k] = f.x;
+      v[2 * k + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi, bool bf16) {
+  return bf16 ? mk::pack_bf16x2(lo, hi) : pack_f16(lo, hi);
+}
+
+constexpr uint32_t kWaitLimit = 1u << 20;
+constexpr float kNone = -1e30f;        // running reference of a row that has seen nothing
+constexpr float kSlack = 5.f;          // weights may reach 2^kSlack before the reference moves
+
+// Bounded wait; each probe may itself suspend for a while.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i)
+    if (mk::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
+// ---- sequences and what their rows see --------------------------------------------------
+
+struct SeqWork {
+  int r0, n, first, len;   // rows, position of the first, positions held
+  int begin, steps;        // first position and number of the steps, at least one step if there are rows
+  int tiles;
+  int error;               // MK_OK, or what is wrong with the sequence
+};
+
+template <int P, int TS, int R>
+__device__ __forceinline__ SeqWork seq_work(const Cache& c, const Attend& a, int b, int group) {
+  SeqWork w;
+  w.r0 = __ldg(c.starts + b);
+  const int r1 = __ldg(c.starts + b + 1);
+  w.first = __ldg(c.first + b);
+  w.n = r1 - w.r0;
+  w.len = a.kv_lens ? __ldg(a.kv_lens + b) : 0;
+  w.begin = w.steps = w.tiles = 0;
+  w.error = w.r0 < 0 || r1 < w.r0 || r1 > c.rows || w.first > (1 << 30) ? MK_ERR_INVALID_ARG : MK_OK;
+  if (w.error != MK_OK || w.n == 0) {
+    w.n = 0;
+    return w;
+  }
+  if (!a.kv_lens) w.len = w.first + w.n;
+  if (w.len > c.table_width * P) {
+    w.len = c.table_width * P;
+    w.error = MK_ERR_CAPACITY;
+  }
+  const int last = w.first + w.n - 1, low = max(w.first, 0);
+  const int hi = last < 0 ? 0 : a.causal ? min(w.len, last + 1) : w.len;
+  const int lo = a.window ? max(low - a.window + 1, 0) : 0;
+  w.begin = lo / TS * TS;
+  w.steps = hi > w.begin ? (hi - w.begin + TS - 1) / TS : 1;
+  w.tiles = (int)(((long long)w.n * group + R - 1) / R);
+  return w;
+}
+
+// What row index m of a sequence sees: [lo, hi).
+__device__ __forceinline__ void row_sees(const SeqWork& w, const Attend& a, int group, int m, int& lo, int& hi) {
+  const int pos = w.first + m / group;
+  lo = hi = 0;
+  if (m < w.n * group && pos >= 0) {
+    hi = max(a.causal ? min(w.len, pos + 1) : w.len, 0);
+    lo = a.window ? max(pos - a.window + 1, 0) : 0;
+  }
+}
+
+// Whether a position that row index m sees holds a NaN code in dimension d of V.  Only
+// positions of steps that some row of the tile does not see wholly are looked at.
+template <class F, int P, int TS, int D>
+__device__ __noinline__ bool sees_nan(const Cache& c, const Attend& a, const SeqWork& w, int b, int h, int group, int tile_first,
+                                      int tile_last, int m, int d) {
+  if (F::kTopExp != 8) return false;
+  int lo, hi, lo_max, hi_min, x;
+  row_sees(w, a, group, m, lo, hi);
+  row_sees(w, a, group, tile_last, lo_max, x);
+  row_sees(w, a, group, tile_first, x, hi_min);
+  for (int j = lo; j < hi; ++j) {
+    if (j >= lo_max + TS && j < hi_min - TS) j = hi_min - TS;
+    const int id = page_id(c, b, j / P, nullptr);
+    if (id < 0) continue;
+    const uint8_t code = c.codes[id * c.page_stride + ((long long)(c.kv_heads + h) * P + j % P) * D + d];
+    if ((code & 127) == 127) return true;
+  }
+  return false;
+}
+
+}  // namespace mkp

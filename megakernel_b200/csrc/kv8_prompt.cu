@@ -1,0 +1,536 @@
+// Attention of many rows per sequence over the paged 8-bit cache, on tcgen05
+// tensor cores (megakernel_kv8_attend chooses it, see kv8_attend.cu).
+#include <atomic>
+
+#include "kv8_attend.cuh"
+
+namespace mkp {
+
+// ---- tcgen05 pieces -------------------------------------------------------------------
+
+// D[tmem] (+)= A[smem] B[smem], f16 in, fp32 accumulate (kind::f16 with f16 operands).
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  mk::tc_mma_bf16(d, adesc, bdesc, idesc, accumulate);   // the operand types are idesc's
+}
+// The same with A in tensor memory: 128 lanes, two f16 per 32-bit column.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// f16 A and B, fp32 D, M x N; b_mn: B is stored with N contiguous.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// Operand of 64-element rows of 128 bytes, 128-byte swizzle, 8-row groups 1,024 bytes
+// apart: K contiguous (K-major), or N contiguous with the next 64 of N `next`
+// bytes on.
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr, uint32_t next) {
+  return (mk::tc_desc_sw128(addr) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)((next >> 4) & 0x3fff) << 16);
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- layout ------------------------------------------------------------------------------
+
+constexpr int kTile = 128;                       // rows of a query tile, positions of a step
+constexpr int kRowWarps = 8, kCodeWarps = 4;     // two query tiles; converters
+constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 1) * 32;
+constexpr int kMetaSlots = 4;
+
+template <int D>
+struct PromptSmem {
+  static constexpr int kOperand = kTile * D * 2;                 // Q tile, K or V step in f16
+  static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kBytes = 6 * kOperand;
+};
+
+// ---- attention of many rows per sequence ---------------------------------------------------
+//
+// Work item: 256 rows of one (sequence, kv head), as two tiles of 128, all their
+// positions in steps of 128.  Roles of a block's 13 warps:
+//   warps 0-3, 4-7   one tile of rows each, one row per thread: softmax
+//   warps 8-11       codes from global memory to f16 operands in shared memory
+//   warp 12          one thread issues every tcgen05.mma
+// S = Q K^T [128 x 128] and O [128 x D] live in tensor memory; the weights go
+// back to tensor memory as f16, over their scores, and are the A operand of
+// O += P V.  While one tile's scores are with its warps the tensor cores work
+// for the other.  Two steps of K and of V are in shared memory at once, each
+// converted once for both tiles.
+//
+// Softmax and scales as in kv8_attend.cu: a reference m per row that moves only
+// when some weight would pass 2^5, weights 2^10 p in f16; the scale of a K page
+// multiplies its scores.  A V page's scale relative to the largest so far
+// multiplies its codes on their way to f16: exact for powers of two (an absolute
+// 2^-25 of the largest scale at worst), one rounding to 11 bits otherwise.
+template <class F, int P, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const Cache c, const Attend a) {
+  using S = PromptSmem<D>;
+  constexpr int kSub = kTile / P;                    // pages of a step
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+  __shared__ float s_ks[kMetaSlots][kSub], s_vref[kMetaSlots];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_nan;
+  __shared__ volatile int s_abort;
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = a.q_heads / c.kv_heads;
+  // items in reverse: the last tiles of a sequence see the most positions
+  const int unit = (int)(gridDim.x - 1 - blockIdx.x), h = unit % c.kv_heads, item = unit / c.kv_heads;
+  auto key = [&](int i) { return (int)((long long)__ldg(c.starts + i) * group / (2 * kTile)) + i; };
+  const int b = warp_search(c.seqs, item, key);
+  const SeqWork w = seq_work<P, kTile, 2 * kTile>(c, a, b, group);
+  if (w.error != MK_OK && threadIdx.x == 0) report(a.status, w.error);
+  const int tile = item - key(b);
+  if (w.n == 0 || tile < 0 || tile >= w.tiles) return;
+  const int row0 = tile * 2 * kTile, row_last = min(row0 + 2 * kTile, w.n * group) - 1;
+  const int tiles = row_last - row0 >= kTile ? 2 : 1;
+
+  // positions that some row, and that every row, of a range of rows sees
+  struct Range { int lo, hi, lo_max, hi_min; };
+  auto range_of = [&](int m_first, int m_last) {
+    Range r;
+    row_sees(w, a, group, m_last, r.lo_max, r.hi);
+    row_sees(w, a, group, m_first, r.lo, r.hi_min);
+    return r;
+  };
+  const Range all = range_of(row0, row_last);
+  Range own[2];
+  int j_lo[2], j_hi[2];   // steps of each tile
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    own[x] = range_of(row0 + x * kTile, min(row0 + (x + 1) * kTile - 1, row_last));
+    j_lo[x] = own[x].lo / kTile;
+    j_hi[x] = x < tiles && own[x].hi > own[x].lo ? (own[x].hi + kTile - 1) / kTile : j_lo[x];
+  }
+  const int first = all.lo / kTile, last = max(j_hi[0], tiles == 2 ? j_hi[1] : 0);
+
+  if (threadIdx.x == 0) {
+    s_nan = 0;
+    s_abort = 0;
+    for (int i = 0; i < 2; ++i) {
+      mk::mbar_init(&k_full[i], kCodeWarps * 32);
+      mk::mbar_init(&v_full[i], kCodeWarps * 32);
+      mk::mbar_init(&k_empty[i], 1);
+      mk::mbar_init(&v_empty[i], 1);
+      mk::mbar_init(&s_full[i], 1);
+      mk::mbar_init(&p_full[i], 128);
+      mk::mbar_init(&o_full[i], 1);
+    }
+    mk::fence_mbar_init();
+  }
+  if (warp == kRowWarps + kCodeWarps) {
+    mk::tmem_alloc(&s_tmem, 512);
+    mk::tmem_relinquish();
+  }
+
+  // Bounded wait that also ends when another role gave up.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+      if (mk::mbar_try_wait(bar, parity)) return true;
+      if ((i & 63) == 63 && s_abort) return false;
+    }
+    s_abort = 1;
+    return false;
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
+
+  // ---- Q: thread r < 256 brings its row to f16, K contiguous, swizzled
+  const int x = warp >> 2, r = threadIdx.x & 127;   // tile and row of a softmax thread
+  const int m_row = row0 + x * kTile + r;
+  float rq = 0.f;
+  if (warp < kRowWarps) {
+    const bool real = m_row <= row_last;
+    const uint16_t* src = (const uint16_t*)a.q + (long long)(w.r0 + m_row / group) * a.q_row + (h * group + m_row % group) * a.q_head;
+    float top = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      float v[8];
+      unpack8(real ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0), a.bf16, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+    }
+    const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);   // as in kv8_attend.cu
+    const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
+    rq = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
+    uint8_t* dst = smem + S::kQ + x * S::kOperand + r * 128;
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      float v[8];
+      unpack8(real ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0), a.bf16, v);
+      uint4 o;
+      o.x = pack_f16(v[0] * up, v[1] * up);
+      o.y = pack_f16(v[2] * up, v[3] * up);
+      o.z = pack_f16(v[4] * up, v[5] * up);
+      o.w = pack_f16(v[6] * up, v[7] * up);
+      *reinterpret_cast<uint4*>(dst + i / 8 * (kTile * 128) + ((i % 8) ^ (r & 7)) * 16) = o;
+    }
+    fence_async_shared();
+  }
+  mk::tc_fence_before();
+  __syncthreads();
+  mk::tc_fence_after();
+  const uint32_t tm = s_tmem, smem0 = mk::smem_u32(smem);
+  const uint32_t tm_s[2] = {tm, tm + kTile}, tm_o[2] = {tm + 2 * kTile, tm + 2 * kTile + D};
+
+  if (warp < kRowWarps) {
+    // ---- softmax of one row
+    const uint32_t quarter = (uint32_t)(warp & 3) << 21;   // lanes 32 (warp % 4) ..
+    const uint32_t ts = (x ? tm_s[1] : tm_s[0]) + quarter, to = (x ? tm_o[1] : tm_o[0]) + quarter;
+    int lo, hi;
+    row_sees(w, a, group, m_row, lo, hi);
+    const int my_lo = x ? j_lo[1] : j_lo[0], my_hi = x ? j_hi[1] : j_hi[0];
+    const int lo_max = x ? own[1].lo_max : own[0].lo_max, hi_min = x ? own[1].hi_min : own[0].hi_min;
+    float m = kNone, l = 0.f, vref = 0.f;
+    bool ok = true;
+    uint32_t phase = 0;
+    for (int j = my_lo; j < my_hi; ++j, phase ^= 1) {
+      if (!(ok = wait_warp(&s_full[x], phase))) break;
+      mk::tc_fence_after();
+      const int pos = j * kTile;
+      float f[kSub];
+      bool whole = pos >= lo_max && pos + kTile <= hi_min;
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        const float ks = s_ks[j % kMetaSlots][i];
+        whole = whole && ks > 0.f;
+        f[i] = ks > 0.f ? fmaxf(rq * ks, 1.17549435e-38f) : 0.f;
+      }
+      const float vnow = s_vref[j % kMetaSlots];
+      // hidden positions of 32 scores from column c0 on
+      auto hide = [&](float (&v)[32], int c0) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int p = pos + c0 + i;
+          if (p < lo || p >= hi || f[(c0 + i) / P] == 0.f) v[i] = -INFINITY;
+        }
+      };
+      float top = kNone;
+#pragma unroll
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+        uint32_t raw[32];
+        mk::tmem_ld_32x32b_x32(ts + c0, raw);
+        mk::tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+        if (!whole) hide(v, c0);
+        constexpr int kRun = P < 32 ? P : 32;
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += kRun) {
+          float t = v[i0];
+#pragma unroll
+          for (int i = 1; i < kRun; ++i) t = fmaxf(t, v[i0 + i]);
+          const float g = f[(c0 + i0) / P];
+          top = fmaxf(top, g == 0.f ? kNone : t * g);
+        }
+      }
+      const bool move = top > m + kSlack;
+      if (__any_sync(0xffffffffu, move) || vnow > vref) {
+        float keep = vnow > vref ? vref / vnow : 1.f;
+        if (move) {
+          const float k = ex2(m - top);
+          l *= k;
+          keep *= k;
+          m = top;
+        }
+        vref = vnow;
+        if (j > my_lo) {   // P V of the step before is complete: its scores came after it
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            mk::tmem_ld_32x32b_x32(to + c0, o);
+            mk::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+            tmem_st_x32(to + c0, o);
+          }
+        }
+      }
+      const float back = 10.f - m;   // weights are 2^10 p
+#pragma unroll
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+        uint32_t raw[32];
+        mk::tmem_ld_32x32b_x32(ts + c0, raw);
+        mk::tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+        if (!whole) hide(v, c0);
+        uint32_t p[16];
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float g = f[(c0 + i) / P];
+          if (!whole) g = fmaxf(g, 1.17549435e-38f);   // -inf x 0 would be NaN
+          const float e0 = ex2(fmaf(v[i], g, back)), e1 = ex2(fmaf(v[i + 1], g, back));
+          sum[0] += e0;
+          sum[1] += e1;
+          p[i / 2] = pack_f16(e0, e1);
+        }
+        l += sum[0] + sum[1];
+        tmem_st_x16(ts + c0 / 2, p);
+      }
+      tmem_st_wait();
+      mk::tc_fence_before();
+      mk::mbar_arrive(&p_full[x]);
+    }
+    // ---- write the row
+    if (ok && my_hi > my_lo) ok = wait_warp(&o_full[x], 0);
+    if (ok && x < tiles) {
+      mk::tc_fence_after();
+      const bool real = m_row <= row_last;
+      const float inv = l == 0.f ? 0.f : vref / l;   // nothing seen: 0
+      const bool nan = s_nan != 0;
+      const long long at = (long long)(w.r0 + m_row / group) * a.q_heads + h * group + m_row % group;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        if (my_hi > my_lo) {
+          mk::tmem_ld_32x32b_x32(to + c0, o);
+          mk::tmem_ld_wait();
+        }
+        if (!real) continue;
+        uint4* out = reinterpret_cast<uint4*>((uint16_t*)a.out + at * D + c0);
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            v[k] = my_hi > my_lo && l != 0.f ? __uint_as_float(o[i + k]) * inv : 0.f;
+            if (nan && sees_nan<F, P, kTile, D>(c, a, w, b, h, group, row0, row_last, m_row, c0 + i + k))
+              v[k] = __int_as_float(0x7fffffff);
+          }
+          out[i / 8] = make_uint4(pack_out(v[0], v[1], a.bf16), pack_out(v[2], v[3], a.bf16), pack_out(v[4], v[5], a.bf16),
+                                  pack_out(v[6], v[7], a.bf16));
+        }
+      }
+      if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - 10.f + log2f(l)) * 0.6931471805599453f;
+    }
+  } else if (warp < kRowWarps + kCodeWarps) {
+    // ---- codes to f16
+    constexpr int kLanes = D / 16, kRowsPer = kCodeWarps * 32 / kLanes, kPasses = kTile / kRowsPer;
+    const int ct = threadIdx.x - kRowWarps * 32, cc = ct % kLanes, cr = ct / kLanes;
+    struct Page { int id; float ks, vs; };
+    auto page_of = [&](int j) {   // lane i: page i of step j
+      Page p{-1, 0.f, 0.f};
+      const int pos = j * kTile + lane * P;
+      if (j < last && lane < kSub && pos < all.hi && pos + P > all.lo) {
+        p.id = page_id(c, b, pos / P, a.status);
+        if (p.id >= 0) {
+          const float* sc = c.scales + p.id * c.scale_stride + h;
+          p.ks = fmaxf(__ldg(sc), 1.17549435e-38f);
+          p.vs = __ldg(sc + c.kv_heads);
+        }
+      }
+      return p;
+    };
+    auto load = [&](const Page& p, int kv, uint4 (&v)[kPasses]) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int row = cr + i * kRowsPer;
+        const int id = __shfl_sync(0xffffffffu, p.id, row / P);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (id >= 0)
+          v[i] = __ldg(reinterpret_cast<const uint4*>(c.codes + id * c.page_stride +
+                                                      ((long long)(kv * c.kv_heads + h) * P + row % P) * D + 16 * cc));
+      }
+    };
+    // 16 dimensions of a position, from 16 cc on: chunks 2 cc and 2 cc + 1 of its row(s)
+    auto store = [&](uint8_t* base, int row, const uint4& codes, bool scaled, __half2 factor) {
+      uint32_t e[8];
+      expand<F>(codes.x, e[0], e[1]);
+      expand<F>(codes.y, e[2], e[3]);
+      expand<F>(codes.z, e[4], e[5]);
+      expand<F>(codes.w, e[6], e[7]);
+      if (scaled) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&e[k]), factor);
+          e[k] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+      }
+      uint8_t* at = base + cc / 4 * (kTile * 128) + row * 128;
+      const int ch = cc % 4 * 2;
+      *reinterpret_cast<uint4*>(at + ((ch ^ (row & 7)) * 16)) = make_uint4(e[0], e[1], e[2], e[3]);
+      *reinterpret_cast<uint4*>(at + (((ch + 1) ^ (row & 7)) * 16)) = make_uint4(e[4], e[5], e[6], e[7]);
+    };
+    Page now = page_of(first), next = page_of(first + 1);
+    uint4 kv[kPasses], vv[kPasses];
+    load(now, 0, kv);
+    load(now, 1, vv);
+    float vref = 0.f;
+    for (int j = first; j < last; ++j) {
+      const int st = (j - first) & 1;
+      const uint32_t phase = ((j - first) >> 1) & 1;
+      vref = fmaxf(vref, mk::warp_max(now.vs));
+      const bool whole = j * kTile >= all.lo_max && (j + 1) * kTile <= all.hi_min;
+      if (!wait_warp(&k_empty[st], phase ^ 1)) break;
+      if (ct < kSub) s_ks[j % kMetaSlots][ct] = now.ks;
+      if (ct == 0) s_vref[j % kMetaSlots] = vref;
+      uint8_t* kb = smem + S::kK + st * S::kOperand;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) store(kb, cr + i * kRowsPer, kv[i], false, __half2{});
+      fence_async_shared();
+      mk::mbar_arrive(&k_full[st]);
+      load(next, 0, kv);
+      if (!wait_warp(&v_empty[st], phase ^ 1)) break;
+      uint8_t* vb = smem + S::kV + st * S::kOperand;
+      const float inv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int row = cr + i * kRowsPer;
+        const float factor = __shfl_sync(0xffffffffu, now.vs, row / P) * inv;
+        if (!whole) {
+          // What no row sees may hold anything: its codes count as 0.  A NaN that
+          // only some rows see is taken out here and put back at the end.
+          uint32_t* u = reinterpret_cast<uint32_t*>(&vv[i]);
+          const int p = j * kTile + row;
+          const bool dead = p >= all.hi || p < all.lo;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (dead) u[k] = 0;
+            if constexpr (F::kTopExp == 8) {
+              const uint32_t bad = nan_bytes(u[k]);
+              if (bad) {
+                s_nan = 1;
+                u[k] &= ~((bad >> 7) * 0xffu);
+              }
+            }
+          }
+        }
+        store(vb, row, vv[i], factor != 1.f, __float2half2_rn(factor));
+      }
+      fence_async_shared();
+      mk::mbar_arrive(&v_full[st]);
+      load(next, 1, vv);
+      now = next;
+      next = page_of(j + 2);
+    }
+  } else if (lane == 0) {
+    // ---- tensor cores: one thread
+    constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, D, true);
+    bool ok = true;
+    uint32_t p_phase[2] = {0, 0};
+    auto scores = [&](int t, int st) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = k / 4 * (kTile * 128) + k % 4 * 32;
+        tc_mma_ss(t ? tm_s[1] : tm_s[0], mk::tc_desc_sw128(smem0 + S::kQ + t * S::kOperand + off),
+                  mk::tc_desc_sw128(smem0 + S::kK + st * S::kOperand + off), kS, k > 0);
+      }
+      mk::tc_commit(&s_full[t]);
+    };
+    auto in = [&](int t, int j) { return t ? j >= j_lo[1] && j < j_hi[1] : j >= j_lo[0] && j < j_hi[0]; };
+    if (first < last) {
+      ok = wait(&k_full[0], 0);
+      mk::tc_fence_after();
+      if (ok) {
+        if (in(0, first)) scores(0, 0);
+        if (in(1, first)) scores(1, 0);
+        mk::tc_commit(&k_empty[0]);
+      }
+    }
+    for (int j = first; ok && j < last; ++j) {
+      const int st = (j - first) & 1, st2 = st ^ 1;
+      const uint32_t phase = ((j - first) >> 1) & 1, phase2 = ((j + 1 - first) >> 1) & 1;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok) break;
+        if (in(t, j)) {
+          ok = wait(&p_full[t], p_phase[t]) && wait(&v_full[st], phase);
+          p_phase[t] ^= 1;
+          if (!ok) break;
+          mk::tc_fence_after();
+          const bool more = t ? j > j_lo[1] : j > j_lo[0];
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            tc_mma_ts(t ? tm_o[1] : tm_o[0], (t ? tm_s[1] : tm_s[0]) + k * 8,
+                      desc_n_major(smem0 + S::kV + st * S::kOperand + k * 2048, kTile * 128), kO, more || k > 0);
+          if (t ? j + 1 == j_hi[1] : j + 1 == j_hi[0]) mk::tc_commit(&o_full[t]);
+        }
+        if (j + 1 < last && in(t, j + 1)) {
+          ok = wait(&k_full[st2], phase2);
+          if (!ok) break;
+          mk::tc_fence_after();
+          scores(t, st2);
+        }
+      }
+      if (!ok) break;
+      mk::tc_commit(&v_empty[st]);
+      if (j + 1 < last) mk::tc_commit(&k_empty[st2]);
+    }
+    if (!ok) {   // nothing of this block's may be in flight when its memory is given away
+      report(a.status, MK_ERR_TIMEOUT);
+      mk::mbar_init(&k_full[0], 1);
+      mk::fence_mbar_init();
+      mk::tc_commit(&k_full[0]);
+      wait_bar(&k_full[0], 0);
+    }
+  }
+  __syncwarp();
+  mk::tc_fence_before();
+  __syncthreads();
+  if (warp == kRowWarps + kCodeWarps) {
+    mk::tmem_dealloc(tm, 512);
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------------
+
+template <class F, int P, int D>
+static int launch_prompt(const Cache& c, const Attend& a, cudaStream_t stream) {
+  constexpr int bytes = PromptSmem<D>::kBytes + 1024;
+  auto kernel = &attend_prompt_kernel<F, P, D>;
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return MK_ERR_CUDA;
+  if (!ready[dev].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return MK_ERR_CUDA;
+    ready[dev].store(true, std::memory_order_relaxed);
+  }
+  const int group = a.q_heads / c.kv_heads;
+  const long long blocks = ((long long)c.rows * group / (2 * kTile) + c.seqs) * c.kv_heads;
+  if (blocks > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
+  kernel<<<(unsigned)blocks, kPromptThreads, bytes, stream>>>(c, a);
+  return cudaGetLastError() == cudaSuccess ? MK_OK : MK_ERR_CUDA;
+}
+
+int attend_prompt(const Cache& c, const Attend& a, int format, int page_size, int head_dim, cudaStream_t stream) {
+  auto with_d = [&](auto f, auto p) {
+    using F = decltype(f);
+    constexpr int P = decltype(p)::value;
+    return head_dim == 64 ? launch_prompt<F, P, 64>(c, a, stream) : launch_prompt<F, P, 128>(c, a, stream);
+  };
+  auto with_p = [&](auto f) {
+    if (page_size == 16) return with_d(f, std::integral_constant<int, 16>{});
+    if (page_size == 32) return with_d(f, std::integral_constant<int, 32>{});
+    return with_d(f, std::integral_constant<int, 64>{});
+  };
+  return format == MK_KV8_E4M3 ? with_p(E4M3{}) : with_p(I8{});
+}
+
+}  // namespace mkp
