@@ -128,7 +128,7 @@ __device__ __forceinline__ void row_sees(const SeqWork& w, const Attend& a, int 
 // Whether a position that row index m sees holds a NaN code in dimension d of V.  Only
 // positions of steps that some row of the tile does not see wholly are looked at.
 template <class F, int P, int TS, int D>
-__device__ __noinline__ bool sees_nan(const Cache& c, const Attend& a, const SeqWork& w, int b, int h, int group, int tile_first,
+__device__ __forceinline__ bool sees_nan(const Cache& c, const Attend& a, const SeqWork& w, int b, int h, int group, int tile_first,
                                       int tile_last, int m, int d) {
   if (F::kTopExp != 8) return false;
   int lo, hi, lo_max, hi_min, x;

@@ -39,15 +39,25 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&v)[
         "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
-        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
-        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_f32x32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -57,7 +67,10 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 
 constexpr int kTile = 128;                       // rows of a query tile, positions of a step
 constexpr int kRowWarps = 8, kCodeWarps = 4;     // two query tiles; converters
-constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 1) * 32;
+constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 4) * 32;
+// Registers a thread of each role keeps (the block starts with 128 each): the sum
+// over the four warpgroups is the launch's 512.
+constexpr int kRowRegs = 184, kCodeRegs = 104, kMmaRegs = 40;
 constexpr int kMetaSlots = 4;
 
 template <int D>
@@ -69,10 +82,11 @@ struct PromptSmem {
 // ---- attention of many rows per sequence ---------------------------------------------------
 //
 // Work item: 256 rows of one (sequence, kv head), as two tiles of 128, all their
-// positions in steps of 128.  Roles of a block's 13 warps:
+// positions in steps of 128.  Roles of a block's four warpgroups:
 //   warps 0-3, 4-7   one tile of rows each, one row per thread: softmax
 //   warps 8-11       codes from global memory to f16 operands in shared memory
-//   warp 12          one thread issues every tcgen05.mma
+//   warp 12          one thread issues every tcgen05.mma (13-15 only give their
+//                    registers away)
 // S = Q K^T [128 x 128] and O [128 x D] live in tensor memory; the weights go
 // back to tensor memory as f16, over their scores, and are the A operand of
 // O += P V.  While one tile's scores are with its warps the tensor cores work
@@ -198,6 +212,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 
   if (warp < kRowWarps) {
     // ---- softmax of one row
+    mk::setmaxnreg_inc<kRowRegs>();
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;   // lanes 32 (warp % 4) ..
     const uint32_t ts = (x ? tm_s[1] : tm_s[0]) + quarter, to = (x ? tm_o[1] : tm_o[0]) + quarter;
     int lo, hi;
@@ -210,6 +225,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     for (int j = my_lo; j < my_hi; ++j, phase ^= 1) {
       if (!(ok = wait_warp(&s_full[x], phase))) break;
       mk::tc_fence_after();
+      float v[kTile];
+#pragma unroll
+      for (int c0 = 0; c0 < kTile; c0 += 32) tmem_ld_f32x32(ts + c0, v + c0);
       const int pos = j * kTile;
       float f[kSub];
       bool whole = pos >= lo_max && pos + kTile <= hi_min;
@@ -217,36 +235,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       for (int i = 0; i < kSub; ++i) {
         const float ks = s_ks[j % kMetaSlots][i];
         whole = whole && ks > 0.f;
-        f[i] = ks > 0.f ? fmaxf(rq * ks, 1.17549435e-38f) : 0.f;
+        f[i] = fmaxf(rq * ks, 1.17549435e-38f);   // -inf x 0 would be NaN
       }
       const float vnow = s_vref[j % kMetaSlots];
-      // hidden positions of 32 scores from column c0 on
-      auto hide = [&](float (&v)[32], int c0) {
+      mk::tmem_ld_wait();
+      if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int p = pos + c0 + i;
-          if (p < lo || p >= hi || f[(c0 + i) / P] == 0.f) v[i] = -INFINITY;
-        }
-      };
+        for (int i = 0; i < kTile; ++i)
+          if (pos + i < lo || pos + i >= hi || s_ks[j % kMetaSlots][i / P] == 0.f) v[i] = -INFINITY;
+      }
       float top = kNone;
 #pragma unroll
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t raw[32];
-        mk::tmem_ld_32x32b_x32(ts + c0, raw);
-        mk::tmem_ld_wait();
-        float v[32];
+      for (int i0 = 0; i0 < kTile; i0 += P) {
+        float t[2] = {v[i0], v[i0 + 1]};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-        if (!whole) hide(v, c0);
-        constexpr int kRun = P < 32 ? P : 32;
-#pragma unroll
-        for (int i0 = 0; i0 < 32; i0 += kRun) {
-          float t = v[i0];
-#pragma unroll
-          for (int i = 1; i < kRun; ++i) t = fmaxf(t, v[i0 + i]);
-          const float g = f[(c0 + i0) / P];
-          top = fmaxf(top, g == 0.f ? kNone : t * g);
+        for (int i = 2; i < P; i += 4) {
+          t[0] = fmaxf(fmaxf(t[0], v[i0 + i]), v[i0 + i + 1]);
+          if (i + 2 < P) t[1] = fmaxf(fmaxf(t[1], v[i0 + i + 2]), v[i0 + i + 3]);
         }
+        top = fmaxf(top, fmaxf(t[0], t[1]) * f[i0 / P]);
       }
       const bool move = top > m + kSlack;
       if (__any_sync(0xffffffffu, move) || vnow > vref) {
@@ -259,41 +266,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         }
         vref = vnow;
         if (j > my_lo) {   // P V of the step before is complete: its scores came after it
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            mk::tmem_ld_32x32b_x32(to + c0, o);
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld_x16(to + c0, o);
             mk::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-            tmem_st_x32(to + c0, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+            tmem_st_x16(to + c0, o);
           }
         }
       }
       const float back = 10.f - m;   // weights are 2^10 p
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t raw[32];
-        mk::tmem_ld_32x32b_x32(ts + c0, raw);
-        mk::tmem_ld_wait();
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-        if (!whole) hide(v, c0);
         uint32_t p[16];
-        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float g = f[(c0 + i) / P];
-          if (!whole) g = fmaxf(g, 1.17549435e-38f);   // -inf x 0 would be NaN
-          const float e0 = ex2(fmaf(v[i], g, back)), e1 = ex2(fmaf(v[i + 1], g, back));
-          sum[0] += e0;
-          sum[1] += e1;
+          const float g = f[(c0 + i) / P];
+          const float e0 = ex2(fmaf(v[c0 + i], g, back)), e1 = ex2(fmaf(v[c0 + i + 1], g, back));
+          sum[i & 2] += e0;
+          sum[(i & 2) + 1] += e1;
           p[i / 2] = pack_f16(e0, e1);
         }
-        l += sum[0] + sum[1];
         tmem_st_x16(ts + c0 / 2, p);
       }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       mk::tc_fence_before();
       mk::mbar_arrive(&p_full[x]);
@@ -304,34 +303,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       mk::tc_fence_after();
       const bool real = m_row <= row_last;
       const float inv = l == 0.f ? 0.f : vref / l;   // nothing seen: 0
-      const bool nan = s_nan != 0;
       const long long at = (long long)(w.r0 + m_row / group) * a.q_heads + h * group + m_row % group;
-#pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t o[32];
+      uint16_t* out = (uint16_t*)a.out + at * D;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 16) {
+        uint32_t o[16];
         if (my_hi > my_lo) {
-          mk::tmem_ld_32x32b_x32(to + c0, o);
+          tmem_ld_x16(to + c0, o);
           mk::tmem_ld_wait();
         }
         if (!real) continue;
-        uint4* out = reinterpret_cast<uint4*>((uint16_t*)a.out + at * D + c0);
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          float v[8];
+        for (int i = 0; i < 16; ++i) o[i] = my_hi > my_lo && l != 0.f ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
+        uint32_t y[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            v[k] = my_hi > my_lo && l != 0.f ? __uint_as_float(o[i + k]) * inv : 0.f;
-            if (nan && sees_nan<F, P, kTile, D>(c, a, w, b, h, group, row0, row_last, m_row, c0 + i + k))
-              v[k] = __int_as_float(0x7fffffff);
-          }
-          out[i / 8] = make_uint4(pack_out(v[0], v[1], a.bf16), pack_out(v[2], v[3], a.bf16), pack_out(v[4], v[5], a.bf16),
-                                  pack_out(v[6], v[7], a.bf16));
-        }
+        for (int i = 0; i < 8; ++i) y[i] = pack_out(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]), a.bf16);
+        *reinterpret_cast<uint4*>(out + c0) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(out + c0 + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+      if (real && s_nan) {
+#pragma unroll 1
+        for (int d = 0; d < D; ++d)
+          if (sees_nan<F, P, kTile, D>(c, a, w, b, h, group, row0, row_last, m_row, d))
+            out[d] = 0x7fff;   // NaN in bf16 and in f16
       }
       if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - 10.f + log2f(l)) * 0.6931471805599453f;
     }
   } else if (warp < kRowWarps + kCodeWarps) {
     // ---- codes to f16
+    mk::setmaxnreg_dec<kCodeRegs>();
     constexpr int kLanes = D / 16, kRowsPer = kCodeWarps * 32 / kLanes, kPasses = kTile / kRowsPer;
     const int ct = threadIdx.x - kRowWarps * 32, cc = ct % kLanes, cr = ct / kLanes;
     struct Page { int id; float ks, vs; };
@@ -375,8 +375,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       }
       uint8_t* at = base + cc / 4 * (kTile * 128) + row * 128;
       const int ch = cc % 4 * 2;
-      *reinterpret_cast<uint4*>(at + ((ch ^ (row & 7)) * 16)) = make_uint4(e[0], e[1], e[2], e[3]);
-      *reinterpret_cast<uint4*>(at + (((ch + 1) ^ (row & 7)) * 16)) = make_uint4(e[4], e[5], e[6], e[7]);
+      // odd chunks first in the second half of a row: eight lanes, eight banks
+      const bool odd = cc >= 4;
+      const uint4 even4 = make_uint4(e[0], e[1], e[2], e[3]), odd4 = make_uint4(e[4], e[5], e[6], e[7]);
+      *reinterpret_cast<uint4*>(at + (((ch + odd) ^ (row & 7)) * 16)) = odd ? odd4 : even4;
+      *reinterpret_cast<uint4*>(at + (((ch + !odd) ^ (row & 7)) * 16)) = odd ? even4 : odd4;
     };
     Page now = page_of(first), next = page_of(first + 1);
     uint4 kv[kPasses], vv[kPasses];
@@ -430,7 +433,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       now = next;
       next = page_of(j + 2);
     }
-  } else if (lane == 0) {
+  } else {
+    mk::setmaxnreg_dec<kMmaRegs>();
+    if (warp == kRowWarps + kCodeWarps && lane == 0) {
     // ---- tensor cores: one thread
     constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, D, true);
     bool ok = true;
@@ -489,6 +494,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       mk::fence_mbar_init();
       mk::tc_commit(&k_full[0]);
       wait_bar(&k_full[0], 0);
+    }
     }
   }
   __syncwarp();
