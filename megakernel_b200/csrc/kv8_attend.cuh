@@ -71,6 +71,12 @@ constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kNone = -1e30f;        // running reference of a row that has seen nothing
 constexpr float kSlack = 5.f;          // weights may reach 2^kSlack before the reference moves
 
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+
 // Bounded wait; each probe may itself suspend for a while.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < kWaitLimit; ++i)

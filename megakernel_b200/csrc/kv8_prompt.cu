@@ -66,27 +66,32 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 // ---- layout ------------------------------------------------------------------------------
 
 constexpr int kTile = 128;                       // rows of a query tile, positions of a step
-constexpr int kRowWarps = 8, kCodeWarps = 4;     // two query tiles; converters
+constexpr int kRowWarps = 8, kCodeWarps = 8;     // two query tiles; converters
+constexpr int kMmaWarp = kRowWarps + kCodeWarps, kCopyWarp = kMmaWarp + 1;
 constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 4) * 32;
-// Registers a thread of each role keeps (the block starts with 128 each): the sum
-// over the four warpgroups is the launch's 512.
-constexpr int kRowRegs = 184, kCodeRegs = 104, kMmaRegs = 40;
-constexpr int kMetaSlots = 4;
+// Registers a thread of each role keeps; the block starts with 96 each, and the
+// sum over the five warpgroups is the launch's 480.
+constexpr int kRowRegs = 168, kCodeRegs = 56, kMmaRegs = 32;
+constexpr int kMetaSlots = 8;   // the copies run at most five steps ahead of the softmax
 
 template <int D>
 struct PromptSmem {
   static constexpr int kOperand = kTile * D * 2;                 // Q tile, K or V step in f16
-  static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kBytes = 6 * kOperand;
+  static constexpr int kCodes = kTile * D;                       // K or V codes of a step
+  static constexpr int kStages = D == 64 ? 2 : 1;                // of codes; what shared memory leaves room for
+  static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kRaw = 6 * kOperand;
+  static constexpr int kBytes = kRaw + 2 * kStages * kCodes;
 };
 
 // ---- attention of many rows per sequence ---------------------------------------------------
 //
 // Work item: 256 rows of one (sequence, kv head), as two tiles of 128, all their
-// positions in steps of 128.  Roles of a block's four warpgroups:
+// positions in steps of 128.  Roles of a block's five warpgroups:
 //   warps 0-3, 4-7   one tile of rows each, one row per thread: softmax
-//   warps 8-11       codes from global memory to f16 operands in shared memory
-//   warp 12          one thread issues every tcgen05.mma (13-15 only give their
-//                    registers away)
+//   warps 8-15       8-bit codes to f16 operands, shared memory to shared memory
+//   warp 16          one thread issues every tcgen05.mma
+//   warp 17          looks pages and scales up and copies their codes to shared
+//                    memory (18 and 19 only give their registers away)
 // S = Q K^T [128 x 128] and O [128 x D] live in tensor memory; the weights go
 // back to tensor memory as f16, over their scores, and are the A operand of
 // O += P V.  While one tile's scores are with its warps the tensor cores work
@@ -105,7 +110,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
-  __shared__ float s_ks[kMetaSlots][kSub], s_vref[kMetaSlots];
+  __shared__ __align__(8) uint64_t raw_full[2][S::kStages], raw_empty[2][S::kStages];   // codes of K, of V
+  // of a step: scales of the K pages (0: not there), of the V pages relative to
+  // s_vref, the largest V scale up to it; whether all its pages are there
+  __shared__ float s_ks[kMetaSlots][kSub], s_vf[kMetaSlots][kSub], s_vref[kMetaSlots];
+  __shared__ int s_there[kMetaSlots];
   __shared__ uint32_t s_tmem;
   __shared__ int s_nan;
   __shared__ volatile int s_abort;
@@ -153,10 +162,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       mk::mbar_init(&s_full[i], 1);
       mk::mbar_init(&p_full[i], 128);
       mk::mbar_init(&o_full[i], 1);
+      for (int k = 0; k < S::kStages; ++k) {
+        mk::mbar_init(&raw_full[i][k], kSub);
+        mk::mbar_init(&raw_empty[i][k], kCodeWarps);
+      }
     }
     mk::fence_mbar_init();
   }
-  if (warp == kRowWarps + kCodeWarps) {
+  if (warp == kMmaWarp) {
     mk::tmem_alloc(&s_tmem, 512);
     mk::tmem_relinquish();
   }
@@ -332,33 +345,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   } else if (warp < kRowWarps + kCodeWarps) {
     // ---- codes to f16
     mk::setmaxnreg_dec<kCodeRegs>();
-    constexpr int kLanes = D / 16, kRowsPer = kCodeWarps * 32 / kLanes, kPasses = kTile / kRowsPer;
+    constexpr int kLanes = D / 16, kRowsPer = kCodeWarps * 32 / kLanes;
     const int ct = threadIdx.x - kRowWarps * 32, cc = ct % kLanes, cr = ct / kLanes;
-    struct Page { int id; float ks, vs; };
-    auto page_of = [&](int j) {   // lane i: page i of step j
-      Page p{-1, 0.f, 0.f};
-      const int pos = j * kTile + lane * P;
-      if (j < last && lane < kSub && pos < all.hi && pos + P > all.lo) {
-        p.id = page_id(c, b, pos / P, a.status);
-        if (p.id >= 0) {
-          const float* sc = c.scales + p.id * c.scale_stride + h;
-          p.ks = fmaxf(__ldg(sc), 1.17549435e-38f);
-          p.vs = __ldg(sc + c.kv_heads);
-        }
-      }
-      return p;
-    };
-    auto load = [&](const Page& p, int kv, uint4 (&v)[kPasses]) {
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int row = cr + i * kRowsPer;
-        const int id = __shfl_sync(0xffffffffu, p.id, row / P);
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (id >= 0)
-          v[i] = __ldg(reinterpret_cast<const uint4*>(c.codes + id * c.page_stride +
-                                                      ((long long)(kv * c.kv_heads + h) * P + row % P) * D + 16 * cc));
-      }
-    };
     // 16 dimensions of a position, from 16 cc on: chunks 2 cc and 2 cc + 1 of its row(s)
     auto store = [&](uint8_t* base, int row, const uint4& codes, bool scaled, __half2 factor) {
       uint32_t e[8];
@@ -381,61 +369,109 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       *reinterpret_cast<uint4*>(at + (((ch + odd) ^ (row & 7)) * 16)) = odd ? odd4 : even4;
       *reinterpret_cast<uint4*>(at + (((ch + !odd) ^ (row & 7)) * 16)) = odd ? even4 : odd4;
     };
-    Page now = page_of(first), next = page_of(first + 1);
-    uint4 kv[kPasses], vv[kPasses];
-    load(now, 0, kv);
-    load(now, 1, vv);
-    float vref = 0.f;
     for (int j = first; j < last; ++j) {
-      const int st = (j - first) & 1;
-      const uint32_t phase = ((j - first) >> 1) & 1;
-      vref = fmaxf(vref, mk::warp_max(now.vs));
-      const bool whole = j * kTile >= all.lo_max && (j + 1) * kTile <= all.hi_min;
-      if (!wait_warp(&k_empty[st], phase ^ 1)) break;
-      if (ct < kSub) s_ks[j % kMetaSlots][ct] = now.ks;
-      if (ct == 0) s_vref[j % kMetaSlots] = vref;
-      uint8_t* kb = smem + S::kK + st * S::kOperand;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) store(kb, cr + i * kRowsPer, kv[i], false, __half2{});
+      const int i = j - first, st = i & 1, raw = i % S::kStages;
+      const uint32_t phase = (i >> 1) & 1, raw_phase = (i / S::kStages) & 1;
+      // K
+      if (!wait_warp(&raw_full[0][raw], raw_phase) || !wait_warp(&k_empty[st], phase ^ 1)) break;
+      const uint8_t* src = smem + S::kRaw + raw * S::kCodes + 16 * cc;
+      uint8_t* dst = smem + S::kK + st * S::kOperand;
+#pragma unroll 2
+      for (int row = cr; row < kTile; row += kRowsPer)
+        store(dst, row, *reinterpret_cast<const uint4*>(src + row * D), false, __half2{});
       fence_async_shared();
       mk::mbar_arrive(&k_full[st]);
-      load(next, 0, kv);
-      if (!wait_warp(&v_empty[st], phase ^ 1)) break;
-      uint8_t* vb = smem + S::kV + st * S::kOperand;
-      const float inv = vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int row = cr + i * kRowsPer;
-        const float factor = __shfl_sync(0xffffffffu, now.vs, row / P) * inv;
+      __syncwarp();
+      if (lane == 0) mk::mbar_arrive(&raw_empty[0][raw]);
+      // V
+      const bool whole = s_there[j % kMetaSlots] && j * kTile >= all.lo_max && (j + 1) * kTile <= all.hi_min;
+      if (!wait_warp(&raw_full[1][raw], raw_phase) || !wait_warp(&v_empty[st], phase ^ 1)) break;
+      src += S::kStages * S::kCodes;
+      dst = smem + S::kV + st * S::kOperand;
+#pragma unroll 2
+      for (int row = cr; row < kTile; row += kRowsPer) {
+        uint4 v = *reinterpret_cast<const uint4*>(src + row * D);
+        const float factor = s_vf[j % kMetaSlots][row / P];
         if (!whole) {
           // What no row sees may hold anything: its codes count as 0.  A NaN that
           // only some rows see is taken out here and put back at the end.
-          uint32_t* u = reinterpret_cast<uint32_t*>(&vv[i]);
           const int p = j * kTile + row;
-          const bool dead = p >= all.hi || p < all.lo;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (dead) u[k] = 0;
-            if constexpr (F::kTopExp == 8) {
-              const uint32_t bad = nan_bytes(u[k]);
-              if (bad) {
-                s_nan = 1;
-                u[k] &= ~((bad >> 7) * 0xffu);
-              }
+          if (p >= all.hi || p < all.lo || s_ks[j % kMetaSlots][row / P] == 0.f) v = make_uint4(0, 0, 0, 0);
+          if constexpr (F::kTopExp == 8) {
+            const uint32_t b0 = nan_bytes(v.x), b1 = nan_bytes(v.y), b2 = nan_bytes(v.z), b3 = nan_bytes(v.w);
+            if (b0 | b1 | b2 | b3) {
+              s_nan = 1;
+              v.x &= ~((b0 >> 7) * 0xffu);
+              v.y &= ~((b1 >> 7) * 0xffu);
+              v.z &= ~((b2 >> 7) * 0xffu);
+              v.w &= ~((b3 >> 7) * 0xffu);
             }
           }
         }
-        store(vb, row, vv[i], factor != 1.f, __float2half2_rn(factor));
+        store(dst, row, v, factor != 1.f, __float2half2_rn(factor));
       }
       fence_async_shared();
       mk::mbar_arrive(&v_full[st]);
-      load(next, 1, vv);
-      now = next;
-      next = page_of(j + 2);
+      __syncwarp();
+      if (lane == 0) mk::mbar_arrive(&raw_empty[1][raw]);
     }
   } else {
     mk::setmaxnreg_dec<kMmaRegs>();
-    if (warp == kRowWarps + kCodeWarps && lane == 0) {
+    if (warp == kCopyWarp) {
+      // ---- pages and copies: lane i, page i of a step
+      struct Page { int id; float ks, vs; };
+      auto page_of = [&](int j) {
+        Page p{-1, 0.f, 0.f};
+        const int pos = j * kTile + lane * P;
+        if (j < last && lane < kSub && pos < all.hi && pos + P > all.lo) {
+          p.id = page_id(c, b, pos / P, a.status);
+          if (p.id >= 0) {
+            const float* sc = c.scales + p.id * c.scale_stride + h;
+            p.ks = fmaxf(__ldg(sc), 1.17549435e-38f);
+            p.vs = __ldg(sc + c.kv_heads);
+          }
+        }
+        return p;
+      };
+      // rows of one sequence and head share the codes with its other items
+      const uint64_t policy = w.tiles > 1 ? policy_evict_normal() : mk::policy_evict_first();
+      Page now = page_of(first), next = page_of(first + 1);
+      float vref = 0.f;
+      bool ok = true;
+      int done = first;
+      for (int j = first; ok && j < last; ++j) {
+        const int i = j - first, raw = i % S::kStages;
+        const uint32_t phase = (i / S::kStages) & 1;
+        vref = fmaxf(vref, mk::warp_max(now.vs));
+        const bool there = __all_sync(0xffffffffu, lane >= kSub || now.id >= 0);
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!(ok = wait_warp(&raw_empty[kv][raw], phase ^ 1))) break;
+          if (lane < kSub) {
+            if (kv == 0) {
+              s_ks[j % kMetaSlots][lane] = now.ks;
+              s_vf[j % kMetaSlots][lane] = vref > 0.f ? now.vs / vref : 0.f;
+              if (lane == 0) {
+                s_vref[j % kMetaSlots] = vref;
+                s_there[j % kMetaSlots] = there;
+              }
+            }
+            mk::mbar_arrive_expect_tx(&raw_full[kv][raw], now.id >= 0 ? P * D : 0);
+            if (now.id >= 0)
+              mk::bulk_g2s(smem + S::kRaw + (kv * S::kStages + raw) * S::kCodes + lane * P * D,
+                           c.codes + now.id * c.page_stride + (long long)(kv * c.kv_heads + h) * P * D, P * D,
+                           &raw_full[kv][raw], policy);
+          }
+          __syncwarp();
+          if (kv == 0) done = j + 1;
+        }
+        now = next;
+        next = page_of(j + 2);
+      }
+      // no copy in flight when the block's memory is given away
+      for (int j = max(first, done - S::kStages); j < done; ++j)
+        for (int kv = 0; kv < 2; ++kv) wait_bar(&raw_full[kv][(j - first) % S::kStages], ((j - first) / S::kStages) & 1);
+    }
+    if (warp == kMmaWarp && lane == 0) {
     // ---- tensor cores: one thread
     constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, D, true);
     bool ok = true;
@@ -500,7 +536,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   __syncwarp();
   mk::tc_fence_before();
   __syncthreads();
-  if (warp == kRowWarps + kCodeWarps) {
+  if (warp == kMmaWarp) {
     mk::tmem_dealloc(tm, 512);
   }
 }
