@@ -8,29 +8,50 @@ namespace mkp {
 
 // ---- tcgen05 pieces -------------------------------------------------------------------
 
-// D[tmem] (+)= A[smem] B[smem], f16 in, fp32 accumulate (kind::f16 with f16 operands).
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-  mk::tc_mma_bf16(d, adesc, bdesc, idesc, accumulate);   // the operand types are idesc's
+// One lane of the (converged) warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+// D[tmem] (+)= A[smem] B[smem], f16 in, fp32 accumulate, by the thread with `one`.
+// Descriptors by halves: the upper one (strides, swizzle) is a constant, the lower
+// one moves with k.  The whole warp comes here, so that the operands stay in
+// uniform registers: in a branch of one thread each product took some 100 cycles to issue.
+__device__ __forceinline__ void tc_mma_ss(uint32_t one, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\tmov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
 }
 // The same with A in tensor memory: 128 lanes, two f16 per 32-bit column.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t one, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 y;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\tmov.b64 y, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(one)
       : "memory");
+}
+__device__ __forceinline__ void tc_commit_one(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(mk::smem_u32(bar)), "r"(one) : "memory");
 }
 // f16 A and B, fp32 D, M x N; b_mn: B is stored with N contiguous.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// Operand of 64-element rows of 128 bytes, 128-byte swizzle, 8-row groups 1,024 bytes
-// apart: K contiguous (K-major), or N contiguous with the next 64 of N `next`
-// bytes on.
-__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr, uint32_t next) {
-  return (mk::tc_desc_sw128(addr) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)((next >> 4) & 0x3fff) << 16);
-}
+// Descriptor of an operand of 64-element rows of 128 bytes, 128-byte swizzle, 8-row
+// groups 1,024 bytes apart (mk::tc_desc_sw128): K contiguous, or N contiguous with
+// the next 64 of N `next` bytes on.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t next = 16) { return (addr >> 4 & 0x3fffu) | (next >> 4) << 16; }
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -60,6 +81,33 @@ __device__ __forceinline__ void tmem_ld_f32x32(uint32_t taddr, float* v) {
       : "r"(taddr)
       : "memory");
 }
+// tcgen05.wait::ld, as what makes the loaded registers: nothing that uses them can
+// be placed before it.
+__device__ __forceinline__ void tmem_arrived(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+        "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+        "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+        "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+        "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+      ::"memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+        "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+      ::"memory");
+}
+// Pairs of fp32 operations in one instruction: (x, y) = (x, y) f + b, (x, y) += (u, v).
+__device__ __forceinline__ void fma2(float& x, float& y, float f, float b) {
+  asm("{\n\t.reg .b64 u, g, c;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 g, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+      "fma.rn.f32x2 u, u, g, c;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "+f"(x), "+f"(y) : "f"(f), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float u, float v) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y) : "f"(u), "f"(v));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -78,8 +126,8 @@ template <int D>
 struct PromptSmem {
   static constexpr int kOperand = kTile * D * 2;                 // Q tile, K or V step in f16
   static constexpr int kCodes = kTile * D;                       // K or V codes of a step
-  static constexpr int kStages = D == 64 ? 2 : 1;                // of codes; what shared memory leaves room for
-  static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kRaw = 6 * kOperand;
+  static constexpr int kStages = 2;                              // of codes
+  static constexpr int kQ = 0, kK = 2 * kOperand, kV = 3 * kOperand, kRaw = 5 * kOperand;
   static constexpr int kBytes = kRaw + 2 * kStages * kCodes;
 };
 
@@ -89,14 +137,14 @@ struct PromptSmem {
 // positions in steps of 128.  Roles of a block's five warpgroups:
 //   warps 0-3, 4-7   one tile of rows each, one row per thread: softmax
 //   warps 8-15       8-bit codes to f16 operands, shared memory to shared memory
-//   warp 16          one thread issues every tcgen05.mma
+//   warp 16          one lane issues every tcgen05.mma
 //   warp 17          looks pages and scales up and copies their codes to shared
 //                    memory (18 and 19 only give their registers away)
 // S = Q K^T [128 x 128] and O [128 x D] live in tensor memory; the weights go
 // back to tensor memory as f16, over their scores, and are the A operand of
 // O += P V.  While one tile's scores are with its warps the tensor cores work
-// for the other.  Two steps of K and of V are in shared memory at once, each
-// converted once for both tiles.
+// for the other.  A step of K and two of V are in shared memory as f16,
+// each converted once for both tiles, and two steps of codes before them.
 //
 // Softmax and scales as in kv8_attend.cu: a reference m per row that moves only
 // when some weight would pass 2^5, weights 2^10 p in f16; the scale of a K page
@@ -109,7 +157,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   constexpr int kSub = kTile / P;                    // pages of a step
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+  __shared__ __align__(8) uint64_t k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
   __shared__ __align__(8) uint64_t raw_full[2][S::kStages], raw_empty[2][S::kStages];   // codes of K, of V
   // of a step: scales of the K pages (0: not there), of the V pages relative to
   // s_vref, the largest V scale up to it; whether all its pages are there
@@ -154,10 +202,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   if (threadIdx.x == 0) {
     s_nan = 0;
     s_abort = 0;
+    mk::mbar_init(&k_full, kCodeWarps * 32);
+    mk::mbar_init(&k_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mk::mbar_init(&k_full[i], kCodeWarps * 32);
       mk::mbar_init(&v_full[i], kCodeWarps * 32);
-      mk::mbar_init(&k_empty[i], 1);
       mk::mbar_init(&v_empty[i], 1);
       mk::mbar_init(&s_full[i], 1);
       mk::mbar_init(&p_full[i], 128);
@@ -238,36 +286,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     for (int j = my_lo; j < my_hi; ++j, phase ^= 1) {
       if (!(ok = wait_warp(&s_full[x], phase))) break;
       mk::tc_fence_after();
-      float v[kTile];
-#pragma unroll
-      for (int c0 = 0; c0 < kTile; c0 += 32) tmem_ld_f32x32(ts + c0, v + c0);
-      const int pos = j * kTile;
+      const int pos = j * kTile, slot = j % kMetaSlots;
+      const bool whole = s_there[slot] && pos >= lo_max && pos + kTile <= hi_min;
+      // The scores stay in registers: tensor memory gives an SM about 128 bytes a
+      // cycle, and reading them a second time took 70 us of 515 a call.
+      float v[4][32];
       float f[kSub];
-      bool whole = pos >= lo_max && pos + kTile <= hi_min;
 #pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        const float ks = s_ks[j % kMetaSlots][i];
-        whole = whole && ks > 0.f;
-        f[i] = fmaxf(rq * ks, 1.17549435e-38f);   // -inf x 0 would be NaN
-      }
-      const float vnow = s_vref[j % kMetaSlots];
-      mk::tmem_ld_wait();
-      if (!whole) {
+      for (int i = 0; i < kSub; ++i) f[i] = fmaxf(rq * s_ks[slot][i], 1.17549435e-38f);   // -inf x 0 would be NaN
+      tmem_ld_f32x32(ts, v[0]);
+      tmem_arrived(v[0]);
 #pragma unroll
-        for (int i = 0; i < kTile; ++i)
-          if (pos + i < lo || pos + i >= hi || s_ks[j % kMetaSlots][i / P] == 0.f) v[i] = -INFINITY;
-      }
+      for (int q = 1; q < 4; ++q) tmem_ld_f32x32(ts + 32 * q, v[q]);
       float top = kNone;
 #pragma unroll
-      for (int i0 = 0; i0 < kTile; i0 += P) {
-        float t[2] = {v[i0], v[i0 + 1]};
+      for (int q = 0; q < 4; ++q) {
+        if (q > 0) tmem_arrived(v[q]);
+        if (!whole) {
 #pragma unroll
-        for (int i = 2; i < P; i += 4) {
-          t[0] = fmaxf(fmaxf(t[0], v[i0 + i]), v[i0 + i + 1]);
-          if (i + 2 < P) t[1] = fmaxf(fmaxf(t[1], v[i0 + i + 2]), v[i0 + i + 3]);
+          for (int i = 0; i < 32; ++i)
+            if (pos + 32 * q + i < lo || pos + 32 * q + i >= hi || s_ks[slot][(32 * q + i) / P] == 0.f) v[q][i] = -INFINITY;
         }
-        top = fmaxf(top, fmaxf(t[0], t[1]) * f[i0 / P]);
+        constexpr int kRun = P < 32 ? P : 32;   // columns of one page
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += kRun) {
+          float t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = fmaxf(fmaxf(v[q][i0 + i], v[q][i0 + 4 + i]), v[q][i0 + 8 + i]);
+#pragma unroll
+          for (int i = 12; i < kRun; ++i) t[i & 3] = fmaxf(t[i & 3], v[q][i0 + i]);
+          top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f[(32 * q + i0) / P]);
+        }
       }
+      const float vnow = s_vref[slot];
       const bool move = top > m + kSlack;
       if (__any_sync(0xffffffffu, move) || vnow > vref) {
         float keep = vnow > vref ? vref / vnow : 1.f;
@@ -283,7 +334,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           for (int c0 = 0; c0 < D; c0 += 16) {
             uint32_t o[16];
             tmem_ld_x16(to + c0, o);
-            mk::tmem_ld_wait();
+            tmem_arrived(o);
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
             tmem_st_x16(to + c0, o);
@@ -293,17 +344,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       const float back = 10.f - m;   // weights are 2^10 p
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
+      for (int q = 0; q < 4; ++q) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float g = f[(c0 + i) / P];
-          const float e0 = ex2(fmaf(v[c0 + i], g, back)), e1 = ex2(fmaf(v[c0 + i + 1], g, back));
-          sum[i & 2] += e0;
-          sum[(i & 2) + 1] += e1;
+          fma2(v[q][i], v[q][i + 1], f[(32 * q + i) / P], back);
+          const float e0 = ex2(v[q][i]), e1 = ex2(v[q][i + 1]);
+          add2(sum[i & 2], sum[(i & 2) + 1], e0, e1);
           p[i / 2] = pack_f16(e0, e1);
         }
-        tmem_st_x16(ts + c0 / 2, p);
+        tmem_st_x16(ts + 16 * q, p);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
@@ -323,7 +373,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         uint32_t o[16];
         if (my_hi > my_lo) {
           tmem_ld_x16(to + c0, o);
-          mk::tmem_ld_wait();
+          tmem_arrived(o);
         }
         if (!real) continue;
 #pragma unroll
@@ -373,14 +423,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       const int i = j - first, st = i & 1, raw = i % S::kStages;
       const uint32_t phase = (i >> 1) & 1, raw_phase = (i / S::kStages) & 1;
       // K
-      if (!wait_warp(&raw_full[0][raw], raw_phase) || !wait_warp(&k_empty[st], phase ^ 1)) break;
+      if (!wait_warp(&raw_full[0][raw], raw_phase) || !wait_warp(&k_empty, (i & 1) ^ 1)) break;
       const uint8_t* src = smem + S::kRaw + raw * S::kCodes + 16 * cc;
-      uint8_t* dst = smem + S::kK + st * S::kOperand;
+      uint8_t* dst = smem + S::kK;
 #pragma unroll 2
       for (int row = cr; row < kTile; row += kRowsPer)
         store(dst, row, *reinterpret_cast<const uint4*>(src + row * D), false, __half2{});
       fence_async_shared();
-      mk::mbar_arrive(&k_full[st]);
+      mk::mbar_arrive(&k_full);
       __syncwarp();
       if (lane == 0) mk::mbar_arrive(&raw_empty[0][raw]);
       // V
@@ -471,66 +521,71 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       for (int j = max(first, done - S::kStages); j < done; ++j)
         for (int kv = 0; kv < 2; ++kv) wait_bar(&raw_full[kv][(j - first) % S::kStages], ((j - first) / S::kStages) & 1);
     }
-    if (warp == kMmaWarp && lane == 0) {
-    // ---- tensor cores: one thread
-    constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, D, true);
-    bool ok = true;
-    uint32_t p_phase[2] = {0, 0};
-    auto scores = [&](int t, int st) {
+    if (warp == kMmaWarp) {
+      // ---- tensor cores: every product issued by one lane
+      constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, D, true);
+      const uint32_t one = elect_one();
+      const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0), smu = __shfl_sync(0xffffffffu, smem0, 0);
+      const int nj = last - first;
+      bool ok = true;
+      uint32_t p_phase = 0;   // bit t: of tile t
+      auto in = [&](int t, int j) { return t ? j >= j_lo[1] && j < j_hi[1] : j >= j_lo[0] && j < j_hi[0]; };
+      auto scores = [&](int t) {
+        const uint32_t qa = desc_lo(smu + S::kQ) + t * (S::kOperand >> 4), ka = desc_lo(smu + S::kK), d = tmu + t * kTile;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = k / 4 * (kTile * 128) + k % 4 * 32;
-        tc_mma_ss(t ? tm_s[1] : tm_s[0], mk::tc_desc_sw128(smem0 + S::kQ + t * S::kOperand + off),
-                  mk::tc_desc_sw128(smem0 + S::kK + st * S::kOperand + off), kS, k > 0);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (uint32_t)(k >> 2) * (kTile * 128 >> 4) + (k & 3) * 2;
+          tc_mma_ss(one, d, qa + off, ka + off, kDescHi, kS, k > 0);
+        }
+        tc_commit_one(one, &s_full[t]);
+      };
+      if (nj > 0) {
+        ok = wait_warp(&k_full, 0);
+        mk::tc_fence_after();
+        if (ok) {
+#pragma unroll 1
+          for (int t = 0; t < 2; ++t)
+            if (in(t, first)) scores(t);
+          tc_commit_one(one, &k_empty);
+        }
       }
-      mk::tc_commit(&s_full[t]);
-    };
-    auto in = [&](int t, int j) { return t ? j >= j_lo[1] && j < j_hi[1] : j >= j_lo[0] && j < j_hi[0]; };
-    if (first < last) {
-      ok = wait(&k_full[0], 0);
-      mk::tc_fence_after();
-      if (ok) {
-        if (in(0, first)) scores(0, 0);
-        if (in(1, first)) scores(1, 0);
-        mk::tc_commit(&k_empty[0]);
-      }
-    }
-    for (int j = first; ok && j < last; ++j) {
-      const int st = (j - first) & 1, st2 = st ^ 1;
-      const uint32_t phase = ((j - first) >> 1) & 1, phase2 = ((j + 1 - first) >> 1) & 1;
+#pragma unroll 1
+      for (int i = 0; ok && i < nj; ++i) {
+        const int j = first + i, st = i & 1;
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          if (in(t, j)) {
+            ok = wait_warp(&p_full[t], p_phase >> t & 1) && wait_warp(&v_full[st], i >> 1 & 1);
+            p_phase ^= 1u << t;
+            if (!ok) break;
+            mk::tc_fence_after();
+            const uint32_t more = j > (t ? j_lo[1] : j_lo[0]);
+            const uint32_t va = desc_lo(smu + S::kV, kTile * 128) + st * (S::kOperand >> 4), pa = tmu + t * kTile, d = tmu + 2 * kTile + t * D;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+            for (int k = 0; k < kTile / 16; ++k) tc_mma_ts(one, d, pa + k * 8, va + k * (2048 >> 4), kDescHi, kO, k > 0 ? 1u : more);
+            if (j + 1 == (t ? j_hi[1] : j_hi[0])) tc_commit_one(one, &o_full[t]);
+          }
+          if (i + 1 < nj && in(t, j + 1)) {
+            ok = wait_warp(&k_full, (i + 1) & 1);
+            if (!ok) break;
+            mk::tc_fence_after();
+            scores(t);
+          }
+        }
         if (!ok) break;
-        if (in(t, j)) {
-          ok = wait(&p_full[t], p_phase[t]) && wait(&v_full[st], phase);
-          p_phase[t] ^= 1;
-          if (!ok) break;
-          mk::tc_fence_after();
-          const bool more = t ? j > j_lo[1] : j > j_lo[0];
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            tc_mma_ts(t ? tm_o[1] : tm_o[0], (t ? tm_s[1] : tm_s[0]) + k * 8,
-                      desc_n_major(smem0 + S::kV + st * S::kOperand + k * 2048, kTile * 128), kO, more || k > 0);
-          if (t ? j + 1 == j_hi[1] : j + 1 == j_hi[0]) mk::tc_commit(&o_full[t]);
-        }
-        if (j + 1 < last && in(t, j + 1)) {
-          ok = wait(&k_full[st2], phase2);
-          if (!ok) break;
-          mk::tc_fence_after();
-          scores(t, st2);
-        }
+        tc_commit_one(one, &v_empty[st]);
+        if (i + 1 < nj) tc_commit_one(one, &k_empty);
       }
-      if (!ok) break;
-      mk::tc_commit(&v_empty[st]);
-      if (j + 1 < last) mk::tc_commit(&k_empty[st2]);
-    }
-    if (!ok) {   // nothing of this block's may be in flight when its memory is given away
-      report(a.status, MK_ERR_TIMEOUT);
-      mk::mbar_init(&k_full[0], 1);
-      mk::fence_mbar_init();
-      mk::tc_commit(&k_full[0]);
-      wait_bar(&k_full[0], 0);
-    }
+      if (!ok) {   // nothing of this block's may be in flight when its memory is given away
+        if (one) {
+          report(a.status, MK_ERR_TIMEOUT);
+          mk::mbar_init(&k_full, 1);
+          mk::fence_mbar_init();
+          mk::tc_commit(&k_full);
+          wait_bar(&k_full, 0);
+        }
+        __syncwarp();
+      }
     }
   }
   __syncwarp();
