@@ -119,7 +119,11 @@ constexpr int kMmaWarp = kRowWarps + kCodeWarps, kCopyWarp = kMmaWarp + 1;
 constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 4) * 32;
 // Registers a thread of each role keeps; the block starts with 96 each, and the
 // sum over the five warpgroups is the launch's 480.
-constexpr int kRowRegs = 168, kCodeRegs = 56, kMmaRegs = 32;
+constexpr int kRowRegs = 168, kCodeRegs = 48, kMmaRegs = 48;
+// Weights 2^kBase p in f16, p up to 2^kMove: the reference moves less often than in
+// kv8_attend.cu (a move costs a pass over the output), and what is lost below is
+// 2^-31 of the row's reference.
+constexpr float kBase = 6.f, kMove = 9.f;
 constexpr int kMetaSlots = 8;   // the copies run at most five steps ahead of the softmax
 
 template <int D>
@@ -147,7 +151,7 @@ struct PromptSmem {
 // each converted once for both tiles, and two steps of codes before them.
 //
 // Softmax and scales as in kv8_attend.cu: a reference m per row that moves only
-// when some weight would pass 2^5, weights 2^10 p in f16; the scale of a K page
+// when some p would pass 2^kMove, weights 2^kBase p in f16; the scale of a K page
 // multiplies its scores.  A V page's scale relative to the largest so far
 // multiplies its codes on their way to f16: exact for powers of two (an absolute
 // 2^-25 of the largest scale at worst), one rounding to 11 bits otherwise.
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     float m = kNone, l = 0.f, vref = 0.f;
     bool ok = true;
     uint32_t phase = 0;
-    for (int j = my_lo; j < my_hi; ++j, phase ^= 1) {
+    for (int j = my_lo; ok && j < my_hi; ++j, phase ^= 1) {
       if (!(ok = wait_warp(&s_full[x], phase))) break;
       mk::tc_fence_after();
       const int pos = j * kTile, slot = j % kMetaSlots;
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         }
       }
       const float vnow = s_vref[slot];
-      const bool move = top > m + kSlack;
+      const bool move = top > m + kMove;
       if (__any_sync(0xffffffffu, move) || vnow > vref) {
         float keep = vnow > vref ? vref / vnow : 1.f;
         if (move) {
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           }
         }
       }
-      const float back = 10.f - m;   // weights are 2^10 p
+      const float back = kBase - m;   // weights are 2^kBase p
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           if (sees_nan<F, P, kTile, D>(c, a, w, b, h, group, row0, row_last, m_row, d))
             out[d] = 0x7fff;   // NaN in bf16 and in f16
       }
-      if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - 10.f + log2f(l)) * 0.6931471805599453f;
+      if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - kBase + log2f(l)) * 0.6931471805599453f;
     }
   } else if (warp < kRowWarps + kCodeWarps) {
     // ---- codes to f16
@@ -554,23 +558,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         const int j = first + i, st = i & 1;
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-          if (in(t, j)) {
-            ok = wait_warp(&p_full[t], p_phase >> t & 1) && wait_warp(&v_full[st], i >> 1 & 1);
+          const bool now = in(t, j), next = i + 1 < nj && in(t, j + 1);
+          // what is there long before goes first: nothing but the weights is waited
+          // for between two tiles' products
+          if (now) ok = wait_warp(&v_full[st], i >> 1 & 1);
+          if (ok && next) ok = wait_warp(&k_full, (i + 1) & 1);
+          if (ok && now) ok = wait_warp(&p_full[t], p_phase >> t & 1);
+          if (!ok) break;
+          mk::tc_fence_after();
+          if (now) {
             p_phase ^= 1u << t;
-            if (!ok) break;
-            mk::tc_fence_after();
             const uint32_t more = j > (t ? j_lo[1] : j_lo[0]);
             const uint32_t va = desc_lo(smu + S::kV, kTile * 128) + st * (S::kOperand >> 4), pa = tmu + t * kTile, d = tmu + 2 * kTile + t * D;
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k) tc_mma_ts(one, d, pa + k * 8, va + k * (2048 >> 4), kDescHi, kO, k > 0 ? 1u : more);
             if (j + 1 == (t ? j_hi[1] : j_hi[0])) tc_commit_one(one, &o_full[t]);
           }
-          if (i + 1 < nj && in(t, j + 1)) {
-            ok = wait_warp(&k_full, (i + 1) & 1);
-            if (!ok) break;
-            mk::tc_fence_after();
-            scores(t);
-          }
+          if (next) scores(t);
         }
         if (!ok) break;
         tc_commit_one(one, &v_empty[st]);
