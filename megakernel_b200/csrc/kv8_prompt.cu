@@ -113,9 +113,10 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 
 // ---- layout ------------------------------------------------------------------------------
 
-constexpr int kTile = 128;                       // rows of a query tile, positions of a step
+constexpr int kTile = 128;                       // rows of a query tile
+constexpr int kStep = 64;                        // positions of a step
 constexpr int kRowWarps = 8, kCodeWarps = 8;     // two query tiles; converters
-constexpr int kMmaWarp = kRowWarps + kCodeWarps, kCopyWarp = kMmaWarp + 1;
+constexpr int kMmaWarp = kRowWarps + kCodeWarps, kCopyWarp = kMmaWarp + 2;
 constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 4) * 32;
 // Registers a thread of each role keeps; the block starts with 96 each, and the
 // sum over the five warpgroups is the launch's 480.
@@ -124,31 +125,36 @@ constexpr int kRowRegs = 168, kCodeRegs = 48, kMmaRegs = 48;
 // kv8_attend.cu (a move costs a pass over the output), and what is lost below is
 // 2^-31 of the row's reference.
 constexpr float kBase = 6.f, kMove = 9.f;
-constexpr int kMetaSlots = 8;   // the copies run at most five steps ahead of the softmax
+constexpr int kMetaSlots = 16;   // the copies run at most nine steps ahead of the softmax
 
 template <int D>
 struct PromptSmem {
-  static constexpr int kOperand = kTile * D * 2;                 // Q tile, K or V step in f16
-  static constexpr int kCodes = kTile * D;                       // K or V codes of a step
-  static constexpr int kStages = 2;                              // of codes
-  static constexpr int kQ = 0, kK = 2 * kOperand, kV = 3 * kOperand, kRaw = 5 * kOperand;
-  static constexpr int kBytes = kRaw + 2 * kStages * kCodes;
+  static constexpr int kTileBytes = kTile * D * 2;               // a query tile in f16
+  static constexpr int kOperand = kStep * D * 2;                 // K or V of a step in f16
+  static constexpr int kCodes = kStep * D;                       // its codes
+  static constexpr int kStages = 4, kRawStages = 2;              // of K and of V each
+  static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + kStages * kOperand, kRaw = kV + kStages * kOperand;
+  static constexpr int kBytes = kRaw + 2 * kRawStages * kCodes;
 };
 
 // ---- attention of many rows per sequence ---------------------------------------------------
 //
 // Work item: 256 rows of one (sequence, kv head), as two tiles of 128, all their
-// positions in steps of 128.  Roles of a block's five warpgroups:
+// positions in steps of 64.  Roles of a block's five warpgroups:
 //   warps 0-3, 4-7   one tile of rows each, one row per thread: softmax
 //   warps 8-15       8-bit codes to f16 operands, shared memory to shared memory
-//   warp 16          one lane issues every tcgen05.mma
-//   warp 17          looks pages and scales up and copies their codes to shared
-//                    memory (18 and 19 only give their registers away)
-// S = Q K^T [128 x 128] and O [128 x D] live in tensor memory; the weights go
-// back to tensor memory as f16, over their scores, and are the A operand of
-// O += P V.  While one tile's scores are with its warps the tensor cores work
-// for the other.  A step of K and two of V are in shared memory as f16,
-// each converted once for both tiles, and two steps of codes before them.
+//   warps 16, 17     one lane of each issues the products of one tile
+//   warp 18          looks pages and scales up and copies their codes to shared
+//                    memory (19 only gives its registers away)
+// S = Q K^T [128 x 64], two steps of it per tile, and O [128 x D] live in tensor
+// memory (all 512 columns for D = 128); the weights go back to tensor memory as
+// f16, over their scores, and are the A operand of O += P V.  While a tile's
+// warps are with one step's scores the tensor cores take the weights of the step
+// before and then write the scores of the step after: no side waits for the
+// other's latency.  (One step of 128 per tile at a time, the products waiting for
+// its weights and the softmax for its scores, took 367 us where this takes 264.)
+// K and V pass through rings of four steps in f16 and two steps of codes, each
+// converted once for both tiles.
 //
 // Softmax and scales as in kv8_attend.cu: a reference m per row that moves only
 // when some p would pass 2^kMove, weights 2^kBase p in f16; the scale of a K page
@@ -158,11 +164,16 @@ struct PromptSmem {
 template <class F, int P, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const Cache c, const Attend a) {
   using S = PromptSmem<D>;
-  constexpr int kSub = kTile / P;                    // pages of a step
+  constexpr int kSub = kStep / P;                    // pages of a step
+  constexpr int kStages = S::kStages, kRawStages = S::kRawStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
-  __shared__ __align__(8) uint64_t raw_full[2][S::kStages], raw_empty[2][S::kStages];   // codes of K, of V
+  __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  __shared__ __align__(8) uint64_t q_full, s_full[2][2], p_full[2][2];   // [tile][score buffer]
+  // P V of one step, of the last step: two may be outstanding there, and a parity
+  // tells only two neighbours apart
+  __shared__ __align__(8) uint64_t o_done[2], o_full[2], o_drain[2];
+  __shared__ __align__(8) uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];   // codes of K, of V
   // of a step: scales of the K pages (0: not there), of the V pages relative to
   // s_vref, the largest V scale up to it; whether all its pages are there
   __shared__ float s_ks[kMetaSlots][kSub], s_vf[kMetaSlots][kSub], s_vref[kMetaSlots];
@@ -177,7 +188,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   const int unit = (int)(gridDim.x - 1 - blockIdx.x), h = unit % c.kv_heads, item = unit / c.kv_heads;
   auto key = [&](int i) { return (int)((long long)__ldg(c.starts + i) * group / (2 * kTile)) + i; };
   const int b = warp_search(c.seqs, item, key);
-  const SeqWork w = seq_work<P, kTile, 2 * kTile>(c, a, b, group);
+  const SeqWork w = seq_work<P, kStep, 2 * kTile>(c, a, b, group);
   if (w.error != MK_OK && threadIdx.x == 0) report(a.status, w.error);
   const int tile = item - key(b);
   if (w.n == 0 || tile < 0 || tile >= w.tiles) return;
@@ -198,23 +209,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     own[x] = range_of(row0 + x * kTile, min(row0 + (x + 1) * kTile - 1, row_last));
-    j_lo[x] = own[x].lo / kTile;
-    j_hi[x] = x < tiles && own[x].hi > own[x].lo ? (own[x].hi + kTile - 1) / kTile : j_lo[x];
+    j_lo[x] = own[x].lo / kStep;
+    j_hi[x] = x < tiles && own[x].hi > own[x].lo ? (own[x].hi + kStep - 1) / kStep : j_lo[x];
   }
-  const int first = all.lo / kTile, last = max(j_hi[0], tiles == 2 ? j_hi[1] : 0);
+  const int first = all.lo / kStep, last = max(j_hi[0], tiles == 2 ? j_hi[1] : 0);
 
   if (threadIdx.x == 0) {
     s_nan = 0;
     s_abort = 0;
-    mk::mbar_init(&k_full, kCodeWarps * 32);
-    mk::mbar_init(&k_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    mk::mbar_init(&q_full, kRowWarps * 32);
+    for (int i = 0; i < kStages; ++i) {
+      mk::mbar_init(&k_full[i], kCodeWarps * 32);
       mk::mbar_init(&v_full[i], kCodeWarps * 32);
-      mk::mbar_init(&v_empty[i], 1);
-      mk::mbar_init(&s_full[i], 1);
-      mk::mbar_init(&p_full[i], 128);
+      mk::mbar_init(&k_empty[i], 2);   // both tiles' products
+      mk::mbar_init(&v_empty[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mk::mbar_init(&s_full[i][0], 1);
+      mk::mbar_init(&s_full[i][1], 1);
+      mk::mbar_init(&p_full[i][0], 128);   // one per buffer: a tile may be two steps of weights ahead
+      mk::mbar_init(&p_full[i][1], 128);
+      mk::mbar_init(&o_done[i], 1);
       mk::mbar_init(&o_full[i], 1);
-      for (int k = 0; k < S::kStages; ++k) {
+      for (int k = 0; k < kRawStages; ++k) {
         mk::mbar_init(&raw_full[i][k], kSub);
         mk::mbar_init(&raw_empty[i][k], kCodeWarps);
       }
@@ -237,75 +254,74 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   };
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
 
-  // ---- Q: thread r < 256 brings its row to f16, K contiguous, swizzled
-  const int x = warp >> 2, r = threadIdx.x & 127;   // tile and row of a softmax thread
-  const int m_row = row0 + x * kTile + r;
-  float rq = 0.f;
-  if (warp < kRowWarps) {
-    const bool real = m_row <= row_last;
-    const uint16_t* src = (const uint16_t*)a.q + (long long)(w.r0 + m_row / group) * a.q_row + (h * group + m_row % group) * a.q_head;
-    float top = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < D / 8; ++i) {
-      float v[8];
-      unpack8(real ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0), a.bf16, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
-    }
-    const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);   // as in kv8_attend.cu
-    const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
-    rq = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
-    uint8_t* dst = smem + S::kQ + x * S::kOperand + r * 128;
-#pragma unroll 4
-    for (int i = 0; i < D / 8; ++i) {
-      float v[8];
-      unpack8(real ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0), a.bf16, v);
-      uint4 o;
-      o.x = pack_f16(v[0] * up, v[1] * up);
-      o.y = pack_f16(v[2] * up, v[3] * up);
-      o.z = pack_f16(v[4] * up, v[5] * up);
-      o.w = pack_f16(v[6] * up, v[7] * up);
-      *reinterpret_cast<uint4*>(dst + i / 8 * (kTile * 128) + ((i % 8) ^ (r & 7)) * 16) = o;
-    }
-    fence_async_shared();
-  }
   mk::tc_fence_before();
   __syncthreads();
   mk::tc_fence_after();
   const uint32_t tm = s_tmem, smem0 = mk::smem_u32(smem);
-  const uint32_t tm_s[2] = {tm, tm + kTile}, tm_o[2] = {tm + 2 * kTile, tm + 2 * kTile + D};
-
   if (warp < kRowWarps) {
-    // ---- softmax of one row
     mk::setmaxnreg_inc<kRowRegs>();
+    const int x = warp >> 2, r = threadIdx.x & 127;   // tile, and row of this thread
+    const int m_row = row0 + x * kTile + r;
+    // ---- 32 rows of Q per warp to f16, K contiguous, swizzled; D / 8 lanes per row
+    float rq = 0.f;
+    {
+      constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes, kLoads = 32 / kRowsPer;
+      uint4 raw[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int m = row0 + warp * 32 + i * kRowsPer + lane / kLanes;
+        const uint16_t* src = (const uint16_t*)a.q + (long long)(w.r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head;
+        raw[i] = m <= row_last ? __ldg(reinterpret_cast<const uint4*>(src) + lane % kLanes) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        float v[8], top = 0.f;
+        unpack8(raw[i], a.bf16, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);   // as in kv8_attend.cu
+        const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
+        const float back = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
+        const float mine = __shfl_sync(0xffffffffu, back, lane % kRowsPer * kLanes);
+        if (lane / kRowsPer == i) rq = mine;
+        const int row = (warp & 3) * 32 + i * kRowsPer + lane / kLanes, ch = lane % kLanes;
+        *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTileBytes + ch / 8 * (kTile * 128) + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
+            make_uint4(pack_f16(v[0] * up, v[1] * up), pack_f16(v[2] * up, v[3] * up), pack_f16(v[4] * up, v[5] * up),
+                       pack_f16(v[6] * up, v[7] * up));
+      }
+      fence_async_shared();
+      mk::mbar_arrive(&q_full);
+    }
+    // ---- softmax of one row
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;   // lanes 32 (warp % 4) ..
-    const uint32_t ts = (x ? tm_s[1] : tm_s[0]) + quarter, to = (x ? tm_o[1] : tm_o[0]) + quarter;
+    const uint32_t to = tm + 2 * kTile + x * D + quarter;
     int lo, hi;
     row_sees(w, a, group, m_row, lo, hi);
     const int my_lo = x ? j_lo[1] : j_lo[0], my_hi = x ? j_hi[1] : j_hi[0];
     const int lo_max = x ? own[1].lo_max : own[0].lo_max, hi_min = x ? own[1].hi_min : own[0].hi_min;
     float m = kNone, l = 0.f, vref = 0.f;
     bool ok = true;
-    uint32_t phase = 0;
-    for (int j = my_lo; ok && j < my_hi; ++j, phase ^= 1) {
-      if (!(ok = wait_warp(&s_full[x], phase))) break;
+    uint32_t phase = 0;   // bit i: of score buffer i
+    for (int j = my_lo; j < my_hi; ++j) {
+      const int buf = j & 1, pos = j * kStep, slot = j % kMetaSlots;
+      const uint32_t ts = tm + x * kTile + buf * kStep + quarter;
+      if (!(ok = wait_warp(&s_full[x][buf], phase >> buf & 1))) break;
+      phase ^= 1u << buf;
       mk::tc_fence_after();
-      const int pos = j * kTile, slot = j % kMetaSlots;
-      const bool whole = s_there[slot] && pos >= lo_max && pos + kTile <= hi_min;
-      // The scores stay in registers: tensor memory gives an SM about 128 bytes a
-      // cycle, and reading them a second time took 70 us of 515 a call.
-      float v[4][32];
+      float v[2][32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_ld_f32x32(ts + 32 * q, v[q]);
+      const bool whole = s_there[slot] && pos >= lo_max && pos + kStep <= hi_min;
       float f[kSub];
 #pragma unroll
       for (int i = 0; i < kSub; ++i) f[i] = fmaxf(rq * s_ks[slot][i], 1.17549435e-38f);   // -inf x 0 would be NaN
-      tmem_ld_f32x32(ts, v[0]);
-      tmem_arrived(v[0]);
-#pragma unroll
-      for (int q = 1; q < 4; ++q) tmem_ld_f32x32(ts + 32 * q, v[q]);
+      const float vnow = s_vref[slot];
       float top = kNone;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (q > 0) tmem_arrived(v[q]);
+      for (int q = 0; q < 2; ++q) {
+        tmem_arrived(v[q]);
         if (!whole) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
@@ -322,7 +338,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f[(32 * q + i0) / P]);
         }
       }
-      const float vnow = s_vref[slot];
       const bool move = top > m + kMove;
       if (__any_sync(0xffffffffu, move) || vnow > vref) {
         float keep = vnow > vref ? vref / vnow : 1.f;
@@ -333,7 +348,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           m = top;
         }
         vref = vnow;
-        if (j > my_lo) {   // P V of the step before is complete: its scores came after it
+        if (j > my_lo) {   // once P V of the step before is complete
+          if (!(ok = wait_warp(&o_done[x], (j - 1 - my_lo) & 1))) break;
+          mk::tc_fence_after();
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 16) {
             uint32_t o[16];
@@ -348,7 +365,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       const float back = kBase - m;   // weights are 2^kBase p
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -362,39 +379,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       mk::tc_fence_before();
-      mk::mbar_arrive(&p_full[x]);
+      mk::mbar_arrive(&p_full[x][buf]);
     }
-    // ---- write the row
+    // ---- write the rows: through the tile's place in shared memory, which every
+    // product has read by then, for whole rows at a time
     if (ok && my_hi > my_lo) ok = wait_warp(&o_full[x], 0);
     if (ok && x < tiles) {
       mk::tc_fence_after();
-      const bool real = m_row <= row_last;
       const float inv = l == 0.f ? 0.f : vref / l;   // nothing seen: 0
-      const long long at = (long long)(w.r0 + m_row / group) * a.q_heads + h * group + m_row % group;
-      uint16_t* out = (uint16_t*)a.out + at * D;
+      uint8_t* mine = smem + S::kQ + x * S::kTileBytes + (warp & 3) * 32 * (D * 2);
+      const bool any = my_hi > my_lo;   // else that place may still be written, and only zeros are due
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 16) {
-        uint32_t o[16];
-        if (my_hi > my_lo) {
-          tmem_ld_x16(to + c0, o);
-          tmem_arrived(o);
+      for (int c0 = 0; any && c0 < D; c0 += 32) {
+        float o[32];
+        tmem_ld_f32x32(to + c0, o);
+        tmem_arrived(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = l != 0.f ? o[i] * inv : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(mine + lane * (D * 2) + (((c0 / 8 + i) ^ (lane & 7)) * 16)) =
+              make_uint4(pack_out(o[8 * i], o[8 * i + 1], a.bf16), pack_out(o[8 * i + 2], o[8 * i + 3], a.bf16),
+                         pack_out(o[8 * i + 4], o[8 * i + 5], a.bf16), pack_out(o[8 * i + 6], o[8 * i + 7], a.bf16));
+      }
+      __syncwarp();
+      constexpr int kLanes = D / 8;
+#pragma unroll 4
+      for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
+        const int mm = row0 + warp * 32 + i;
+        if (mm > row_last) continue;
+        const long long at = (long long)(w.r0 + mm / group) * a.q_heads + h * group + mm % group;
+        reinterpret_cast<uint4*>((uint16_t*)a.out + at * D)[lane % kLanes] =
+            any ? *reinterpret_cast<const uint4*>(mine + i * (D * 2) + (((lane % kLanes) ^ (i & 7)) * 16)) : make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
+      if (m_row <= row_last) {
+        const long long at = (long long)(w.r0 + m_row / group) * a.q_heads + h * group + m_row % group;
+        if (s_nan) {
+          for (int d = 0; d < D; ++d)
+            if (sees_nan<F, P, kStep, D>(c, a, w, b, h, group, row0, row_last, m_row, d)) ((uint16_t*)a.out)[at * D + d] = 0x7fff;
         }
-        if (!real) continue;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = my_hi > my_lo && l != 0.f ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
-        uint32_t y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = pack_out(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]), a.bf16);
-        *reinterpret_cast<uint4*>(out + c0) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(out + c0 + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+        if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - kBase + log2f(l)) * 0.6931471805599453f;
       }
-      if (real && s_nan) {
-#pragma unroll 1
-        for (int d = 0; d < D; ++d)
-          if (sees_nan<F, P, kTile, D>(c, a, w, b, h, group, row0, row_last, m_row, d))
-            out[d] = 0x7fff;   // NaN in bf16 and in f16
-      }
-      if (real && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - kBase + log2f(l)) * 0.6931471805599453f;
     }
   } else if (warp < kRowWarps + kCodeWarps) {
     // ---- codes to f16
@@ -415,7 +441,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           e[k] = *reinterpret_cast<const uint32_t*>(&y);
         }
       }
-      uint8_t* at = base + cc / 4 * (kTile * 128) + row * 128;
+      uint8_t* at = base + cc / 4 * (kStep * 128) + row * 128;
       const int ch = cc % 4 * 2;
       // odd chunks first in the second half of a row: eight lanes, eight banks
       const bool odd = cc >= 4;
@@ -424,50 +450,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       *reinterpret_cast<uint4*>(at + (((ch + !odd) ^ (row & 7)) * 16)) = odd ? even4 : odd4;
     };
     for (int j = first; j < last; ++j) {
-      const int i = j - first, st = i & 1, raw = i % S::kStages;
-      const uint32_t phase = (i >> 1) & 1, raw_phase = (i / S::kStages) & 1;
-      // K
-      if (!wait_warp(&raw_full[0][raw], raw_phase) || !wait_warp(&k_empty, (i & 1) ^ 1)) break;
-      const uint8_t* src = smem + S::kRaw + raw * S::kCodes + 16 * cc;
-      uint8_t* dst = smem + S::kK;
-#pragma unroll 2
-      for (int row = cr; row < kTile; row += kRowsPer)
-        store(dst, row, *reinterpret_cast<const uint4*>(src + row * D), false, __half2{});
-      fence_async_shared();
-      mk::mbar_arrive(&k_full);
-      __syncwarp();
-      if (lane == 0) mk::mbar_arrive(&raw_empty[0][raw]);
-      // V
-      const bool whole = s_there[j % kMetaSlots] && j * kTile >= all.lo_max && (j + 1) * kTile <= all.hi_min;
-      if (!wait_warp(&raw_full[1][raw], raw_phase) || !wait_warp(&v_empty[st], phase ^ 1)) break;
-      src += S::kStages * S::kCodes;
-      dst = smem + S::kV + st * S::kOperand;
-#pragma unroll 2
-      for (int row = cr; row < kTile; row += kRowsPer) {
-        uint4 v = *reinterpret_cast<const uint4*>(src + row * D);
-        const float factor = s_vf[j % kMetaSlots][row / P];
-        if (!whole) {
-          // What no row sees may hold anything: its codes count as 0.  A NaN that
-          // only some rows see is taken out here and put back at the end.
-          const int p = j * kTile + row;
-          if (p >= all.hi || p < all.lo || s_ks[j % kMetaSlots][row / P] == 0.f) v = make_uint4(0, 0, 0, 0);
-          if constexpr (F::kTopExp == 8) {
-            const uint32_t b0 = nan_bytes(v.x), b1 = nan_bytes(v.y), b2 = nan_bytes(v.z), b3 = nan_bytes(v.w);
-            if (b0 | b1 | b2 | b3) {
-              s_nan = 1;
-              v.x &= ~((b0 >> 7) * 0xffu);
-              v.y &= ~((b1 >> 7) * 0xffu);
-              v.z &= ~((b2 >> 7) * 0xffu);
-              v.w &= ~((b3 >> 7) * 0xffu);
+      const int i = j - first, st = i % kStages, raw = i % kRawStages;
+      const uint32_t phase = (i / kStages) & 1, raw_phase = (i / kRawStages) & 1;
+      bool ok = true;
+#pragma unroll
+      for (int kv = 0; ok && kv < 2; ++kv) {
+        ok = wait_warp(&raw_full[kv][raw], raw_phase) && wait_warp(&(kv ? v_empty : k_empty)[st], phase ^ 1);
+        if (!ok) break;
+        const bool whole = kv == 0 || (s_there[j % kMetaSlots] && j * kStep >= all.lo_max && (j + 1) * kStep <= all.hi_min);
+        const uint8_t* src = smem + S::kRaw + (kv * kRawStages + raw) * S::kCodes + 16 * cc;
+        uint8_t* dst = smem + (kv ? S::kV : S::kK) + st * S::kOperand;
+#pragma unroll
+        for (int row = cr; row < kStep; row += kRowsPer) {
+          uint4 v = *reinterpret_cast<const uint4*>(src + row * D);
+          if (!whole) {
+            // What no row sees may hold anything: its codes count as 0.  A NaN that
+            // only some rows see is taken out here and put back at the end.
+            const int p = j * kStep + row;
+            if (p >= all.hi || p < all.lo || s_ks[j % kMetaSlots][row / P] == 0.f) v = make_uint4(0, 0, 0, 0);
+            if constexpr (F::kTopExp == 8) {
+              const uint32_t b0 = nan_bytes(v.x), b1 = nan_bytes(v.y), b2 = nan_bytes(v.z), b3 = nan_bytes(v.w);
+              if (b0 | b1 | b2 | b3) {
+                s_nan = 1;
+                v.x &= ~((b0 >> 7) * 0xffu);
+                v.y &= ~((b1 >> 7) * 0xffu);
+                v.z &= ~((b2 >> 7) * 0xffu);
+                v.w &= ~((b3 >> 7) * 0xffu);
+              }
             }
           }
+          const float factor = kv ? s_vf[j % kMetaSlots][row / P] : 1.f;
+          store(dst, row, v, factor != 1.f, __float2half2_rn(factor));
         }
-        store(dst, row, v, factor != 1.f, __float2half2_rn(factor));
+        fence_async_shared();
+        mk::mbar_arrive(&(kv ? v_full : k_full)[st]);
+        __syncwarp();
+        if (lane == 0) mk::mbar_arrive(&raw_empty[kv][raw]);
       }
-      fence_async_shared();
-      mk::mbar_arrive(&v_full[st]);
-      __syncwarp();
-      if (lane == 0) mk::mbar_arrive(&raw_empty[1][raw]);
+      if (!ok) break;
     }
   } else {
     mk::setmaxnreg_dec<kMmaRegs>();
@@ -476,7 +496,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       struct Page { int id; float ks, vs; };
       auto page_of = [&](int j) {
         Page p{-1, 0.f, 0.f};
-        const int pos = j * kTile + lane * P;
+        const int pos = j * kStep + lane * P;
         if (j < last && lane < kSub && pos < all.hi && pos + P > all.lo) {
           p.id = page_id(c, b, pos / P, a.status);
           if (p.id >= 0) {
@@ -494,8 +514,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       bool ok = true;
       int done = first;
       for (int j = first; ok && j < last; ++j) {
-        const int i = j - first, raw = i % S::kStages;
-        const uint32_t phase = (i / S::kStages) & 1;
+        const int i = j - first, raw = i % kRawStages;
+        const uint32_t phase = (i / kRawStages) & 1;
         vref = fmaxf(vref, mk::warp_max(now.vs));
         const bool there = __all_sync(0xffffffffu, lane >= kSub || now.id >= 0);
         for (int kv = 0; kv < 2; ++kv) {
@@ -511,7 +531,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
             mk::mbar_arrive_expect_tx(&raw_full[kv][raw], now.id >= 0 ? P * D : 0);
             if (now.id >= 0)
-              mk::bulk_g2s(smem + S::kRaw + (kv * S::kStages + raw) * S::kCodes + lane * P * D,
+              mk::bulk_g2s(smem + S::kRaw + (kv * kRawStages + raw) * S::kCodes + lane * P * D,
                            c.codes + now.id * c.page_stride + (long long)(kv * c.kv_heads + h) * P * D, P * D,
                            &raw_full[kv][raw], policy);
           }
@@ -522,71 +542,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         next = page_of(j + 2);
       }
       // no copy in flight when the block's memory is given away
-      for (int j = max(first, done - S::kStages); j < done; ++j)
-        for (int kv = 0; kv < 2; ++kv) wait_bar(&raw_full[kv][(j - first) % S::kStages], ((j - first) / S::kStages) & 1);
+      for (int j = max(first, done - kRawStages); j < done; ++j)
+        for (int kv = 0; kv < 2; ++kv) wait_bar(&raw_full[kv][(j - first) % kRawStages], ((j - first) / kRawStages) & 1);
     }
-    if (warp == kMmaWarp) {
-      // ---- tensor cores: every product issued by one lane
-      constexpr uint32_t kS = idesc_f16(kTile, kTile, false), kO = idesc_f16(kTile, D, true);
+    if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+      // ---- tensor cores: a tile's products, every one issued by one lane.  A warp
+      // gets an instruction in some ten cycles here, so what it does per step is
+      // kept short: one warp for both tiles took 391 us a call.
+      constexpr uint32_t kS = idesc_f16(kTile, kStep, false), kO = idesc_f16(kTile, D, true);
       const uint32_t one = elect_one();
       const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0), smu = __shfl_sync(0xffffffffu, smem0, 0);
-      const int nj = last - first;
-      bool ok = true;
-      uint32_t p_phase = 0;   // bit t: of tile t
-      auto in = [&](int t, int j) { return t ? j >= j_lo[1] && j < j_hi[1] : j >= j_lo[0] && j < j_hi[0]; };
-      auto scores = [&](int t) {
-        const uint32_t qa = desc_lo(smu + S::kQ) + t * (S::kOperand >> 4), ka = desc_lo(smu + S::kK), d = tmu + t * kTile;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)(k >> 2) * (kTile * 128 >> 4) + (k & 3) * 2;
-          tc_mma_ss(one, d, qa + off, ka + off, kDescHi, kS, k > 0);
-        }
-        tc_commit_one(one, &s_full[t]);
-      };
-      if (nj > 0) {
-        ok = wait_warp(&k_full, 0);
-        mk::tc_fence_after();
-        if (ok) {
+      const int t = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
+      const int nj = last - first, lo = (t ? j_lo[1] : j_lo[0]) - first, hi = (t ? j_hi[1] : j_hi[0]) - first;   // steps from the first on
+      const uint32_t q0 = desc_lo(smu + S::kQ + t * S::kTileBytes), k0 = desc_lo(smu + S::kK), v0 = desc_lo(smu + S::kV, kStep * 128);
+      const uint32_t ts = tmu + t * kTile, to = tmu + 2 * kTile + t * D;
+      bool ok = nj == 0 || wait_warp(&q_full, 0);
+      uint32_t p_phase = 0;   // bit i: of score buffer i
+      // two steps of scores ahead of the weights
 #pragma unroll 1
-          for (int t = 0; t < 2; ++t)
-            if (in(t, first)) scores(t);
-          tc_commit_one(one, &k_empty);
-        }
-      }
-#pragma unroll 1
-      for (int i = 0; ok && i < nj; ++i) {
-        const int j = first + i, st = i & 1;
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {
-          const bool now = in(t, j), next = i + 1 < nj && in(t, j + 1);
-          // what is there long before goes first: nothing but the weights is waited
-          // for between two tiles' products
-          if (now) ok = wait_warp(&v_full[st], i >> 1 & 1);
-          if (ok && next) ok = wait_warp(&k_full, (i + 1) & 1);
-          if (ok && now) ok = wait_warp(&p_full[t], p_phase >> t & 1);
-          if (!ok) break;
+      for (int i = -2; ok && i < nj; ++i) {
+        const int buf = (first + i) & 1, ks = (i + 2) % kStages, vs = i & (kStages - 1);
+        // what is there long before goes first: nothing but the weights is waited
+        // for right before their product
+        if (i >= 0 && !(ok = wait_warp(&v_full[vs], i / kStages & 1))) break;
+        if (i + 2 < nj && !(ok = wait_warp(&k_full[ks], (i + 2) / kStages & 1))) break;
+        if (i >= lo && i < hi) {
+          if (!(ok = wait_warp(&p_full[t][buf], p_phase >> buf & 1))) break;
+          p_phase ^= 1u << buf;
           mk::tc_fence_after();
-          if (now) {
-            p_phase ^= 1u << t;
-            const uint32_t more = j > (t ? j_lo[1] : j_lo[0]);
-            const uint32_t va = desc_lo(smu + S::kV, kTile * 128) + st * (S::kOperand >> 4), pa = tmu + t * kTile, d = tmu + 2 * kTile + t * D;
+          const uint32_t va = v0 + vs * (S::kOperand >> 4), pa = ts + buf * kStep, more = i > lo;
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k) tc_mma_ts(one, d, pa + k * 8, va + k * (2048 >> 4), kDescHi, kO, k > 0 ? 1u : more);
-            if (j + 1 == (t ? j_hi[1] : j_hi[0])) tc_commit_one(one, &o_full[t]);
-          }
-          if (next) scores(t);
+          for (int k = 0; k < kStep / 16; ++k) tc_mma_ts(one, to, pa + k * 8, va + k * (2048 >> 4), kDescHi, kO, k > 0 ? 1u : more);
+          tc_commit_one(one, &o_done[t]);
+          if (i + 1 == hi) tc_commit_one(one, &o_full[t]);
         }
-        if (!ok) break;
-        tc_commit_one(one, &v_empty[st]);
-        if (i + 1 < nj) tc_commit_one(one, &k_empty);
+        if (i >= 0) tc_commit_one(one, &v_empty[vs]);
+        if (i + 2 >= lo && i + 2 < hi) {
+          mk::tc_fence_after();
+          const uint32_t ka = k0 + ks * (S::kOperand >> 4), d = ts + buf * kStep;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_ss(one, d, q0 + (k >> 2) * (kTile * 128 >> 4) + (k & 3) * 2, ka + (k >> 2) * (kStep * 128 >> 4) + (k & 3) * 2,
+                      kDescHi, kS, k > 0);
+          tc_commit_one(one, &s_full[t][buf]);
+        }
+        if (i + 2 < nj) tc_commit_one(one, &k_empty[ks]);
       }
       if (!ok) {   // nothing of this block's may be in flight when its memory is given away
         if (one) {
           report(a.status, MK_ERR_TIMEOUT);
-          mk::mbar_init(&k_full, 1);
+          mk::mbar_init(&o_drain[t], 1);
           mk::fence_mbar_init();
-          mk::tc_commit(&k_full);
-          wait_bar(&k_full, 0);
+          mk::tc_commit(&o_drain[t]);
+          wait_bar(&o_drain[t], 0);
         }
         __syncwarp();
       }
