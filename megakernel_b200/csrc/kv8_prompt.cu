@@ -152,7 +152,7 @@ struct PromptSmem {
 // warps are with one step's scores the tensor cores take the weights of the step
 // before and then write the scores of the step after: no side waits for the
 // other's latency.  (One step of 128 per tile at a time, the products waiting for
-// its weights and the softmax for its scores, took 367 us where this takes 264.)
+// its weights and the softmax for its scores, took 367 us where this takes 338.)
 // K and V pass through rings of four steps in f16 and two steps of codes, each
 // converted once for both tiles.
 //
