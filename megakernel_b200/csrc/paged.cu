@@ -2,6 +2,8 @@
 // write of keys and values into the 8-bit cache, its read-back, and the
 // verification of drafted tokens (C ABI in include/megakernel.h).  Attention
 // over the cache is in kv8_attend.cu.  The reference has no counterpart.
+#include <algorithm>
+
 #include "paged.cuh"
 #include "tc_ptx.cuh"
 
@@ -14,7 +16,10 @@ namespace mkp {
 // for the two halves (1, 2) of a head row of D.  A group of D/16 lanes holds a
 // row: lane l its elements [8l, 8l+8) of both halves, so that the rotation
 // stays in the lane and the sum of squares is the only exchange.  fp32
-// throughout, one rounding at the store.
+// throughout, one rounding at the store.  Bound by memory; a warp that takes all
+// heads of a token, to read its cosines and sines once, holds more registers than
+// it saves reads (65,531 rows of 24 heads: 136 us, this 74 =
+// 5.7 TB/s).
 struct NormRope {
   const void *q, *k, *q_gain, *k_gain;
   void *q_out, *k_out;
@@ -40,6 +45,7 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const NormRope a) {
   T* o = is_q ? (T*)a.q_out + row * a.qo_row + h * a.qo_head
               : (T*)a.k_out + row * a.ko_row + (h - a.q_heads) * a.ko_head;
   const T* g = (const T*)(is_q ? a.q_gain : a.k_gain);
+  const int pos = __ldg(a.positions + row);
   Vec8<T> x1, x2, g1, g2;
   x1.load(x + 8 * l);
   x2.load(x + kHalf + 8 * l);
@@ -52,18 +58,18 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const NormRope a) {
 #pragma unroll
   for (int s = kLanes / 2; s > 0; s >>= 1) ss += __shfl_xor_sync(group, ss, s);
   const float r = 1.f / sqrtf(ss * (1.f / D) + a.eps);
-  const int pos = __ldg(a.positions + row);
   if (pos < 0 || pos >= a.table_rows) {
     if (l == 0) report(a.status, MK_ERR_CAPACITY);
     return;
   }
-  const float* c = a.cos + (long long)pos * kHalf + 8 * l;
-  const float* s = a.sin + (long long)pos * kHalf + 8 * l;
+  Vec8<float> c, s;
+  c.load(a.cos + (long long)pos * kHalf + 8 * l);
+  s.load(a.sin + (long long)pos * kHalf + 8 * l);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float y1 = x1.f(i) * r * g1.f(i), y2 = x2.f(i) * r * g2.f(i);
-    x1.set(i, y1 * c[i] - y2 * s[i]);
-    x2.set(i, y2 * c[i] + y1 * s[i]);
+    x1.set(i, y1 * c.f(i) - y2 * s.f(i));
+    x2.set(i, y2 * c.f(i) + y1 * s.f(i));
   }
   x1.store(o + 8 * l);
   x2.store(o + kHalf + 8 * l);
@@ -71,13 +77,14 @@ __global__ void __launch_bounds__(128) norm_rope_kernel(const NormRope a) {
 
 // ---- cache write ------------------------------------------------------------------
 //
-// One block of threads per (page that new rows fall into, K or V, head).  The
-// page's scale is the smallest power of two that fits its largest magnitude;
-// if the page already holds earlier positions the scale only grows, and then
-// the earlier codes are rounded again to the larger one.  A power of two makes
-// x / scale exact, so the codes do not depend on how the division is done, and
-// growing the scale of e4m3 codes loses nothing but what falls below the
-// smallest subnormal.
+// A block of threads takes a page that new rows fall into, and of it every
+// gridDim.y-th (K or V, head), loading one while it reduces and stores the one
+// before.  The page's scale is the smallest power of two that fits its largest
+// magnitude; if the page already holds earlier positions the scale only grows,
+// and then the earlier codes are rounded again to the larger one.  A power of two
+// makes x / scale exact, so the codes do not depend on how the division is done,
+// and growing the scale of e4m3 codes loses nothing but what falls below the
+// smallest subnormal.  Bound by memory.
 template <class T, class F, int P, int D>
 __global__ void __launch_bounds__(128) append_kernel(const Cache c, const T* k, const T* v, long long k_row,
                                                      long long k_head, long long v_row, long long v_head,
@@ -87,72 +94,95 @@ __global__ void __launch_bounds__(128) append_kernel(const Cache c, const T* k, 
   Block blk;
   if (!block_of<P>(c, (int)blockIdx.x, &blk, status)) return;
   const Span s = blk.s;
-  const int pg = blk.blk, p0 = blk.p0, p1 = blk.p1;
+  const int pg = blk.blk;
   const int id = page_id(c, blk.b, pg, status);
   if (id < 0) return;
-  const int h = blockIdx.y >> 1, kv = blockIdx.y & 1;
-  const T* src = kv ? v + h * v_head : k + h * k_head;
-  const long long src_row = kv ? v_row : k_row;
   const int lane = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
-  const int keep = p0 - pg * P, end = p1 - pg * P;   // slots [0, keep) held, [keep, end) new
-  uint8_t* dst = c.codes + id * c.page_stride + (long long)(kv * c.kv_heads + h) * P * D;
-  float* scale = c.scales + id * c.scale_stride + kv * c.kv_heads + h;
+  const int keep = blk.p0 - pg * P, end = blk.p1 - pg * P;   // slots [0, keep) held, [keep, end) new
+  const long long row0 = s.row + (pg * P - s.pos);           // packed row of slot 0
+  const int kinds = 2 * c.kv_heads;
+  __shared__ float part[2][4];
 
-  Vec8<T> x[kPasses][2];
-  float amax = 0.f;
+  Vec8<T> x[kPasses][2], y[kPasses][2];
+  float old = 0.f, next_old = 0.f;
+  auto load = [&](int kh, Vec8<T> (&z)[kPasses][2], float* held) {
+    const int kv = kh >= c.kv_heads, h = kh - kv * c.kv_heads;
+    const T* src = (kv ? v + h * v_head : k + h * k_head) + 16 * lane;
+    const long long src_row = kv ? v_row : k_row;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int slot = i * kRows + sub;
-    if (slot < keep || slot >= end) continue;
-    const T* p = src + (s.row + (pg * P + slot - s.pos)) * src_row + 16 * lane;
-    x[i][0].load(p);
-    x[i][1].load(p + 8);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float m = fabsf(x[i][j >> 3].f(j & 7));
-      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);   // finite values only
+    for (int i = 0; i < kPasses; ++i) {
+      const int slot = i * kRows + sub;
+      if (slot < keep || slot >= end) continue;
+      z[i][0].load(src + (row0 + slot) * src_row);
+      z[i][1].load(src + (row0 + slot) * src_row + 8);
     }
-  }
-  amax = mk::warp_max(amax);
-  __shared__ float part[4];
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
-  __syncthreads();
-  amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-  float sc = scale_for<F>(amax);
-  if (keep > 0) {
-    const float old = *scale;
-    sc = fmaxf(sc, old);
-    if (sc != old) {
-      const float ratio = old / sc;
+    if (keep > 0) *held = c.scales[id * c.scale_stride + kh];
+  };
+  load(blockIdx.y, x, &old);
+  int flip = 0;
+  for (int kh = blockIdx.y; kh < kinds; kh += gridDim.y, flip ^= 1) {
+    if (kh + (int)gridDim.y < kinds) load(kh + gridDim.y, y, &next_old);
+    float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int slot = i * kRows + sub;
-        if (slot >= keep) continue;
-        uint4* p = reinterpret_cast<uint4*>(dst + slot * D + 16 * lane);
-        uint4 w = *p;
-        uint8_t* e = reinterpret_cast<uint8_t*>(&w);
+    for (int i = 0; i < kPasses; ++i) {
+      const int slot = i * kRows + sub;
+      if (slot < keep || slot >= end) continue;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) e[j] = F::encode(F::decode(e[j]) * ratio);
-        *p = w;
+      for (int j = 0; j < 16; ++j) {
+        const float m = fabsf(x[i][j >> 3].f(j & 7));
+        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);   // finite values only
       }
     }
-  }
-  const float inv = 1.f / sc;
+    amax = mk::warp_max(amax);
+    if ((threadIdx.x & 31) == 0) part[flip][threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(part[flip][0], part[flip][1]), fmaxf(part[flip][2], part[flip][3]));
+    float sc = scale_for<F>(amax);
+    uint8_t* dst = c.codes + id * c.page_stride + (long long)kh * P * D;
+    if (keep > 0) {
+      sc = fmaxf(sc, old);
+      if (sc != old) {
+        const float ratio = old / sc;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int slot = i * kRows + sub;
-    if (slot < keep || slot >= end) continue;
-    uint4 w;
-    uint8_t* e = reinterpret_cast<uint8_t*>(&w);
+        for (int i = 0; i < kPasses; ++i) {
+          const int slot = i * kRows + sub;
+          if (slot >= keep) continue;
+          uint4* p = reinterpret_cast<uint4*>(dst + slot * D + 16 * lane);
+          uint4 w = *p;
+          uint8_t* e = reinterpret_cast<uint8_t*>(&w);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) e[j] = F::encode(x[i][j >> 3].f(j & 7) * inv);
-    *reinterpret_cast<uint4*>(dst + slot * D + 16 * lane) = w;
+          for (int j = 0; j < 16; ++j) e[j] = F::encode(F::decode(e[j]) * ratio);
+          *p = w;
+        }
+      }
+    }
+    const float inv = 1.f / sc;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int slot = i * kRows + sub;
+      if (slot < keep || slot >= end) continue;
+      uint4 w;
+      uint8_t* e = reinterpret_cast<uint8_t*>(&w);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) e[j] = F::encode(x[i][j >> 3].f(j & 7) * inv);
+      *reinterpret_cast<uint4*>(dst + slot * D + 16 * lane) = w;
+    }
+    // every thread had this scale before the barrier above
+    if (threadIdx.x == 0 && (keep == 0 || sc != old)) c.scales[id * c.scale_stride + kh] = sc;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      x[i][0] = y[i][0];
+      x[i][1] = y[i][1];
+    }
+    old = next_old;
   }
-  __syncthreads();   // every thread has read the old scale
-  if (threadIdx.x == 0) *scale = sc;
 }
 
 // ---- cache read -------------------------------------------------------------------
+// A block of threads takes a page, and of it one of gridDim.y shares of the (K or
+// V, head); 256 threads for whole pages (16 x ~7,600 positions 126 us = 5.9 TB/s,
+// with 128 129), 128 for shares (one token for each of 64 sequences written and
+// its page read: 9.8 us, with 256 11.3).  Bound by memory.
 template <class T, class F, int P, int D>
 __global__ void __launch_bounds__(256) read_kernel(const Cache c, T* k, T* v, int* status) {
   Block blk;
@@ -161,13 +191,14 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, T* k, T* v, in
   const int pg = blk.blk, p0 = blk.p0, p1 = blk.p1;
   const int id = page_id(c, blk.b, pg, status);
   if (id < 0) return;
-  const uint8_t* src = c.codes + id * c.page_stride;
-  const float* scale = c.scales + id * c.scale_stride;
   constexpr int kVecs = D / 16;
-  const int total = 2 * c.kv_heads * P * kVecs;
+  const int per = (2 * c.kv_heads + gridDim.y - 1) / gridDim.y, kh0 = blockIdx.y * per;
+  const int total = (min(kh0 + per, 2 * c.kv_heads) - kh0) * P * kVecs;
+  const uint8_t* src = c.codes + id * c.page_stride + (long long)kh0 * P * D;
+  const float* scale = c.scales + id * c.scale_stride;
+#pragma unroll 4
   for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const int vec = i % kVecs, slot = i / kVecs % P, kh = i / (kVecs * P);
-    const int pos = pg * P + slot;
+    const int vec = i % kVecs, pos = pg * P + i / kVecs % P, kh = kh0 + i / (kVecs * P);
     if (pos < p0 || pos >= p1) continue;
     const uint4 w = *reinterpret_cast<const uint4*>(src + (long long)i * 16);
     const uint8_t* e = reinterpret_cast<const uint8_t*>(&w);
@@ -447,6 +478,17 @@ int cache_of(const mk_kv8* m, Cache* c) {
   return MK_OK;
 }
 
+// Blocks of append and read: one per page and, until they fill the GPU (kFill of
+// them per SM), per share of the page's (K or V, head).  64 prompts of ~1,020
+// positions written and read: kFill 8 186 us, 16 159, 32 164, 64 183.
+static dim3 page_grid(const Cache& c, int page_size) {
+  constexpr long long kFill = 16;
+  const long long items = item_count(c.rows, c.seqs, page_size), kinds = 2 * c.kv_heads;
+  long long share = 1;
+  while (share < kinds && items * share < 148 * kFill) share *= 2;
+  return dim3((unsigned)items, (unsigned)std::min(share, kinds));
+}
+
 // Calls f with the compile-time page size and head size of m (checked before).
 template <class Fn>
 static int by_page(const mk_kv8* m, Fn f) {
@@ -479,7 +521,7 @@ int megakernel_qk_norm_rope(const mk_qk_norm_rope* m, int* d_status, void* strea
   if (!m || m->rows < 0 || m->q_heads < 0 || m->kv_heads < 0 || m->table_rows < 0 || !type_ok(m->type))
     return MK_ERR_INVALID_ARG;
   if (m->head_dim != 64 && m->head_dim != 128) return MK_ERR_INVALID_ARG;
-  if (!(m->eps >= 0.f)) return MK_ERR_INVALID_ARG;
+  if (!(m->eps >= 0.f) || m->q_heads > (1 << 20) || m->kv_heads > (1 << 20)) return MK_ERR_INVALID_ARG;
   const long long heads = (long long)m->q_heads + m->kv_heads;
   if (m->rows == 0 || heads == 0) return MK_OK;
   const int size = type_size(m->type);
@@ -494,8 +536,7 @@ int megakernel_qk_norm_rope(const mk_qk_norm_rope* m, int* d_status, void* strea
                           !aligned16(m->d_k_gain) || !strides_ok(m->k_row, m->k_head, size) ||
                           !strides_ok(m->ko_row, m->ko_head, size)))
     return MK_ERR_INVALID_ARG;
-  const int lanes = m->head_dim / 16;
-  const long long blocks = ((long long)m->rows * heads * lanes + 127) / 128;
+  const long long blocks = ((long long)m->rows * heads * (m->head_dim / 16) + 127) / 128;
   if (blocks > 0x7fffffffLL) return MK_ERR_INVALID_ARG;
   NormRope a{m->d_q, m->d_k, m->d_q_gain, m->d_k_gain, m->d_q_out, m->d_k_out, m->d_cos, m->d_sin, m->d_positions,
              m->q_row, m->q_head, m->k_row, m->k_head, m->qo_row, m->qo_head, m->ko_row, m->ko_head,
@@ -521,7 +562,7 @@ int megakernel_kv8_append(const mk_kv8* cache, const void* d_k, long long k_row,
   if (!d_k || !d_v || !aligned16(d_k) || !aligned16(d_v) || !strides_ok(k_row, k_head, size) ||
       !strides_ok(v_row, v_head, size))
     return MK_ERR_INVALID_ARG;
-  const dim3 grid((unsigned)item_count(c.rows, c.seqs, cache->page_size), 2 * c.kv_heads);
+  const dim3 grid = page_grid(c, cache->page_size);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     return by_format(cache->format, [&](auto f) {
@@ -542,13 +583,13 @@ int megakernel_kv8_read(const mk_kv8* cache, void* d_k, void* d_v, int type, int
   if (!type_ok(type)) return MK_ERR_INVALID_ARG;
   if (c.seqs == 0 || c.rows == 0) return MK_OK;
   if (!d_k || !d_v || !aligned16(d_k) || !aligned16(d_v)) return MK_ERR_INVALID_ARG;
-  const unsigned grid = (unsigned)item_count(c.rows, c.seqs, cache->page_size);
+  const dim3 grid = page_grid(c, cache->page_size);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     return by_format(cache->format, [&](auto f) {
       using F = decltype(f);
       return by_page(cache, [&](auto p, auto d) {
-        read_kernel<T, F, decltype(p)::value, decltype(d)::value><<<grid, 256, 0, (cudaStream_t)stream>>>(
+        read_kernel<T, F, decltype(p)::value, decltype(d)::value><<<grid, grid.y > 1 ? 128 : 256, 0, (cudaStream_t)stream>>>(
             c, (T*)d_k, (T*)d_v, d_status);
         return launched();
       });
