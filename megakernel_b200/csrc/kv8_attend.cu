@@ -718,7 +718,14 @@ static int launch(const Cache& c, const Attend& a, void* work, size_t work_bytes
   }
   // rows of a sequence, once per query head of the group, on average
   const long long per = ((long long)c.rows * (a.q_heads / c.kv_heads) + c.seqs - 1) / c.seqs;
-  if (per > 64) return attend_prompt(c, a, std::is_same<F, E4M3>::value ? MK_KV8_E4M3 : MK_KV8_INT8, P, D, stream);
+  // Either kernel's time grows with the positions, which the host does not know:
+  // the rows' kernel with its items of 16 rows (4,096 positions: 0.2 to 0.25 us
+  // each), the prompts' with the waves of its blocks of 256 rows (78 to 92 us each).
+  // 32 sequences x 16 rows: 95 against 157 us, x 32 rows 241 against 158; one of
+  // 256 rows 51 against 83, four of 128 92 against 83 (head_dim 64, 16 / 8 heads).
+  const long long kvs = (long long)c.seqs * c.kv_heads, items = (per + 15) / 16 * kvs;
+  const long long waves = ((per + 255) / 256 * kvs + 147) / 148;
+  if (items > 350 * waves) return attend_prompt(c, a, std::is_same<F, E4M3>::value ? MK_KV8_E4M3 : MK_KV8_INT8, P, D, stream);
   return per <= 8 ? launch_rows<F, P, D, 1>(c, a, work, work_bytes, need, stream)
                   : launch_rows<F, P, D, 2>(c, a, work, work_bytes, need, stream);
 }
