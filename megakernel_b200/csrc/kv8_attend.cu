@@ -403,28 +403,31 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
 
       // ---- weights
       float f[kSub][NT][2];
-      bool over = false;
 #pragma unroll
       for (int x = 0; x < kSub; ++x)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) f[x][nt][e] = fmaxf(rq[nt][e] * ks[x], 1.17549435e-38f);   // -inf x 0 would be NaN
+      if (!whole) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int sub = mt * 16 / kSubRows;
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int j = pos + mt * 16 + g + 8 * (x >> 1);
+              if (ks[mt * 16 / kSubRows] == 0.f || j < lo[nt][x & 1] || j >= hi[nt][x & 1]) s[mt][nt][x] = -INFINITY;
+            }
+      }
+      float high = -INFINITY;   // the largest s - m
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (!whole) {
-              const int j = pos + mt * 16 + g + 8 * (x >> 1);
-              if (ks[sub] == 0.f || j < lo[nt][x & 1] || j >= hi[nt][x & 1]) s[mt][nt][x] = -INFINITY;
-            }
-            over = over || fmaf(s[mt][nt][x], f[sub][nt][x & 1], -m[nt][x & 1]) > kSlack;
-          }
-      }
-      if (__any_sync(0xffffffffu, over)) {
+          for (int x = 0; x < 4; ++x) high = fmaxf(high, fmaf(s[mt][nt][x], f[mt * 16 / kSubRows][nt][x & 1], -m[nt][x & 1]));
+      if (__any_sync(0xffffffffu, high > kSlack)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -483,10 +486,13 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
             const uint4 u = *reinterpret_cast<const uint4*>(vb + row * D);
             v[x][0] = u.x; v[x][1] = u.y; v[x][2] = u.z; v[x][3] = u.w;
           }
-          if (!whole) {
-            // What no row sees may hold anything: its codes count as 0.  A NaN
-            // that only some rows see is taken out here and put back at the end.
-            const int j = pos + 2 * t + row;
+        }
+        if (!whole) {
+          // What no row sees may hold anything: its codes count as 0.  A NaN that
+          // only some rows see is taken out here and put back at the end.
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int j = pos + 2 * t + mt * 16 + (x & 1) + 8 * (x >> 1);
             const bool dead = ks[mt * 16 / kSubRows] == 0.f || j >= hi_all || j < lo_all;
 #pragma unroll
             for (int y = 0; y < D / 32; ++y) {
