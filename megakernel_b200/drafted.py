@@ -1,0 +1,167 @@
+"""``DraftedDecoder``: decoding of several sequences with drafted tokens.
+
+A serving loop over the paged operators (``megakernel_b200.paged``), beside the
+single-stream engine and ``BatchDecoder``: sequences of any length share a pool
+of 8-bit pages, a step feeds each sequence its last token and a few drafted
+ones, and verification keeps the drafts that stand plus one more token.  Per
+layer: norm and rotation of the heads (``qk_norm_rope``), the write into the
+cache (``kv8_append``), attention over it (``kv8_attend``); per step
+``verify_drafts``.  The projections are plain matrix products.  Drafts come
+from a lookup: the tokens that followed the last occurrence of the sequence's
+final n-gram.  Same flat-binary weights as the other engines, every shape of
+``megakernel_b200.shapes``.  There is no CPU path.
+
+    python -m megakernel_b200.drafted --shape tiny --tokens 64
+"""
+from __future__ import annotations
+
+import argparse
+import sys
+import time
+
+import numpy as np
+import torch
+
+from . import paged, weights as W
+from .shapes import SHAPES, Shape
+
+
+def lookup_draft(tokens, most, ngram=3):
+    """Up to `most` tokens that followed the latest earlier occurrence of the
+    last n tokens, for the largest n <= ngram that occurs earlier."""
+    for n in range(min(ngram, len(tokens) - 1), 0, -1):
+        tail = tokens[-n:]
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if tokens[at:at + n] == tail:
+                return tokens[at + n:at + n + most]
+    return []
+
+
+class DraftedDecoder:
+    def __init__(self, flat, offsets, shape: Shape, *, seqs, max_seq, pages=None, page_size=64, kv_dtype="fp8", device=0):
+        """flat, offsets: the flat binary and its offsets; seqs sequences of up
+        to max_seq positions share `pages` pages (default: enough for all)."""
+        self.shape, self.device, self.seqs, self.max_seq = shape, torch.device("cuda", device), int(seqs), int(max_seq)
+        raw = flat if isinstance(flat, torch.Tensor) else torch.from_numpy(np.asarray(flat, dtype=np.uint8))
+        raw = raw.to(self.device)
+        w = {}
+        for name, s in shape.tensor_shapes():
+            n = int(np.prod(s))
+            w[name] = raw[offsets[name]:offsets[name] + 2 * n].clone().view(torch.bfloat16).view(*s)
+        self.w = w
+        self.w_qkv = [torch.cat([w[f"layer.{i}.{k}"] for k in ("w_q", "w_k", "w_v")]) for i in range(shape.layers)]
+        self.w_gate_up = [torch.cat([w[f"layer.{i}.{k}"] for k in ("w_gate", "w_up")]) for i in range(shape.layers)]
+        inv = 1.0 / shape.rope_theta ** (torch.arange(0, shape.head_dim, 2, dtype=torch.float32) / shape.head_dim)
+        angle = torch.arange(max_seq, dtype=torch.float32)[:, None] * inv
+        self.cos, self.sin = angle.cos().to(self.device), angle.sin().to(self.device)
+        per = -(-self.max_seq // page_size)
+        self.cache = paged.PagedCache8(shape.layers, shape.kv_heads, shape.head_dim, pages or seqs * per, seqs, max_seq,
+                                       page_size=page_size, kv_dtype=kv_dtype, device=device)
+
+    def _int32(self, v):
+        return torch.tensor(v, dtype=torch.int32).to(self.device)
+
+    def _norm(self, x, gain):
+        return (x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.shape.rms_eps)).to(torch.bfloat16) * gain
+
+    def forward(self, tokens, first):
+        """Feed tokens[b] (a list, possibly empty) to sequence b from position
+        first[b] on; returns the fp32 logits of all rows, packed, and the row
+        starts (int32, on the device)."""
+        s = self.shape
+        rows = [len(t) for t in tokens]
+        for b, (f, n) in enumerate(zip(first, rows)):
+            self.cache.reserve(b, f + n)
+        starts = self._int32(np.concatenate([[0], np.cumsum(rows)]).tolist())
+        at = self._int32(list(first))
+        pos = self._int32([f + i for f, n in zip(first, rows) for i in range(n)])
+        x = self.w["embedding"][self._int32([t for ts in tokens for t in ts]).long()].float()
+        q_dim, kv_dim = s.q_dim, s.kv_dim
+        for i in range(s.layers):
+            w = {k: self.w[f"layer.{i}.{k}"] for k in s.LAYER_KEYS}
+            qkv = self._norm(x, w["attn_norm"]) @ self.w_qkv[i].T
+            q = qkv[:, :q_dim].unflatten(1, (s.q_heads, s.head_dim))
+            k = qkv[:, q_dim:q_dim + kv_dim].unflatten(1, (s.kv_heads, s.head_dim))
+            v = qkv[:, q_dim + kv_dim:].unflatten(1, (s.kv_heads, s.head_dim))
+            q, k = paged.qk_norm_rope(q, k, w["q_norm"], w["k_norm"], self.cos, self.sin, pos, eps=s.rms_eps)
+            self.cache.append(i, k, v, starts, at)
+            o = self.cache.attend(i, q, starts, at)
+            x = x + (o.flatten(1) @ w["w_o"].T).float()
+            gate, up = (self._norm(x, w["ffn_norm"]) @ self.w_gate_up[i].T).float().chunk(2, 1)
+            x = x + ((torch.nn.functional.silu(gate) * up).to(torch.bfloat16) @ w["w_down"].T).float()
+        return (self._norm(x, self.w["final_norm"]) @ self.w["embedding"].T).float(), starts
+
+    def generate(self, prompts, n_new, *, max_drafts=4, temperature=0.0, seed=0):
+        """n_new tokens after each prompt (token ids, at least one each).
+        temperature 0 picks the most likely token.  Returns (tokens per
+        sequence, number of model steps)."""
+        if len(prompts) > self.seqs or not all(prompts):
+            raise ValueError("at most `seqs` prompts, none of them empty")
+        if max(len(p) for p in prompts) + n_new > self.max_seq:
+            raise ValueError("prompt and new tokens exceed max_seq")
+        gen = torch.Generator(device=self.device).manual_seed(seed)
+        b = len(prompts)
+        for i in range(self.seqs):
+            self.cache.release(i)
+        text, held, steps = [list(p) for p in prompts], [0] * b, 0   # held: positions in the cache
+        goal = [len(p) + n_new for p in prompts]
+        while any(len(t) < g for t, g in zip(text, goal)):
+            fed, drafts = [], []
+            for t, h, g in zip(text, held, goal):
+                room = g - len(t)
+                d = lookup_draft(t, min(max_drafts, room - 1)) if room > 1 and h else []
+                drafts.append(d)
+                fed.append(t[h:] + d if room > 0 else [])
+            logits, starts = self.forward(fed + [[]] * (self.seqs - b), held + [0] * (self.seqs - b))
+            steps += 1
+            # verification looks at each sequence's last token and its drafts
+            n = [len(d) + 1 if f else 0 for f, d in zip(fed, drafts)]
+            ends = np.cumsum([len(f) for f in fed])
+            rows = [r for e, k in zip(ends, n) for r in range(e - k, e)]
+            kept = logits[self._int32(rows).long()]
+            if temperature > 0:
+                probs = torch.softmax(kept / temperature, 1)
+            else:
+                probs = torch.zeros_like(kept).scatter_(1, kept.argmax(1, keepdim=True), 1.0)
+            looked = self._int32([t for f, k in zip(fed, n) for t in f[len(f) - k:]])
+            u = torch.rand(len(rows), generator=gen, device=self.device)
+            su = torch.rand(b, generator=gen, device=self.device)
+            out, accepted = paged.verify_drafts(looked, probs, None, u, su,
+                                                self._int32(np.concatenate([[0], np.cumsum(n)]).tolist()))
+            out, accepted = out.tolist(), accepted.tolist()
+            at = 0
+            for i in range(b):
+                if n[i]:
+                    text[i] += out[at:at + accepted[i] + 1]
+                    # all but the newest token are in the cache; refused drafts will be written over
+                    held[i] = len(text[i]) - 1
+                at += n[i]
+        paged.check(self.device)
+        return [t[len(p):] for t, p in zip(text, prompts)], steps
+
+
+def main(argv=None):
+    ap = argparse.ArgumentParser(description="Decode random prompts with drafted tokens.")
+    ap.add_argument("--shape", choices=sorted(SHAPES), default="tiny")
+    ap.add_argument("--seqs", type=int, default=4)
+    ap.add_argument("--prompt", type=int, default=24)
+    ap.add_argument("--tokens", type=int, default=64)
+    ap.add_argument("--drafts", type=int, default=4)
+    ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--kv", choices=sorted(paged.KV_DTYPES), default="fp8")
+    a = ap.parse_args(argv)
+    shape = SHAPES[a.shape]
+    flat, offsets = W.flat_bytes(shape, W.random_weights(shape, 0))
+    dec = DraftedDecoder(flat, offsets, shape, seqs=a.seqs, max_seq=a.prompt + a.tokens, kv_dtype=a.kv)
+    prompts = [W.prompt_ids(shape, a.prompt, seed=i + 1) for i in range(a.seqs)]
+    start = time.perf_counter()
+    out, steps = dec.generate(prompts, a.tokens, max_drafts=a.drafts, temperature=a.temperature)
+    took = time.perf_counter() - start
+    for i, t in enumerate(out):
+        print(f"sequence {i}: {t}")
+    print(f"{a.seqs} x {a.tokens} tokens in {steps} steps, {a.seqs * a.tokens / took:.0f} tok/s")
+    return 0
+
+
+if __name__ == "__main__":
+    sys.exit(main())
