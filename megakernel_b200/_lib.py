@@ -7,8 +7,10 @@ caller gets an exception.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import subprocess
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -22,6 +24,10 @@ SOURCES = [os.path.join(CSRC, f) for f in ("megakernel.cu", "noalloc.cu", "decod
 # Translation units, compiled in parallel and linked into one library.
 UNITS = ["megakernel.cu", "tp.cu", "paged.cu", "kv8_attend.cu",
          "kv8_prompt.cu"]
+
+# The Python entry of the paged operators, compiled by the host compiler.
+BINDING = os.path.join(CSRC, "paged_binding.cpp")
+BINDING_PATH = os.path.join(PKG_DIR, "_paged" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
@@ -37,8 +43,48 @@ def nvcc() -> str:
     return cand if os.path.exists(cand) else "nvcc"
 
 
+def build_binding(force: bool = False) -> str:
+    """Compile the paged operators' Python entry against this torch if it is missing or older than its source."""
+    if not force and os.path.exists(BINDING_PATH):
+        made = os.path.getmtime(BINDING_PATH)
+        if all(os.path.getmtime(s) <= made for s in (BINDING, HEADER)):
+            return BINDING_PATH
+    import torch
+    from torch.utils import cpp_extension
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{i}" for i in include), BINDING, "-o", BINDING_PATH + ".tmp", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python", f"-Wl,-rpath,{libs}", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed:\n{r.stderr[-4000:]}")
+    os.replace(BINDING_PATH + ".tmp", BINDING_PATH)
+    return BINDING_PATH
+
+
+_BINDING = None
+
+
+def binding(make_status):
+    """The paged operators' Python entry, bound to the in-tree library (raises if either has not been built)."""
+    global _BINDING
+    if _BINDING is None:
+        if not os.path.exists(BINDING_PATH):
+            raise RuntimeError(f"{BINDING_PATH} is missing: run megakernel_b200._lib.build() (needs nvcc and g++)")
+        load()
+        spec = importlib.util.spec_from_file_location("megakernel_b200._paged", BINDING_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind(LIB_PATH, make_status)
+        _BINDING = mod
+    return _BINDING
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile libmegakernel.so in-tree if it is missing or older than its sources."""
+    """Compile libmegakernel.so in-tree, and the paged operators' Python entry, if missing or older than their sources."""
+    build_binding(force)
     if not force and os.path.exists(LIB_PATH):
         lib_m = os.path.getmtime(LIB_PATH)
         if all(os.path.getmtime(s) <= lib_m for s in SOURCES + [HEADER]):

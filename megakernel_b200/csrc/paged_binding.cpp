@@ -1,0 +1,391 @@
+// Python entry of the paged operators (megakernel_b200/paged.py): the checks of
+// their tensors, the allocation of their results and the call of the C ABI, in
+// one step each.  Written in Python these took 10 of the 13 us that a call with
+// one row lasts; here they take about two.
+//
+// The functions take positional arguments in the order of paged.py and raise
+// ValueError for what they refuse.  The C entries are looked up in the library
+// that bind() is given.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+#include <dlfcn.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/megakernel.h"
+
+namespace {
+
+using at::Tensor;
+
+struct Refused : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+void need(bool ok, const char* what) {
+  if (!ok) throw Refused(what);
+}
+
+struct Entries {
+  decltype(&megakernel_qk_norm_rope) norm_rope = nullptr;
+  decltype(&megakernel_kv8_append) append = nullptr;
+  decltype(&megakernel_kv8_read) read = nullptr;
+  decltype(&megakernel_kv8_attend) attend = nullptr;
+  decltype(&megakernel_kv8_attend_workspace) workspace = nullptr;
+  decltype(&megakernel_verify_drafts) verify = nullptr;
+  decltype(&megakernel_error_string) text = nullptr;
+} g_lib;
+
+constexpr int kMaxDevices = 64;
+int* g_status[kMaxDevices] = {};
+PyObject* g_make_status = nullptr;   // device index -> address of its status word
+
+int* status_of(int device) {
+  need(device >= 0 && device < kMaxDevices, "device index");
+  if (!g_status[device]) {
+    PyObject* r = g_make_status ? PyObject_CallFunction(g_make_status, "i", device) : nullptr;
+    if (!r) throw Refused("no status word");
+    g_status[device] = static_cast<int*>(PyLong_AsVoidPtr(r));
+    Py_DECREF(r);
+  }
+  return g_status[device];
+}
+
+void check(int rc, const char* what) {
+  if (rc != MK_OK)
+    throw std::runtime_error(std::string(what) + ": " + g_lib.text(rc) + " (" + std::to_string(rc) + ")");
+}
+
+// ---- arguments ---------------------------------------------------------------------
+const Tensor& tensor(PyObject* o, const char* what) {
+  need(THPVariable_Check(o), what);
+  return THPVariable_Unpack(o);
+}
+const Tensor* maybe(PyObject* o, const char* what) { return o == Py_None ? nullptr : &tensor(o, what); }
+
+int type_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return MK_TYPE_F32;
+    case at::kBFloat16: return MK_TYPE_BF16;
+    case at::kHalf: return MK_TYPE_F16;
+    default: return -1;
+  }
+}
+bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+struct Strides { long long row, head; };
+
+// Strides of a [rows, heads, head_dim] operand that is read in 16-byte vectors (0
+// for an axis of one element).
+Strides rows_of(const Tensor& t, const char* shape, const char* layout) {
+  need(t.dim() == 3 && t.is_cuda() && type_of(t) >= 0, shape);
+  const long long per = t.scalar_type() == at::kFloat ? 3 : 7;
+  const Strides s{t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
+  need((t.size(2) <= 1 || t.stride(2) == 1) && ((s.row | s.head) & per) == 0 && s.row >= 0 && s.head >= 0 && aligned16(t), layout);
+  return s;
+}
+void vector(const Tensor& t, at::ScalarType type, long long n, int device, const char* what) {
+  need(t.scalar_type() == type && t.is_cuda() && t.get_device() == device && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), what);
+}
+long long integer(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    throw Refused("a whole number is expected");
+  }
+  return v;
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    throw Refused("a number is expected");
+  }
+  return v;
+}
+
+struct CacheArgs {
+  mk_kv8 m;
+  int device;
+};
+
+CacheArgs cache_of(PyObject* const* a, long long rows) {
+  const Tensor &codes = tensor(a[0], "codes: a tensor"), &scales = tensor(a[1], "scales: a tensor"),
+               &table = tensor(a[2], "page_table: a tensor"), &starts = tensor(a[3], "starts: a tensor"),
+               &first = tensor(a[4], "first: a tensor");
+  const bool fp8 = codes.scalar_type() == at::kFloat8_e4m3fn;
+  need(codes.dim() == 5 && codes.is_cuda() && (fp8 || codes.scalar_type() == at::kChar) && codes.size(1) == 2,
+       "codes: CUDA float8_e4m3fn or int8 [pages, 2, kv_heads, page_size, head_dim]");
+  const long long pages = codes.size(0), hk = codes.size(2), page = codes.size(3), d = codes.size(4);
+  need(hk >= 1 && (page == 16 || page == 32 || page == 64) && (d == 64 || d == 128),
+       "codes: page_size 16, 32 or 64, head_dim 64 or 128");
+  const long long held = page * d, whole = 2 * hk * held;
+  need(codes.stride(4) == 1 && codes.stride(3) == d && (hk == 1 || codes.stride(2) == held) && codes.stride(1) == hk * held,
+       "codes: a page's codes contiguous");
+  CacheArgs c;
+  c.device = codes.get_device();
+  c.m.page_stride = pages > 1 ? codes.stride(0) : whole;
+  need(c.m.page_stride >= whole && c.m.page_stride % 16 == 0 && aligned16(codes), "codes: pages at multiples of 16 bytes, not overlapping");
+  need(scales.scalar_type() == at::kFloat && scales.is_cuda() && scales.get_device() == c.device && scales.dim() == 3 &&
+           scales.size(0) == pages && scales.size(1) == 2 && scales.size(2) == hk,
+       "scales: float32 [pages, 2, kv_heads] on the cache's device");
+  c.m.scale_stride = pages > 1 ? scales.stride(0) : 2 * hk;
+  need((hk == 1 || scales.stride(2) == 1) && scales.stride(1) == hk && c.m.scale_stride >= 2 * hk,
+       "scales: a page's scales contiguous, pages not overlapping");
+  need(table.dim() == 2 && table.scalar_type() == at::kInt && table.is_cuda() && table.get_device() == c.device,
+       "page_table: int32 [seqs, pages] on the cache's device");
+  const long long seqs = table.size(0), width = table.size(1);
+  c.m.table_stride = seqs > 1 ? table.stride(0) : width;
+  need((width <= 1 || table.stride(1) == 1) && c.m.table_stride >= width,
+       "page_table: a sequence's pages contiguous, rows not overlapping");
+  vector(starts, at::kInt, seqs + 1, c.device, "starts: contiguous int32 [seqs + 1] on the cache's device");
+  vector(first, at::kInt, seqs, c.device, "first: contiguous int32 [seqs] on the cache's device");
+  need(pages <= 0x7fffffff && width <= 0x7fffffff && seqs <= 0x7fffffff && rows <= 0x7fffffff && hk <= 0x7fffffff, "sizes: below 2^31");
+  c.m.d_codes = codes.data_ptr();
+  c.m.d_scales = static_cast<float*>(scales.data_ptr());
+  c.m.d_page_table = static_cast<const int*>(table.data_ptr());
+  c.m.d_starts = static_cast<const int*>(starts.data_ptr());
+  c.m.d_first = static_cast<const int*>(first.data_ptr());
+  c.m.num_pages = (int)pages;
+  c.m.table_width = (int)width;
+  c.m.kv_heads = (int)hk;
+  c.m.page_size = (int)page;
+  c.m.head_dim = (int)d;
+  c.m.format = fp8 ? MK_KV8_E4M3 : MK_KV8_INT8;
+  c.m.seqs = (int)seqs;
+  c.m.rows = (int)rows;
+  return c;
+}
+
+void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
+
+PyObject* both(const Tensor& a, const Tensor& b) {
+  PyObject* t = PyTuple_New(2);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(a));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(b));
+  return t;
+}
+
+// An exception of any kind becomes a Python one; nothing passes through the C API.
+template <class Fn>
+PyObject* guarded(Py_ssize_t n, Py_ssize_t want, Fn f) {
+  try {
+    need(n == want, "wrong number of arguments");
+    need(g_lib.attend != nullptr, "the library is not bound");
+    return f();
+  } catch (const Refused& e) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const c10::Error& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "paged operators: unknown error");
+  }
+  return nullptr;
+}
+
+// ---- the operators ------------------------------------------------------------------
+
+// q, k, q_gain, k_gain, cos, sin, positions, eps, q_out, k_out
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 10, [&]() -> PyObject* {
+    const Tensor &q = tensor(a[0], "q: a tensor"), &k = tensor(a[1], "k: a tensor"), &qg = tensor(a[2], "q_gain: a tensor"),
+                 &kg = tensor(a[3], "k_gain: a tensor"), &cos = tensor(a[4], "cos: a tensor"), &sin = tensor(a[5], "sin: a tensor"),
+                 &pos = tensor(a[6], "positions: a tensor");
+    const double eps = number(a[7]);
+    const Strides qs = rows_of(q, "q: CUDA [rows, heads, head_dim] of float32, bfloat16 or float16",
+                               "q: head_dim contiguous, rows and heads at multiples of 16 bytes");
+    const Strides ks = rows_of(k, "k: CUDA [rows, heads, head_dim] of float32, bfloat16 or float16",
+                               "k: head_dim contiguous, rows and heads at multiples of 16 bytes");
+    const int dev = q.get_device();
+    const auto type = q.scalar_type();
+    const long long rows = q.size(0), hq = q.size(1), d = q.size(2), hk = k.size(1);
+    need(k.size(0) == rows && k.size(2) == d && k.scalar_type() == type && k.get_device() == dev, "k: q's rows, head_dim, dtype and device");
+    need(d == 64 || d == 128, "head_dim: 64 or 128");
+    vector(qg, type, d, dev, "q_gain: contiguous [head_dim] of q's dtype and device");
+    vector(kg, type, d, dev, "k_gain: contiguous [head_dim] of q's dtype and device");
+    need(cos.dim() == 2 && sin.dim() == 2 && cos.size(1) == d / 2 && cos.sizes() == sin.sizes() && cos.scalar_type() == at::kFloat &&
+             sin.scalar_type() == at::kFloat && cos.is_cuda() && sin.is_cuda() && cos.get_device() == dev && sin.get_device() == dev &&
+             cos.is_contiguous() && sin.is_contiguous(),
+         "cos, sin: contiguous float32 [positions, head_dim / 2] on q's device");
+    need(aligned16(qg) && aligned16(kg) && aligned16(cos) && aligned16(sin), "q_gain, k_gain, cos, sin: 16-byte aligned");
+    vector(pos, at::kInt, rows, dev, "positions: contiguous int32 [rows] on q's device");
+    need(eps >= 0.0, "eps: not negative");
+    need(rows <= 0x7fffffff && hq <= 0x7fffffff && hk <= 0x7fffffff && cos.size(0) <= 0x7fffffff, "sizes: below 2^31");
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != dev) guard.set_index(dev);
+    auto out_of = [&](PyObject* o, const Tensor& in, Strides* s, const char* what) {
+      if (o == Py_None) {
+        *s = {in.size(1) * d, d};
+        return at::empty(in.sizes(), in.options());
+      }
+      const Tensor& t = tensor(o, what);
+      need(t.sizes() == in.sizes() && t.scalar_type() == type && t.is_cuda() && t.get_device() == dev, what);
+      *s = rows_of(t, what, what);
+      return t;
+    };
+    Strides qos, kos;
+    const Tensor qo = out_of(a[8], q, &qos, "q_out: q's shape, dtype and device, rows and heads at multiples of 16 bytes");
+    const Tensor ko = out_of(a[9], k, &kos, "k_out: k's shape, dtype and device, rows and heads at multiples of 16 bytes");
+    const mk_qk_norm_rope m{q.data_ptr(), k.data_ptr(), qg.data_ptr(), kg.data_ptr(), qo.data_ptr(), ko.data_ptr(),
+                            static_cast<const float*>(cos.data_ptr()), static_cast<const float*>(sin.data_ptr()),
+                            static_cast<const int*>(pos.data_ptr()), qs.row, qs.head, ks.row, ks.head, qos.row, qos.head, kos.row,
+                            kos.head, (int)cos.size(0), (int)rows, (int)hq, (int)hk, (int)d, type_of(q), (float)eps};
+    check(g_lib.norm_rope(&m, status_of(dev), stream_of(dev)), "megakernel_qk_norm_rope");
+    return both(qo, ko);
+  });
+}
+
+// codes, scales, page_table, starts, first, k, v
+PyObject* kv8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject* {
+    const Tensor &k = tensor(a[5], "k: a tensor"), &v = tensor(a[6], "v: a tensor");
+    const Strides ks = rows_of(k, "k: CUDA [rows, kv_heads, head_dim] of float32, bfloat16 or float16",
+                               "k: head_dim contiguous, rows and heads at multiples of 16 bytes");
+    const Strides vs = rows_of(v, "v: CUDA [rows, kv_heads, head_dim] of float32, bfloat16 or float16",
+                               "v: head_dim contiguous, rows and heads at multiples of 16 bytes");
+    const CacheArgs c = cache_of(a, k.size(0));
+    need(k.sizes() == v.sizes() && k.size(1) == c.m.kv_heads && k.size(2) == c.m.head_dim && k.scalar_type() == v.scalar_type() &&
+             k.get_device() == c.device && v.get_device() == c.device,
+         "k, v: one shape [rows, kv_heads, head_dim] and dtype, on the cache's device");
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != c.device) guard.set_index(c.device);
+    check(g_lib.append(&c.m, k.data_ptr(), ks.row, ks.head, v.data_ptr(), vs.row, vs.head, type_of(k), status_of(c.device),
+                       stream_of(c.device)),
+          "megakernel_kv8_append");
+    Py_RETURN_NONE;
+  });
+}
+
+// codes, scales, page_table, starts, first, rows, type
+PyObject* kv8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject* {
+    const long long rows = integer(a[5]), type = integer(a[6]);
+    need(rows >= 0, "rows: not negative");
+    const CacheArgs c = cache_of(a, rows);
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != c.device) guard.set_index(c.device);
+    const auto options = THPVariable_Unpack(a[1]).options().dtype(type == MK_TYPE_F32 ? at::kFloat : type == MK_TYPE_BF16 ? at::kBFloat16 : at::kHalf);
+    const Tensor k = at::empty({rows, c.m.kv_heads, c.m.head_dim}, options), v = at::empty({rows, c.m.kv_heads, c.m.head_dim}, options);
+    check(g_lib.read(&c.m, k.data_ptr(), v.data_ptr(), (int)type, status_of(c.device), stream_of(c.device)), "megakernel_kv8_read");
+    return both(k, v);
+  });
+}
+
+// codes, scales, page_table, starts, first, q, kv_lens, sm_scale, causal, window, out, return_lse
+PyObject* kv8_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 12, [&]() -> PyObject* {
+    const Tensor& q = tensor(a[5], "q: a tensor");
+    const Strides qs = rows_of(q, "q: CUDA [rows, q_heads, head_dim]", "q: head_dim contiguous, rows and heads at multiples of 16 bytes");
+    const long long rows = q.size(0), hq = q.size(1);
+    const CacheArgs c = cache_of(a, rows);
+    need(q.scalar_type() != at::kFloat && q.get_device() == c.device && q.size(2) == c.m.head_dim,
+         "q: bfloat16 or float16 [rows, q_heads, head_dim] on the cache's device");
+    need(hq >= 1 && hq % c.m.kv_heads == 0 && hq <= 65535, "q_heads: a multiple of kv_heads, at most 65,535");
+    need(c.m.seqs > 0 || rows == 0, "rows without a sequence");
+    const Tensor* lens = maybe(a[6], "kv_lens: a tensor");
+    if (lens) vector(*lens, at::kInt, c.m.seqs, c.device, "kv_lens: contiguous int32 [seqs] on the cache's device");
+    const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)c.m.head_dim) : number(a[7]);
+    need(scale > 0.0 && scale < 3e38, "sm_scale: positive");
+    const int causal = PyObject_IsTrue(a[8]), lse_too = PyObject_IsTrue(a[11]);
+    const long long window = integer(a[9]);
+    need(window >= 0 && window <= 0x7fffffff, "window: not negative");
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != c.device) guard.set_index(c.device);
+    const Tensor* given = maybe(a[10], "out: a tensor");
+    if (given)
+      need(given->sizes() == q.sizes() && given->scalar_type() == q.scalar_type() && given->is_cuda() && given->get_device() == c.device &&
+               given->is_contiguous() && aligned16(*given),
+           "out: contiguous, of q's shape, dtype and device");
+    const Tensor out = given ? *given : at::empty(q.sizes(), q.options());
+    const Tensor& scales = THPVariable_Unpack(a[1]);
+    Tensor lse, work;
+    if (lse_too) lse = at::empty({rows, hq}, scales.options());
+    const long long bytes = g_lib.workspace(&c.m, (int)hq);
+    if (bytes < 0) check((int)bytes, "megakernel_kv8_attend_workspace");
+    if (bytes > 0) work = at::empty({(bytes + 3) / 4}, scales.options());
+    check(g_lib.attend(&c.m, q.data_ptr(), qs.row, qs.head, (int)hq, type_of(q), (float)scale, causal, (int)window,
+                       lens ? static_cast<const int*>(lens->data_ptr()) : nullptr, out.data_ptr(),
+                       lse_too ? static_cast<float*>(lse.data_ptr()) : nullptr, bytes > 0 ? work.data_ptr() : nullptr, bytes,
+                       status_of(c.device), stream_of(c.device)),
+          "megakernel_kv8_attend");
+    return lse_too ? both(out, lse) : THPVariable_Wrap(out);
+  });
+}
+
+// tokens, target_probs, draft_probs, uniforms, sample_u, starts
+PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    const Tensor &tokens = tensor(a[0], "tokens: a tensor"), &target = tensor(a[1], "target_probs: a tensor"),
+                 &u = tensor(a[3], "uniforms: a tensor"), &su = tensor(a[4], "sample_u: a tensor"), &starts = tensor(a[5], "starts: a tensor");
+    const Tensor* draft = maybe(a[2], "draft_probs: a tensor");
+    need(target.dim() == 2 && target.is_cuda() && target.scalar_type() == at::kFloat, "target_probs: CUDA float32 [rows, vocab]");
+    const int dev = target.get_device();
+    const long long rows = target.size(0), vocab = target.size(1);
+    need(vocab >= 1 && starts.dim() == 1 && starts.size(0) >= 1, "vocab: at least one token; starts: int32 [seqs + 1]");
+    const long long seqs = starts.size(0) - 1;
+    vector(starts, at::kInt, seqs + 1, dev, "starts: contiguous int32 [seqs + 1] on target_probs' device");
+    vector(tokens, at::kInt, rows, dev, "tokens: contiguous int32 [rows] on target_probs' device");
+    vector(u, at::kFloat, rows, dev, "uniforms: contiguous float32 [rows] on target_probs' device");
+    vector(su, at::kFloat, seqs, dev, "sample_u: contiguous float32 [seqs] on target_probs' device");
+    if (draft)
+      need(draft->sizes() == target.sizes() && draft->scalar_type() == at::kFloat && draft->is_cuda() && draft->get_device() == dev,
+           "draft_probs: float32, of target_probs' shape and device");
+    const long long t0 = rows > 1 ? target.stride(0) : vocab, d0 = draft && rows > 1 ? draft->stride(0) : vocab;
+    need((vocab == 1 || (target.stride(1) == 1 && (!draft || draft->stride(1) == 1))) && t0 >= vocab && d0 >= vocab,
+         "probabilities: vocab contiguous, rows not overlapping");
+    need(rows <= 0x7fffffff && vocab <= 0x7fffffff && seqs <= 0x7fffffff, "sizes: below 2^31");
+    c10::cuda::OptionalCUDAGuard guard;
+    if (c10::cuda::current_device() != dev) guard.set_index(dev);
+    const Tensor out = at::empty({rows}, tokens.options()), accepted = at::empty({seqs}, tokens.options());
+    check(g_lib.verify(static_cast<const int*>(tokens.data_ptr()), static_cast<const float*>(target.data_ptr()), t0,
+                       draft ? static_cast<const float*>(draft->data_ptr()) : nullptr, d0, static_cast<const float*>(u.data_ptr()),
+                       static_cast<const float*>(su.data_ptr()), static_cast<const int*>(starts.data_ptr()), (int)seqs, (int)rows,
+                       (int)vocab, static_cast<int*>(out.data_ptr()), static_cast<int*>(accepted.data_ptr()), status_of(dev),
+                       stream_of(dev)),
+          "megakernel_verify_drafts");
+    return both(out, accepted);
+  });
+}
+
+// bind(path, make_status): the library to call, and where status words come from.
+PyObject* bind(PyObject*, PyObject* args) {
+  const char* path;
+  PyObject* make;
+  if (!PyArg_ParseTuple(args, "sO", &path, &make)) return nullptr;
+  void* h = dlopen(path, RTLD_NOW | RTLD_LOCAL);
+  if (!h) {
+    PyErr_Format(PyExc_RuntimeError, "%s: %s", path, dlerror());
+    return nullptr;
+  }
+  Entries e;
+  auto find = [&](auto& f, const char* name) { return (f = reinterpret_cast<std::decay_t<decltype(f)>>(dlsym(h, name))) != nullptr; };
+  if (!find(e.norm_rope, "megakernel_qk_norm_rope") || !find(e.append, "megakernel_kv8_append") || !find(e.read, "megakernel_kv8_read") ||
+      !find(e.attend, "megakernel_kv8_attend") || !find(e.workspace, "megakernel_kv8_attend_workspace") ||
+      !find(e.verify, "megakernel_verify_drafts") || !find(e.text, "megakernel_error_string")) {
+    PyErr_Format(PyExc_RuntimeError, "%s lacks a paged operator", path);
+    return nullptr;
+  }
+  g_lib = e;
+  Py_INCREF(make);
+  Py_XSETREF(g_make_status, make);
+  for (int*& s : g_status) s = nullptr;
+  Py_RETURN_NONE;
+}
+
+#define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef kMethods[] = {FAST(qk_norm_rope), FAST(kv8_append), FAST(kv8_read), FAST(kv8_attend), FAST(verify_drafts),
+                          {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_paged", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__paged() { return PyModule_Create(&kModule); }
