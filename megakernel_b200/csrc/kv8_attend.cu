@@ -52,9 +52,9 @@ __device__ __forceinline__ int parts_of(int steps, int run) {
   return n - ((n - 1) * run >= steps && n > 0);
 }
 
-// The sequences 128 at a time, four to a lane, so that their loads do not wait
+// The sequences 64 at a time, two to a lane, so that their loads do not wait
 // for one another.
-constexpr int kPer = 4;
+constexpr int kPer = 2;
 struct Chunk { int steps[kPer], tiles[kPer]; };
 
 template <int P, int TS, int R>
@@ -139,7 +139,7 @@ __device__ __forceinline__ int seq_of_part(const Cache& c, const Attend& a, int 
       if (lane >= o) upto += other;
     }
     upto += before;
-    // the sequence within the lane's four, and what lies before it
+    // the sequence within the lane's two, and what lies before it
     int at = upto - mine, found = kPer;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -157,6 +157,50 @@ __device__ __forceinline__ int seq_of_part(const Cache& c, const Attend& a, int 
   }
   *base_part = before;
   return -1;
+}
+
+// The plan of a block: made by its first warp, for up to 64 sequences with the
+// number of parts up to and with each.  (By each of the 16 warps of an SM for
+// itself it took 3.5 us of issue slots; 64 sequences.)
+struct SharedPlan {
+  Plan p;
+  int upto[32 * kPer];
+};
+
+template <int P, int TS, int R>
+__device__ __forceinline__ void share_plan(const Cache& c, const Attend& a, int group, int warps, int* status, SharedPlan* out) {
+  if (threadIdx.x < 32) {
+    Chunk k;
+    const Plan p = make_plan<P, TS, R>(c, a, group, warps, status, &k);
+    int n[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine += n[i] = k.tiles[i] * parts_of(k.steps[i], p.run) * c.kv_heads;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, upto, o);
+      if ((int)threadIdx.x >= o) upto += other;
+    }
+    upto -= mine;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out->upto[threadIdx.x * kPer + i] = upto += n[i];
+    if (threadIdx.x == 0) out->p = p;
+  }
+  __syncthreads();
+}
+
+// seq_of_part with the shared plan.
+template <int P, int TS, int R>
+__device__ __forceinline__ int find_part(const Cache& c, const Attend& a, int group, const SharedPlan& s, int x, int seq, int* base_part) {
+  if (c.seqs > 32 * kPer)
+    return seq_of_part<P, TS, R>(c, a, group, s.p, load_chunk<P, TS, R>(c, a, 0, group, nullptr), x, seq, base_part);
+  if (seq < 0) {
+    seq = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) seq += __popc(__ballot_sync(0xffffffffu, s.upto[i * 32 + (threadIdx.x & 31)] <= x));
+  }
+  *base_part = seq ? s.upto[seq - 1] : 0;
+  return seq < c.seqs ? seq : -1;
 }
 
 // A part in the workspace: R x D sums, then m and l of each row, then whether a NaN was taken out.
@@ -221,15 +265,11 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
   __syncwarp();
 
   int x = warp * (int)gridDim.x + (int)blockIdx.x;   // the part; neighbours go to different SMs
-  int b, base_part;
-  Plan plan;
-  {
-    Chunk chunk;
-    plan = make_plan<P, TS, R>(c, a, group, (int)gridDim.x * kWarps,
-                               blockIdx.x == 0 && warp == 0 ? a.status : nullptr, &chunk);
-    if (x >= plan.parts) return;
-    b = seq_of_part<P, TS, R>(c, a, group, plan, chunk, x, -1, &base_part);
-  }
+  __shared__ SharedPlan s_plan;
+  share_plan<P, TS, R>(c, a, group, (int)gridDim.x * kWarps, blockIdx.x == 0 ? a.status : nullptr, &s_plan);
+  const Plan plan = s_plan.p;
+  if (x >= plan.parts) return;
+  int base_part, b = find_part<P, TS, R>(c, a, group, s_plan, x, -1, &base_part);
   int slot = 0;
   uint32_t phase = 0;   // of ring slot `slot`; slots are used in turn over all parts
 
@@ -582,7 +622,7 @@ attend_rows_kernel(const Cache c, const Attend a, float* work) {
       }
     x += (int)gridDim.x * kWarps;
     if (x >= plan.parts) return;
-    b = seq_of_part<P, TS, R>(c, a, group, plan, load_chunk<P, TS, R>(c, a, 0, group, nullptr), x, -1, &base_part);
+    b = find_part<P, TS, R>(c, a, group, s_plan, x, -1, &base_part);
   }
 }
 
@@ -597,18 +637,18 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const Cache c
   const int row = (int)(unit / a.q_heads), hq = (int)(unit % a.q_heads), h = hq / group;
   int b = -1, parts = 1, first_part = 0, m = 0, tile_first = 0;
   SeqWork w;
+  __shared__ SharedPlan s_plan;
+  share_plan<P, TS, R>(c, a, group, warps, nullptr, &s_plan);
   if (row < c.rows) {
-    Chunk chunk;
-    const Plan plan = make_plan<P, TS, R>(c, a, group, warps, nullptr, &chunk);
     b = warp_search(c.seqs, row, [&](int i) { return __ldg(c.starts + i); });
     w = seq_work<P, TS, R>(c, a, b, group);
     if (row < w.r0 || row >= w.r0 + w.n) b = -1;   // of no sequence
     if (b >= 0) {
       int base_part;
-      seq_of_part<P, TS, R>(c, a, group, plan, chunk, 0, b, &base_part);
+      find_part<P, TS, R>(c, a, group, s_plan, 0, b, &base_part);
       m = (row - w.r0) * group + hq % group;
       tile_first = m / R * R;
-      parts = parts_of(w.steps, plan.run);
+      parts = parts_of(w.steps, s_plan.p.run);
       first_part = base_part + (m / R * c.kv_heads + h) * parts;
     }
   }

@@ -115,17 +115,17 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 
 constexpr int kTile = 128;                       // rows of a query tile
 constexpr int kStep = 64;                        // positions of a step
-constexpr int kRowWarps = 8, kCodeWarps = 8;     // two query tiles; converters
-constexpr int kMmaWarp = kRowWarps + kCodeWarps, kCopyWarp = kMmaWarp + 2;
-constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 4) * 32;
-// Registers a thread of each role keeps; the block starts with 96 each, and the
-// sum over the five warpgroups is the launch's 480.
-constexpr int kRowRegs = 168, kCodeRegs = 48, kMmaRegs = 48;
+constexpr int kRowWarps = 16, kCodeWarps = 8;    // two query tiles, two warps to 32 rows; converters
+constexpr int kMmaWarp = kRowWarps + kCodeWarps, kCopyWarp = kMmaWarp + 4;
+constexpr int kPromptThreads = (kRowWarps + kCodeWarps + 8) * 32;
+// Registers a thread of each role keeps; the block starts with 64 each, and the
+// sum over the eight warpgroups is the launch's 512.
+constexpr int kRowRegs = 80, kCodeRegs = 48, kMmaRegs = 48;
 // Weights 2^kBase p in f16, p up to 2^kMove: the reference moves less often than in
 // kv8_attend.cu (a move costs a pass over the output), and what is lost below is
 // 2^-31 of the row's reference.
 constexpr float kBase = 6.f, kMove = 9.f;
-constexpr int kMetaSlots = 16;   // the copies run at most nine steps ahead of the softmax
+constexpr int kMetaSlots = 8;   // the copies run at most six steps ahead of the softmax
 
 template <int D>
 struct PromptSmem {
@@ -140,12 +140,12 @@ struct PromptSmem {
 // ---- attention of many rows per sequence ---------------------------------------------------
 //
 // Work item: 256 rows of one (sequence, kv head), as two tiles of 128, all their
-// positions in steps of 64.  Roles of a block's five warpgroups:
-//   warps 0-3, 4-7   one tile of rows each, one row per thread: softmax
-//   warps 8-15       8-bit codes to f16 operands, shared memory to shared memory
-//   warps 16, 17     one lane of each issues the products of one tile
-//   warp 18          looks pages and scales up and copies their codes to shared
-//                    memory (19 only gives its registers away)
+// positions in steps of 64.  Roles of a block's eight warpgroups:
+//   warps 0-7, 8-15  one tile of rows each, half a row's scores per thread: softmax
+//   warps 16-23      8-bit codes to f16 operands, shared memory to shared memory
+//   warps 24, 25     one lane of each issues P V of one tile, 26, 27 Q K^T
+//   warp 28          looks pages and scales up and copies their codes to shared
+//                    memory (29-31 only give their registers away)
 // S = Q K^T [128 x 64], two steps of it per tile, and O [128 x D] live in tensor
 // memory (all 512 columns for D = 128); the weights go back to tensor memory as
 // f16, over their scores, and are the A operand of O += P V.  While a tile's
@@ -167,21 +167,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   constexpr int kSub = kStep / P;                    // pages of a step
   constexpr int kStages = S::kStages, kRawStages = S::kRawStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* smem = smem_raw;   // all of it is used: no room to align it here
   __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   __shared__ __align__(8) uint64_t q_full, s_full[2][2], p_full[2][2];   // [tile][score buffer]
-  // P V of one step, of the last step: two may be outstanding there, and a parity
-  // tells only two neighbours apart
-  __shared__ __align__(8) uint64_t o_done[2], o_full[2], o_drain[2];
+  // P V of a step, by tile and score buffer (two may be outstanding, and a parity
+  // tells only two neighbours apart); of the last step
+  __shared__ __align__(8) uint64_t o_done[2][2], o_full[2], drain[4];
   __shared__ __align__(8) uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];   // codes of K, of V
   // of a step: scales of the K pages (0: not there), of the V pages relative to
   // s_vref, the largest V scale up to it; whether all its pages are there
   __shared__ float s_ks[kMetaSlots][kSub], s_vf[kMetaSlots][kSub], s_vref[kMetaSlots];
   __shared__ int s_there[kMetaSlots];
+  // of a row: what its two threads tell one another; before, the factor of its scores
+  __shared__ float s_half[2][2 * kTile];
+  float* s_rq = s_half[0];
+  __shared__ int s_stop[kRowWarps / 2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_nan;
   __shared__ volatile int s_abort;
 
+  if (mk::smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) report(a.status, MK_ERR_LAUNCH);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = a.q_heads / c.kv_heads;
   // items in reverse: the last tiles of a sequence see the most positions
@@ -217,23 +225,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   if (threadIdx.x == 0) {
     s_nan = 0;
     s_abort = 0;
+    for (int i = 0; i < kRowWarps / 2; ++i) s_stop[i] = 0;
     mk::mbar_init(&q_full, kRowWarps * 32);
     for (int i = 0; i < kStages; ++i) {
-      mk::mbar_init(&k_full[i], kCodeWarps * 32);
-      mk::mbar_init(&v_full[i], kCodeWarps * 32);
+      mk::mbar_init(&k_full[i], 64);
+      mk::mbar_init(&v_full[i], 64);
       mk::mbar_init(&k_empty[i], 2);   // both tiles' products
       mk::mbar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mk::mbar_init(&s_full[i][0], 1);
       mk::mbar_init(&s_full[i][1], 1);
-      mk::mbar_init(&p_full[i][0], 128);   // one per buffer: a tile may be two steps of weights ahead
-      mk::mbar_init(&p_full[i][1], 128);
-      mk::mbar_init(&o_done[i], 1);
+      mk::mbar_init(&p_full[i][0], 256);   // one per buffer: a tile may be two steps of weights ahead
+      mk::mbar_init(&p_full[i][1], 256);
+      mk::mbar_init(&o_done[i][0], 1);
+      mk::mbar_init(&o_done[i][1], 1);
       mk::mbar_init(&o_full[i], 1);
       for (int k = 0; k < kRawStages; ++k) {
         mk::mbar_init(&raw_full[i][k], kSub);
-        mk::mbar_init(&raw_empty[i][k], kCodeWarps);
+        mk::mbar_init(&raw_empty[i][k], 2);
       }
     }
     mk::fence_mbar_init();
@@ -260,16 +270,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   const uint32_t tm = s_tmem, smem0 = mk::smem_u32(smem);
   if (warp < kRowWarps) {
     mk::setmaxnreg_inc<kRowRegs>();
-    const int x = warp >> 2, r = threadIdx.x & 127;   // tile, and row of this thread
-    const int m_row = row0 + x * kTile + r;
-    // ---- 32 rows of Q per warp to f16, K contiguous, swizzled; D / 8 lanes per row
-    float rq = 0.f;
+    // tile, half of the columns, row in the tile and in the item; the two warps of
+    // 32 rows meet at barrier 1 + pair
+    const int x = warp >> 3, half = warp >> 2 & 1, pair = x * 4 + (warp & 3), r = (warp & 3) * 32 + lane, rr = x * kTile + r;
+    const int m_row = row0 + rr;
+    // ---- 16 rows of Q per warp to f16, K contiguous, swizzled; D / 8 lanes per row
     {
-      constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes, kLoads = 32 / kRowsPer;
+      constexpr int kLanes = D / 8, kRowsPer = 32 / kLanes, kLoads = 16 / kRowsPer;
       uint4 raw[kLoads];
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int m = row0 + warp * 32 + i * kRowsPer + lane / kLanes;
+        const int m = row0 + warp * 16 + i * kRowsPer + lane / kLanes;
         const uint16_t* src = (const uint16_t*)a.q + (long long)(w.r0 + m / group) * a.q_row + (h * group + m % group) * a.q_head;
         raw[i] = m <= row_last ? __ldg(reinterpret_cast<const uint4*>(src) + lane % kLanes) : make_uint4(0, 0, 0, 0);
       }
@@ -283,65 +294,71 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int ex = min(max((int)(__float_as_uint(top) >> 23), 30), 240);   // as in kv8_attend.cu
         const float up = __uint_as_float((uint32_t)(127 + 127 + 14 - ex) << 23);
-        const float back = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
-        const float mine = __shfl_sync(0xffffffffu, back, lane % kRowsPer * kLanes);
-        if (lane / kRowsPer == i) rq = mine;
-        const int row = (warp & 3) * 32 + i * kRowsPer + lane / kLanes, ch = lane % kLanes;
-        *reinterpret_cast<uint4*>(smem + S::kQ + x * S::kTileBytes + ch / 8 * (kTile * 128) + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
+        const int all_row = warp * 16 + i * kRowsPer + lane / kLanes, t = all_row / kTile, row = all_row % kTile, ch = lane % kLanes;
+        if (ch == 0) s_rq[all_row] = a.scale * __uint_as_float((uint32_t)(ex - 14) << 23);
+        *reinterpret_cast<uint4*>(smem + S::kQ + t * S::kTileBytes + ch / 8 * (kTile * 128) + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
             make_uint4(pack_f16(v[0] * up, v[1] * up), pack_f16(v[2] * up, v[3] * up), pack_f16(v[4] * up, v[5] * up),
                        pack_f16(v[6] * up, v[7] * up));
       }
       fence_async_shared();
       mk::mbar_arrive(&q_full);
     }
-    // ---- softmax of one row
+    bool ok = wait_warp(&q_full, 0);
+    const float rq = s_rq[rr];
+    // ---- softmax: 32 of a row's 64 scores of a step
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;   // lanes 32 (warp % 4) ..
-    const uint32_t to = tm + 2 * kTile + x * D + quarter;
+    const uint32_t to = tm + 2 * kTile + x * D + half * (D / 2) + quarter;
     int lo, hi;
     row_sees(w, a, group, m_row, lo, hi);
     const int my_lo = x ? j_lo[1] : j_lo[0], my_hi = x ? j_hi[1] : j_hi[0];
     const int lo_max = x ? own[1].lo_max : own[0].lo_max, hi_min = x ? own[1].hi_min : own[0].hi_min;
+    constexpr int kRun = P < 32 ? P : 32, kParts = 32 / kRun;   // columns of one page; pages of a thread's columns
     float m = kNone, l = 0.f, vref = 0.f;
-    bool ok = true;
     uint32_t phase = 0;   // bit i: of score buffer i
     for (int j = my_lo; j < my_hi; ++j) {
-      const int buf = j & 1, pos = j * kStep, slot = j % kMetaSlots;
+      const int buf = j & 1, pos = j * kStep + 32 * half, slot = j % kMetaSlots;
       const uint32_t ts = tm + x * kTile + buf * kStep + quarter;
-      if (!(ok = wait_warp(&s_full[x][buf], phase >> buf & 1))) break;
+      if (ok) ok = wait_warp(&s_full[x][buf], phase >> buf & 1);
       phase ^= 1u << buf;
       mk::tc_fence_after();
-      float v[2][32];
+      float v[32];
+      tmem_ld_f32x32(ts + 32 * half, v);
+      const bool whole = s_there[slot] && j * kStep >= lo_max && (j + 1) * kStep <= hi_min;
+      const float* ks = &s_ks[slot][32 * half / P];
+      float f[kParts];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) tmem_ld_f32x32(ts + 32 * q, v[q]);
-      const bool whole = s_there[slot] && pos >= lo_max && pos + kStep <= hi_min;
-      float f[kSub];
-#pragma unroll
-      for (int i = 0; i < kSub; ++i) f[i] = fmaxf(rq * s_ks[slot][i], 1.17549435e-38f);   // -inf x 0 would be NaN
+      for (int i = 0; i < kParts; ++i) f[i] = fmaxf(rq * ks[i], 1.17549435e-38f);   // -inf x 0 would be NaN
       const float vnow = s_vref[slot];
+      tmem_arrived(v);
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (pos + i < lo || pos + i >= hi || ks[i / kRun] == 0.f) v[i] = -INFINITY;
+      }
       float top = kNone;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        tmem_arrived(v[q]);
-        if (!whole) {
+      for (int i0 = 0; i0 < 32; i0 += kRun) {
+        float t[4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (pos + 32 * q + i < lo || pos + 32 * q + i >= hi || s_ks[slot][(32 * q + i) / P] == 0.f) v[q][i] = -INFINITY;
-        }
-        constexpr int kRun = P < 32 ? P : 32;   // columns of one page
+        for (int i = 0; i < 4; ++i) t[i] = fmaxf(fmaxf(v[i0 + i], v[i0 + 4 + i]), v[i0 + 8 + i]);
 #pragma unroll
-        for (int i0 = 0; i0 < 32; i0 += kRun) {
-          float t[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) t[i] = fmaxf(fmaxf(v[q][i0 + i], v[q][i0 + 4 + i]), v[q][i0 + 8 + i]);
-#pragma unroll
-          for (int i = 12; i < kRun; ++i) t[i & 3] = fmaxf(t[i & 3], v[q][i0 + i]);
-          top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f[(32 * q + i0) / P]);
-        }
+        for (int i = 12; i < kRun; ++i) t[i & 3] = fmaxf(t[i & 3], v[i0 + i]);
+        top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f[i0 / kRun]);
       }
-      const bool move = top > m + kMove;
-      if (__any_sync(0xffffffffu, move) || vnow > vref) {
+      // Here both warps have their scores in registers (the weights go over some of
+      // them), and a row whose reference moves does so in both.  A warp that gave up
+      // waiting comes along, so that neither is left at the barrier.
+      if (mk::bar_any(1 + pair, 64, !ok || top > m + kMove || vnow > vref)) {
+        s_half[half][rr] = top;
+        if (!ok) s_stop[pair] = 1;
+        mk::bar_any(1 + pair, 64, false);
+        if (s_stop[pair]) {
+          ok = false;
+          break;
+        }
+        top = fmaxf(top, s_half[half ^ 1][rr]);
         float keep = vnow > vref ? vref / vnow : 1.f;
-        if (move) {
+        if (top > m + kMove) {
           const float k = ex2(m - top);
           l *= k;
           keep *= k;
@@ -349,10 +366,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         }
         vref = vnow;
         if (j > my_lo) {   // once P V of the step before is complete
-          if (!(ok = wait_warp(&o_done[x], (j - 1 - my_lo) & 1))) break;
+          ok = wait_warp(&o_done[x][buf ^ 1], (j - 1 - my_lo) >> 1 & 1);
           mk::tc_fence_after();
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 16) {
+          for (int c0 = 0; c0 < D / 2; c0 += 16) {
             uint32_t o[16];
             tmem_ld_x16(to + c0, o);
             tmem_arrived(o);
@@ -364,33 +381,36 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       }
       const float back = kBase - m;   // weights are 2^kBase p
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t p[16];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t p[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          fma2(v[q][i], v[q][i + 1], f[(32 * q + i) / P], back);
-          const float e0 = ex2(v[q][i]), e1 = ex2(v[q][i + 1]);
-          add2(sum[i & 2], sum[(i & 2) + 1], e0, e1);
-          p[i / 2] = pack_f16(e0, e1);
-        }
-        tmem_st_x16(ts + 16 * q, p);
+      for (int i = 0; i < 32; i += 2) {
+        fma2(v[i], v[i + 1], f[i / kRun], back);
+        const float e0 = ex2(v[i]), e1 = ex2(v[i + 1]);
+        add2(sum[i & 2], sum[(i & 2) + 1], e0, e1);
+        p[i / 2] = pack_f16(e0, e1);
       }
+      tmem_st_x16(ts + 16 * half, p);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       mk::tc_fence_before();
-      mk::mbar_arrive(&p_full[x][buf]);
+      if (ok) mk::mbar_arrive(&p_full[x][buf]);
     }
     // ---- write the rows: through the tile's place in shared memory, which every
     // product has read by then, for whole rows at a time
     if (ok && my_hi > my_lo) ok = wait_warp(&o_full[x], 0);
+    mk::tc_fence_after();
+    const bool any = ok && my_hi > my_lo;   // else that place may still be written, and only zeros are due
+    mk::bar_any(1 + pair, 64, false);       // s_half is free
+    s_half[half][rr] = l;
+    if (!ok) s_stop[pair] = 1;
+    mk::bar_any(1 + pair, 64, false);
+    l += s_half[half ^ 1][rr];
+    ok = !s_stop[pair];
     if (ok && x < tiles) {
-      mk::tc_fence_after();
       const float inv = l == 0.f ? 0.f : vref / l;   // nothing seen: 0
       uint8_t* mine = smem + S::kQ + x * S::kTileBytes + (warp & 3) * 32 * (D * 2);
-      const bool any = my_hi > my_lo;   // else that place may still be written, and only zeros are due
 #pragma unroll 1
-      for (int c0 = 0; any && c0 < D; c0 += 32) {
+      for (int c0 = 0; any && c0 < D / 2; c0 += 32) {
         float o[32];
         tmem_ld_f32x32(to + c0, o);
         tmem_arrived(o);
@@ -398,35 +418,41 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         for (int i = 0; i < 32; ++i) o[i] = l != 0.f ? o[i] * inv : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(mine + lane * (D * 2) + (((c0 / 8 + i) ^ (lane & 7)) * 16)) =
+          *reinterpret_cast<uint4*>(mine + lane * (D * 2) + (((half * (D / 16) + c0 / 8 + i) ^ (lane & 7)) * 16)) =
               make_uint4(pack_out(o[8 * i], o[8 * i + 1], a.bf16), pack_out(o[8 * i + 2], o[8 * i + 3], a.bf16),
                          pack_out(o[8 * i + 4], o[8 * i + 5], a.bf16), pack_out(o[8 * i + 6], o[8 * i + 7], a.bf16));
       }
-      __syncwarp();
+    }
+    mk::bar_any(1 + pair, 64, false);
+    if (ok && x < tiles) {   // 16 of the 32 rows
+      const uint8_t* mine = smem + S::kQ + x * S::kTileBytes + (warp & 3) * 32 * (D * 2);
       constexpr int kLanes = D / 8;
 #pragma unroll 4
-      for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
-        const int mm = row0 + warp * 32 + i;
+      for (int i = 16 * half + lane / kLanes; i < 16 * half + 16; i += 32 / kLanes) {
+        const int mm = row0 + x * kTile + (warp & 3) * 32 + i;
         if (mm > row_last) continue;
         const long long at = (long long)(w.r0 + mm / group) * a.q_heads + h * group + mm % group;
         reinterpret_cast<uint4*>((uint16_t*)a.out + at * D)[lane % kLanes] =
             any ? *reinterpret_cast<const uint4*>(mine + i * (D * 2) + (((lane % kLanes) ^ (i & 7)) * 16)) : make_uint4(0, 0, 0, 0);
       }
-      __syncwarp();
-      if (m_row <= row_last) {
-        const long long at = (long long)(w.r0 + m_row / group) * a.q_heads + h * group + m_row % group;
-        if (s_nan) {
-          for (int d = 0; d < D; ++d)
-            if (sees_nan<F, P, kStep, D>(c, a, w, b, h, group, row0, row_last, m_row, d)) ((uint16_t*)a.out)[at * D + d] = 0x7fff;
-        }
-        if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m - kBase + log2f(l)) * 0.6931471805599453f;
+    }
+    mk::bar_any(1 + pair, 64, false);
+    if (ok && x < tiles && m_row <= row_last) {
+      const long long at = (long long)(w.r0 + m_row / group) * a.q_heads + h * group + m_row % group;
+      if (s_nan) {
+        for (int d = half * (D / 2); d < (half + 1) * (D / 2); ++d)
+          if (sees_nan<F, P, kStep, D>(c, a, w, b, h, group, row0, row_last, m_row, d)) ((uint16_t*)a.out)[at * D + d] = 0x7fff;
       }
+      if (a.lse && half == 0) a.lse[at] = l == 0.f ? -INFINITY : (m - kBase + log2f(l)) * 0.6931471805599453f;
     }
   } else if (warp < kRowWarps + kCodeWarps) {
     // ---- codes to f16
     mk::setmaxnreg_dec<kCodeRegs>();
-    constexpr int kLanes = D / 16, kRowsPer = kCodeWarps * 32 / kLanes;
-    const int ct = threadIdx.x - kRowWarps * 32, cc = ct % kLanes, cr = ct / kLanes;
+    // Two warps take K or V of every other step: what a step costs whatever its size
+    // (two waits, the fence to the tensor cores' view of shared memory) is a quarter
+    // as often on each warp's way.  With all eight on every K and V it set the pace.
+    constexpr int kLanes = D / 16, kRowsPer = 64 / kLanes;
+    const int which = (warp - kRowWarps) >> 1, kv = which >> 1, ct = threadIdx.x & 63, cc = ct % kLanes, cr = ct / kLanes;
     // 16 dimensions of a position, from 16 cc on: chunks 2 cc and 2 cc + 1 of its row(s)
     auto store = [&](uint8_t* base, int row, const uint4& codes, bool scaled, __half2 factor) {
       uint32_t e[8];
@@ -449,55 +475,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       *reinterpret_cast<uint4*>(at + (((ch + odd) ^ (row & 7)) * 16)) = odd ? odd4 : even4;
       *reinterpret_cast<uint4*>(at + (((ch + !odd) ^ (row & 7)) * 16)) = odd ? even4 : odd4;
     };
-    for (int j = first; j < last; ++j) {
-      const int i = j - first, st = i % kStages, raw = i % kRawStages;
+    for (int i = which & 1; first + i < last; i += 2) {
+      const int j = first + i, st = i % kStages, raw = i % kRawStages;
       const uint32_t phase = (i / kStages) & 1, raw_phase = (i / kRawStages) & 1;
-      bool ok = true;
-#pragma unroll
-      for (int kv = 0; ok && kv < 2; ++kv) {
-        ok = wait_warp(&raw_full[kv][raw], raw_phase) && wait_warp(&(kv ? v_empty : k_empty)[st], phase ^ 1);
-        if (!ok) break;
-        const bool whole = kv == 0 || (s_there[j % kMetaSlots] && j * kStep >= all.lo_max && (j + 1) * kStep <= all.hi_min);
-        const uint8_t* src = smem + S::kRaw + (kv * kRawStages + raw) * S::kCodes + 16 * cc;
-        uint8_t* dst = smem + (kv ? S::kV : S::kK) + st * S::kOperand;
-#pragma unroll
-        for (int row = cr; row < kStep; row += kRowsPer) {
-          uint4 v = *reinterpret_cast<const uint4*>(src + row * D);
-          if (!whole) {
-            // What no row sees may hold anything: its codes count as 0.  A NaN that
-            // only some rows see is taken out here and put back at the end.
-            const int p = j * kStep + row;
-            if (p >= all.hi || p < all.lo || s_ks[j % kMetaSlots][row / P] == 0.f) v = make_uint4(0, 0, 0, 0);
-            if constexpr (F::kTopExp == 8) {
-              const uint32_t b0 = nan_bytes(v.x), b1 = nan_bytes(v.y), b2 = nan_bytes(v.z), b3 = nan_bytes(v.w);
-              if (b0 | b1 | b2 | b3) {
-                s_nan = 1;
-                v.x &= ~((b0 >> 7) * 0xffu);
-                v.y &= ~((b1 >> 7) * 0xffu);
-                v.z &= ~((b2 >> 7) * 0xffu);
-                v.w &= ~((b3 >> 7) * 0xffu);
-              }
+      if (!wait_warp(&raw_full[kv][raw], raw_phase) || !wait_warp(&(kv ? v_empty : k_empty)[st], phase ^ 1)) break;
+      const bool whole = kv == 0 || (s_there[j % kMetaSlots] && j * kStep >= all.lo_max && (j + 1) * kStep <= all.hi_min);
+      const uint8_t* src = smem + S::kRaw + (kv * kRawStages + raw) * S::kCodes + 16 * cc;
+      uint8_t* dst = smem + (kv ? S::kV : S::kK) + st * S::kOperand;
+#pragma unroll 2
+      for (int row = cr; row < kStep; row += kRowsPer) {
+        uint4 v = *reinterpret_cast<const uint4*>(src + row * D);
+        if (!whole) {
+          // What no row sees may hold anything: its codes count as 0.  A NaN that
+          // only some rows see is taken out here and put back at the end.
+          const int p = j * kStep + row;
+          if (p >= all.hi || p < all.lo || s_ks[j % kMetaSlots][row / P] == 0.f) v = make_uint4(0, 0, 0, 0);
+          if constexpr (F::kTopExp == 8) {
+            const uint32_t b0 = nan_bytes(v.x), b1 = nan_bytes(v.y), b2 = nan_bytes(v.z), b3 = nan_bytes(v.w);
+            if (b0 | b1 | b2 | b3) {
+              s_nan = 1;
+              v.x &= ~((b0 >> 7) * 0xffu);
+              v.y &= ~((b1 >> 7) * 0xffu);
+              v.z &= ~((b2 >> 7) * 0xffu);
+              v.w &= ~((b3 >> 7) * 0xffu);
             }
           }
-          const float factor = kv ? s_vf[j % kMetaSlots][row / P] : 1.f;
-          store(dst, row, v, factor != 1.f, __float2half2_rn(factor));
         }
-        fence_async_shared();
-        mk::mbar_arrive(&(kv ? v_full : k_full)[st]);
-        __syncwarp();
-        if (lane == 0) mk::mbar_arrive(&raw_empty[kv][raw]);
+        const float factor = kv ? s_vf[j % kMetaSlots][row / P] : 1.f;
+        store(dst, row, v, factor != 1.f, __float2half2_rn(factor));
       }
-      if (!ok) break;
+      fence_async_shared();
+      mk::mbar_arrive(&(kv ? v_full : k_full)[st]);
+      __syncwarp();
+      if (lane == 0) mk::mbar_arrive(&raw_empty[kv][raw]);
     }
   } else {
     mk::setmaxnreg_dec<kMmaRegs>();
     if (warp == kCopyWarp) {
-      // ---- pages and copies: lane i, page i of a step
+      // ---- pages and copies.  The lanes hold the pages of kBatch steps, and of the
+      // next kBatch on their way: looked up step by step, table and then scales, the
+      // two latencies set the pace of the whole block (338 us a call).
+      constexpr int kBatch = 32 / kSub;
       struct Page { int id; float ks, vs; };
-      auto page_of = [&](int j) {
+      auto pages_from = [&](int j) {
         Page p{-1, 0.f, 0.f};
-        const int pos = j * kStep + lane * P;
-        if (j < last && lane < kSub && pos < all.hi && pos + P > all.lo) {
+        j += lane / kSub;
+        const int pos = j * kStep + lane % kSub * P;
+        if (j < last && pos < all.hi && pos + P > all.lo) {
           p.id = page_id(c, b, pos / P, a.status);
           if (p.id >= 0) {
             const float* sc = c.scales + p.id * c.scale_stride + h;
@@ -509,15 +533,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       };
       // rows of one sequence and head share the codes with its other items
       const uint64_t policy = w.tiles > 1 ? policy_evict_normal() : mk::policy_evict_first();
-      Page now = page_of(first), next = page_of(first + 1);
+      Page cur = pages_from(first), nxt = pages_from(first + kBatch);
+      int base = first;
       float vref = 0.f;
       bool ok = true;
       int done = first;
       for (int j = first; ok && j < last; ++j) {
         const int i = j - first, raw = i % kRawStages;
         const uint32_t phase = (i / kRawStages) & 1;
-        vref = fmaxf(vref, mk::warp_max(now.vs));
-        const bool there = __all_sync(0xffffffffu, lane >= kSub || now.id >= 0);
+        if (j - base == kBatch) {
+          base = j;
+          cur = nxt;
+          nxt = pages_from(base + kBatch);
+        }
+        Page now;   // lane i: page i % kSub of the step
+        const int from = (j - base) * kSub + lane % kSub;
+        now.id = __shfl_sync(0xffffffffu, cur.id, from);
+        now.ks = __shfl_sync(0xffffffffu, cur.ks, from);
+        now.vs = __shfl_sync(0xffffffffu, cur.vs, from);
+        float top = now.vs;
+#pragma unroll
+        for (int o = 1; o < kSub; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        vref = fmaxf(vref, top);
+        const bool there = __all_sync(0xffffffffu, now.id >= 0);
         for (int kv = 0; kv < 2; ++kv) {
           if (!(ok = wait_warp(&raw_empty[kv][raw], phase ^ 1))) break;
           if (lane < kSub) {
@@ -538,63 +576,71 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           __syncwarp();
           if (kv == 0) done = j + 1;
         }
-        now = next;
-        next = page_of(j + 2);
       }
       // no copy in flight when the block's memory is given away
       for (int j = max(first, done - kRawStages); j < done; ++j)
         for (int kv = 0; kv < 2; ++kv) wait_bar(&raw_full[kv][(j - first) % kRawStages], ((j - first) / kRawStages) & 1);
     }
-    if (warp == kMmaWarp || warp == kMmaWarp + 1) {
-      // ---- tensor cores: a tile's products, every one issued by one lane.  A warp
-      // gets an instruction in some ten cycles here, so what it does per step is
-      // kept short: one warp for both tiles took 391 us a call.
-      constexpr uint32_t kS = idesc_f16(kTile, kStep, false), kO = idesc_f16(kTile, D, true);
+    if (warp < kMmaWarp + 4) {
+      // ---- tensor cores: one product of one tile, issued by one lane.  A warp gets
+      // an instruction in some ten cycles here, so what it does per step is kept
+      // short: one warp for all four products took 391 us a call, one per tile 338.
       const uint32_t one = elect_one();
       const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0), smu = __shfl_sync(0xffffffffu, smem0, 0);
-      const int t = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0);
+      const int role = __shfl_sync(0xffffffffu, warp - kMmaWarp, 0), t = role & 1;
       const int nj = last - first, lo = (t ? j_lo[1] : j_lo[0]) - first, hi = (t ? j_hi[1] : j_hi[0]) - first;   // steps from the first on
-      const uint32_t q0 = desc_lo(smu + S::kQ + t * S::kTileBytes), k0 = desc_lo(smu + S::kK), v0 = desc_lo(smu + S::kV, kStep * 128);
-      const uint32_t ts = tmu + t * kTile, to = tmu + 2 * kTile + t * D;
-      bool ok = nj == 0 || wait_warp(&q_full, 0);
-      uint32_t p_phase = 0;   // bit i: of score buffer i
-      // two steps of scores ahead of the weights
+      bool ok = true;
+      uint32_t phase = 0;   // bit i: of score buffer i
+      if (role < 2) {
+        constexpr uint32_t kO = idesc_f16(kTile, D, true);
+        const uint32_t v0 = desc_lo(smu + S::kV, kStep * 128), ts = tmu + t * kTile, to = tmu + 2 * kTile + t * D;
 #pragma unroll 1
-      for (int i = -2; ok && i < nj; ++i) {
-        const int buf = (first + i) & 1, ks = (i + 2) % kStages, vs = i & (kStages - 1);
-        // what is there long before goes first: nothing but the weights is waited
-        // for right before their product
-        if (i >= 0 && !(ok = wait_warp(&v_full[vs], i / kStages & 1))) break;
-        if (i + 2 < nj && !(ok = wait_warp(&k_full[ks], (i + 2) / kStages & 1))) break;
-        if (i >= lo && i < hi) {
-          if (!(ok = wait_warp(&p_full[t][buf], p_phase >> buf & 1))) break;
-          p_phase ^= 1u << buf;
-          mk::tc_fence_after();
-          const uint32_t va = v0 + vs * (S::kOperand >> 4), pa = ts + buf * kStep, more = i > lo;
+        for (int i = 0; i < nj; ++i) {
+          const int buf = (first + i) & 1, st = i & (kStages - 1);
+          if (!(ok = wait_warp(&v_full[st], i / kStages & 1))) break;
+          if (i >= lo && i < hi) {
+            if (!(ok = wait_warp(&p_full[t][buf], phase >> buf & 1))) break;
+            phase ^= 1u << buf;
+            mk::tc_fence_after();
+            const uint32_t va = v0 + st * (S::kOperand >> 4), pa = ts + buf * kStep, more = i > lo;
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k) tc_mma_ts(one, to, pa + k * 8, va + k * (2048 >> 4), kDescHi, kO, k > 0 ? 1u : more);
-          tc_commit_one(one, &o_done[t]);
-          if (i + 1 == hi) tc_commit_one(one, &o_full[t]);
+            for (int k = 0; k < kStep / 16; ++k) tc_mma_ts(one, to, pa + k * 8, va + k * (2048 >> 4), kDescHi, kO, k > 0 ? 1u : more);
+            tc_commit_one(one, &o_done[t][buf]);
+            if (i + 1 == hi) tc_commit_one(one, &o_full[t]);
+          }
+          tc_commit_one(one, &v_empty[st]);
         }
-        if (i >= 0) tc_commit_one(one, &v_empty[vs]);
-        if (i + 2 >= lo && i + 2 < hi) {
-          mk::tc_fence_after();
-          const uint32_t ka = k0 + ks * (S::kOperand >> 4), d = ts + buf * kStep;
+      } else {
+        constexpr uint32_t kS = idesc_f16(kTile, kStep, false);
+        const uint32_t q0 = desc_lo(smu + S::kQ + t * S::kTileBytes), k0 = desc_lo(smu + S::kK), ts = tmu + t * kTile;
+        ok = nj == 0 || wait_warp(&q_full, 0);
+#pragma unroll 1
+        for (int i = 0; ok && i < nj; ++i) {
+          const int buf = (first + i) & 1, st = i & (kStages - 1);
+          if (!(ok = wait_warp(&k_full[st], i / kStages & 1))) break;
+          if (i >= lo && i < hi) {
+            if (i >= lo + 2) {   // the buffer's weights have been used
+              if (!(ok = wait_warp(&o_done[t][buf], phase >> buf & 1))) break;
+              phase ^= 1u << buf;
+            }
+            mk::tc_fence_after();
+            const uint32_t ka = k0 + st * (S::kOperand >> 4), d = ts + buf * kStep;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_ss(one, d, q0 + (k >> 2) * (kTile * 128 >> 4) + (k & 3) * 2, ka + (k >> 2) * (kStep * 128 >> 4) + (k & 3) * 2,
-                      kDescHi, kS, k > 0);
-          tc_commit_one(one, &s_full[t][buf]);
+            for (int k = 0; k < D / 16; ++k)
+              tc_mma_ss(one, d, q0 + (k >> 2) * (kTile * 128 >> 4) + (k & 3) * 2, ka + (k >> 2) * (kStep * 128 >> 4) + (k & 3) * 2,
+                        kDescHi, kS, k > 0);
+            tc_commit_one(one, &s_full[t][buf]);
+          }
+          tc_commit_one(one, &k_empty[st]);
         }
-        if (i + 2 < nj) tc_commit_one(one, &k_empty[ks]);
       }
       if (!ok) {   // nothing of this block's may be in flight when its memory is given away
         if (one) {
           report(a.status, MK_ERR_TIMEOUT);
-          mk::mbar_init(&o_drain[t], 1);
+          mk::mbar_init(&drain[role], 1);
           mk::fence_mbar_init();
-          mk::tc_commit(&o_drain[t]);
-          wait_bar(&o_drain[t], 0);
+          mk::tc_commit(&drain[role]);
+          wait_bar(&drain[role], 0);
         }
         __syncwarp();
       }
@@ -612,7 +658,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 
 template <class F, int P, int D>
 static int launch_prompt(const Cache& c, const Attend& a, cudaStream_t stream) {
-  constexpr int bytes = PromptSmem<D>::kBytes + 1024;
+  constexpr int bytes = PromptSmem<D>::kBytes;
   auto kernel = &attend_prompt_kernel<F, P, D>;
   static std::atomic<bool> ready[64];
   int dev = 0;

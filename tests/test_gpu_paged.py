@@ -450,3 +450,12 @@ def test_attend_nan_in_places_that_only_some_rows_see(rows):
     for pos, dim in marks:
         want[max(0, pos - (n - rows)):, dim] = True
     assert torch.equal(out.isnan().cpu(), want[:, None].expand(rows, hq, d))
+
+
+@pytest.mark.parametrize("seqs,hq,hk,rows,length", [(70, 4, 2, 1, 90), (150, 2, 1, 2, 200), (330, 8, 8, 1, 40), (100, 4, 4, 30, 60)])
+def test_attend_many_sequences(seqs, hq, hk, rows, length):
+    """More sequences than a warp looks over at once, and more items than warps."""
+    r = np.random.RandomState(seqs)
+    n = [int(x) for x in r.randint(0, rows + 1, seqs)]
+    lens = [k + int(x) for k, x in zip(n, r.randint(0, length, seqs))]
+    attend_case("fp8", BF, 16, 64, hq, hk, n, lens)
