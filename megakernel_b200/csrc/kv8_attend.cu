@@ -34,7 +34,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 // the warps of the grid (steps / run + items of them at most), and each warp
 // takes one part: no warp waits for the plan of a second one, and the warps of
 // an SM, whose loads share its bandwidth, hold much the same in sum.  (Equal
-// runs over item borders: 64 x ~1,150 positions 32.7 us, see DESIGN.)  More items
+// runs over item borders: 64 x ~1,150 positions 32.7 us, with parts 28.0.)  More items
 // than warps: one part each, taken in turn.  An item of one part is written
 // where it is computed; the parts of the others go to the workspace, and a
 // second small kernel joins them in order.
@@ -765,10 +765,11 @@ static int launch(const Cache& c, const Attend& a, void* work, size_t work_bytes
   // rows of a sequence, once per query head of the group, on average
   const long long per = ((long long)c.rows * (a.q_heads / c.kv_heads) + c.seqs - 1) / c.seqs;
   // Either kernel's time grows with the positions, which the host does not know:
-  // the rows' kernel with its items of 16 rows (4,096 positions: 0.2 to 0.25 us
-  // each), the prompts' with the waves of its blocks of 256 rows (78 to 92 us each).
-  // 32 sequences x 16 rows: 95 against 157 us, x 32 rows 241 against 158; one of
-  // 256 rows 51 against 83, four of 128 92 against 83 (head_dim 64, 16 / 8 heads).
+  // the rows' kernel with its items of 16 rows (4,096 positions: 0.11 to 0.25 us
+  // each), the prompts' with the waves of its blocks of 256 rows (65 to 91 us each).
+  // head_dim 64, 16 / 8 heads, 4,096 positions, rows' against prompts': 32 sequences
+  // x 16 rows 67 against 132 us, x 32 rows 162 against 132; 4 x 64 rows 38 against
+  // 67, x 256 rows 157 against 80; 64 x 32 rows 275 against 262.
   const long long kvs = (long long)c.seqs * c.kv_heads, items = (per + 15) / 16 * kvs;
   const long long waves = ((per + 255) / 256 * kvs + 147) / 148;
   if (items > 350 * waves) return attend_prompt(c, a, std::is_same<F, E4M3>::value ? MK_KV8_E4M3 : MK_KV8_INT8, P, D, stream);
