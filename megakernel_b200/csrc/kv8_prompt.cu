@@ -164,8 +164,9 @@ struct PromptSmem {
 // 2^-25 of the largest scale at worst), one rounding to 11 bits otherwise.
 //
 // What bounds it: shared memory, whose data path is busy 78 % of the time (operands
-// to the products 39 %, codes to f16 39 %), with two thirds of the issue slots, the
-// exponentials at 42 % and the tensor cores at 40 %.
+// to the products 39 %, the warps' own loads and stores, most of them the
+// converters', 39 %), with two thirds of the issue slots, the exponentials at 42 %
+// and the tensor cores at 40 %.
 template <class F, int P, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const Cache c, const Attend a) {
   using S = PromptSmem<D>;
